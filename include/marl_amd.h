@@ -1,7 +1,8 @@
 /*
  * marl_amd.h -- C ABI of libmarl_amd.so: batched Overcooked step / reset / featurize, the GAE
- * pass, and three small passes of the rollout / update loop (reward-event bookkeeping, action
- * sampling, the PPO minibatch loss) for MI355X (gfx950).
+ * pass, three small passes of the rollout / update loop (reward-event bookkeeping, action
+ * sampling, the PPO minibatch loss) and the low-bit passes of the policy's trunk (layers in 4-bit
+ * floating point, activations kept in 8 bits for the backward pass) for MI355X (gfx950).
  *
  * The reference (loganwoudstra/MARL) is pure Python and has no FFI of its own; the boundary
  * it does have is the duck-typed vector env returned by main.py:66-96 `make_vector_env`
@@ -258,6 +259,55 @@ int marl_ppo_loss(const float *d_logits, int num_samples, int num_actions, int r
                   double value_coef, float *d_grad_logits, float *d_grad_values, double *d_stats, void *d_workspace,
                   void *stream);
 size_t marl_ppo_loss_workspace_bytes(int num_samples);
+
+/* element types of the low-bit passes */
+enum {
+    MARL_F32 = 0,
+    MARL_BF16 = 1,
+    MARL_F16 = 2,
+    MARL_MXFP4 = 3           /* codes and scales as marl_mx_quantize writes them */
+};
+
+/*
+ * 4-bit microscaled floating point (MXFP4) for the layers of an acting policy (no counterpart in the
+ * reference, whose model.py:13-27 computes them in float32).
+ *
+ * A row of num_cols values is cut into blocks of 32, B = ceil(num_cols / 32) of them, the last one
+ * padded with zeros.  A block has
+ *   one scale byte  e + 127 with e = max(floor(log2 max|x|) - 2, -126), or 255 if the block holds an
+ *                   infinity or a NaN: it then reads as NaN throughout;
+ *   32 codes of 4 bits, the nearest of 0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives (sign in bit 3)
+ *                   to x / 2^e, ties to the even code, above 6 to 6; in 16 bytes, the lower half of a
+ *                   byte first.
+ *   d_codes   uint8 [num_rows][B][16], 16-byte aligned;   d_scales   uint8 [num_rows][B]
+ * d_x: num_rows rows of x_type (MARL_F32, MARL_BF16, MARL_F16), row_stride elements from one row to
+ * the next (0 = num_cols).  Fewer than 2^30 blocks a call; no rows is a call that does nothing.
+ */
+int marl_mx_quantize(const void *d_x, int x_type, int64_t num_rows, int num_cols, int64_t row_stride,
+                     uint8_t *d_codes, uint8_t *d_scales, void *stream);
+
+/* the values that codes and scales stand for: out_type [num_rows][num_cols] */
+int marl_mx_dequantize(const uint8_t *d_codes, const uint8_t *d_scales, int64_t num_rows, int num_cols,
+                       int out_type, void *d_out, void *stream);
+
+/*
+ * y = x W^T + bias, then max(y, 0) if relu (a NaN stays), with x and W in MXFP4 and sums in float32.
+ *   d_x       x_type MARL_F32 / MARL_BF16 / MARL_F16: rows as for marl_mx_quantize, quantised within
+ *             the call (d_x_scales NULL); MARL_MXFP4: codes, their scales in d_x_scales, row_stride 0
+ *   d_w_codes, d_w_scales   the weight [num_out][num_cols] as marl_mx_quantize writes it
+ *   d_bias    float32 [num_out] or NULL
+ *   d_y       y_type [num_rows][num_out]; MARL_MXFP4: the result is quantised as marl_mx_quantize would
+ *             quantise its float32 values, codes to d_y (16-byte aligned), scales to d_y_scales
+ *   d_workspace   marl_mx_linear_workspace_bytes() bytes, 16-byte aligned; that is 0 for num_cols up to
+ *             512 (d_workspace may then be NULL)
+ * The same call gives the same bits every time.  At most 2^22 output features; of rows of more than 512
+ * values at most 4,194,240.
+ */
+int marl_mx_linear(const void *d_x, const uint8_t *d_x_scales, int x_type, int64_t num_rows, int num_cols,
+                   int64_t row_stride, const uint8_t *d_w_codes, const uint8_t *d_w_scales, int num_out,
+                   const float *d_bias, int relu, void *d_y, uint8_t *d_y_scales, int y_type,
+                   void *d_workspace, void *stream);
+size_t marl_mx_linear_workspace_bytes(int x_type, int64_t num_rows, int num_cols, int num_out);
 
 #ifdef __cplusplus
 }

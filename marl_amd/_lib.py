@@ -20,6 +20,7 @@ EXPORTS = (
     "marl_env_import_state", "marl_gae", "marl_gae_workspace_bytes", "marl_row_sums",
     "marl_reward_events", "marl_reward_events_workspace_bytes", "marl_reward_events_noalloc", "marl_reward_events_many", "marl_reward_events_many_workspace_bytes", "marl_sample_categorical",
     "marl_ppo_loss", "marl_ppo_loss_workspace_bytes",
+    "marl_mx_quantize", "marl_mx_dequantize", "marl_mx_linear", "marl_mx_linear_workspace_bytes",
 )
 
 _lib = None
@@ -94,6 +95,15 @@ def lib() -> ctypes.CDLL:
                                 vp, vp, vp, vp, vp]
     L.marl_ppo_loss_workspace_bytes.restype = ctypes.c_size_t
     L.marl_ppo_loss_workspace_bytes.argtypes = [ci]
+    i64 = ctypes.c_int64
+    L.marl_mx_quantize.restype = ci
+    L.marl_mx_quantize.argtypes = [vp, ci, i64, ci, i64, vp, vp, vp]
+    L.marl_mx_dequantize.restype = ci
+    L.marl_mx_dequantize.argtypes = [vp, vp, i64, ci, ci, vp, vp]
+    L.marl_mx_linear.restype = ci
+    L.marl_mx_linear.argtypes = [vp, vp, ci, i64, ci, i64, vp, vp, ci, vp, ci, vp, vp, ci, vp, vp]
+    L.marl_mx_linear_workspace_bytes.restype = ctypes.c_size_t
+    L.marl_mx_linear_workspace_bytes.argtypes = [ci, i64, ci, ci]
     _lib = L
     return L
 

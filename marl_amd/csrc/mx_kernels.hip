@@ -1,0 +1,513 @@
+// 4-bit microscaled floating point (MXFP4): quantisation and the product of a policy layer, for gfx950.
+//
+//   block of 32 values x along a row:  e = max(floor(log2 max|x|) - 2, -126),  code = nearest e2m1 value of x / 2^e
+//   (0, .5, 1, 1.5, 2, 3, 4, 6 and negatives; ties to the even code, above 6 to 6), scale byte e + 127;
+//   a block that holds an infinity or a NaN gets scale byte 255 and reads as NaN throughout.
+//   y[m][n] = sum_k x[m][k] w[n][k] + bias[n], ReLU if asked; both operands in that form, sums in float32.
+//
+// The scale rule is the one of the microscaling formats' specification: a block's largest value lies in [4, 8) of its
+// scale, and what is above 6 becomes 6.
+#include "lowbit.h"
+
+namespace oc {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+constexpr int MX_FP4 = 4;  // operand format code of the scaled matrix instruction: e2m1
+
+// scale byte of a block from the bits of its largest |x|
+__device__ __forceinline__ uint32_t mx_scale_byte(uint32_t top) {
+    const uint32_t e = top >> 23;
+    return e == 255u ? 255u : e > 3u ? e - 2u : 1u;
+}
+
+// eight codes, low nibble first; v_cvt_scalef32_pk_fp4_f32 divides by the scale, rounds to nearest even and saturates
+__device__ __forceinline__ uint32_t mx_codes(const float (&v)[8], uint32_t byte) {
+    const float s = bits_f(byte << 23);
+    uint32_t c = 0;
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[0], v[1], s, 0);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[2], v[3], s, 1);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[4], v[5], s, 2);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[6], v[7], s, 3);
+    return byte == 255u ? 0u : c;
+}
+
+// ---------------------------------------------------------------------------------------------- quantise / read back
+
+// Four lanes per block, eight values each: the block's maximum is two DPP moves away and a wave reads 2 KiB of a row in
+// consecutive pieces.  Bound by memory.
+template <int TYPE>
+__global__ void __launch_bounds__(256)
+mx_quantize_kernel(const void* __restrict__ x, int64_t rows, int cols, int64_t pitch, int blocks,
+                   uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+    int64_t row;
+    int b, quarter;
+    split_block(blockIdx.x * 256 + threadIdx.x, (uint32_t)blocks, row, b, quarter);
+    if (row >= rows) return;  // whole quads leave together
+    float v[8];
+    load_eight<TYPE>(x, row * pitch + (int64_t)b * LB_BLOCK + quarter * 8, row * pitch + cols, v);
+    const uint32_t byte = mx_scale_byte(quad_max(abs_top(v)));
+    reinterpret_cast<uint32_t*>(codes)[(row * blocks + b) * 4 + quarter] = mx_codes(v, byte);
+    if (quarter == 0) scales[row * blocks + b] = (uint8_t)byte;
+}
+
+template <int TYPE>
+__global__ void __launch_bounds__(256)
+mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t rows, int cols,
+                     int blocks, void* __restrict__ out) {
+    int64_t row;
+    int b, quarter;
+    split_block(blockIdx.x * 256 + threadIdx.x, (uint32_t)blocks, row, b, quarter);
+    if (row >= rows) return;
+    const uint32_t c = reinterpret_cast<const uint32_t*>(codes)[(row * blocks + b) * 4 + quarter];
+    const float s = scale_value(scales[row * blocks + b]);
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        f32x2 p;
+        if (k == 0) p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 0);
+        else if (k == 1) p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 1);
+        else if (k == 2) p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 2);
+        else p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.0f, 3);
+        v[2 * k] = p.x * s;
+        v[2 * k + 1] = p.y * s;
+    }
+    store_eight<TYPE>(out, row * cols + (int64_t)b * LB_BLOCK + quarter * 8, row * cols + cols, v);
+}
+
+// ------------------------------------------------------------------------------------------------------ the product
+//
+// v_mfma_scale_f32_16x16x128_f8f6f4 takes 16 rows of 128 values from each operand; lane l holds row l % 16, block l / 16
+// of the four 32-value blocks, so a lane's 16 bytes of codes and its scale byte are exactly one stored block: fragments
+// need no rearrangement, neither from memory nor from LDS.  The weight is the first operand, so a lane's four results
+// are four output features of one row.  Rows of the weight are dealt to a wave's four tiles such that a lane's 4 x 4
+// results are 16 consecutive features: feature = 16 (lane / 16) + 4 tile + i.
+
+struct MxLinear {
+    const void* x;            // float rows, or codes
+    const uint8_t* x_scales;  // of codes
+    int64_t rows, pitch;      // pitch in elements, float rows only
+    int cols, blocks;
+    const uint8_t* w;
+    const uint8_t* w_scales;
+    int out;                  // output features
+    const float* bias;        // or NULL
+    int relu;
+    void* y;
+    uint8_t* y_scales;        // MXFP4 output only
+    float* part;              // [splits][rows][out] partial sums (mx_stream_kernel with splits > 1)
+    int splits;
+};
+
+__device__ __forceinline__ f32x4 mx_mfma(u32x4 a, u32x4 b, f32x4 c, int ks, int sa, int sb) {
+    const i32x8 A = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};
+    const i32x8 B = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
+    switch (ks) {  // a constant after unrolling: which byte of the scale words is used
+        case 0: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, c, MX_FP4, MX_FP4, 0, sa, 0, sb);
+        case 1: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, c, MX_FP4, MX_FP4, 1, sa, 1, sb);
+        case 2: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, c, MX_FP4, MX_FP4, 2, sa, 2, sb);
+        default: return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(A, B, c, MX_FP4, MX_FP4, 3, sa, 3, sb);
+    }
+}
+
+// Results of one lane: row m, features n .. n + 15 (v[4 t + i] is feature n + 4 t + i).  All lanes of the wave come
+// here together (the MXFP4 form exchanges maxima between lanes); `live` says whether row m exists.
+template <int OUT>
+__device__ __forceinline__ void mx_store(const MxLinear& P, int64_t m, bool live, int n, float (&v)[16]) {
+    if (P.relu) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] = v[k] < 0.0f ? 0.0f : v[k];  // a NaN stays
+    }
+    if constexpr (OUT == MARL_MXFP4) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            if (n + k >= P.out) v[k] = 0.0f;
+            top = max(top, f_bits(v[k]) & 0x7FFFFFFFu);
+        }
+        top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));  // the lane with the block's other half
+        const int yb = (P.out + LB_BLOCK - 1) / LB_BLOCK, b = n / LB_BLOCK;
+        if (!live || b >= yb) return;
+        const uint32_t byte = mx_scale_byte(top);
+        float lo[8], hi[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) { lo[k] = v[k]; hi[k] = v[8 + k]; }
+        *reinterpret_cast<u32x2*>(static_cast<uint8_t*>(P.y) + (m * yb + b) * 16 + (n & 16) / 2) = u32x2{mx_codes(lo, byte), mx_codes(hi, byte)};
+        if ((n & 16) == 0) P.y_scales[m * yb + b] = (uint8_t)byte;
+    } else {
+        if (!live || n >= P.out) return;
+        const int64_t at = m * P.out + n, end = m * P.out + P.out;
+        float lo[8], hi[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) { lo[k] = v[k]; hi[k] = v[8 + k]; }
+        store_eight<OUT>(P.y, at, end, lo);
+        store_eight<OUT>(P.y, at + 8, end, hi);
+    }
+}
+
+// one 16-byte block of codes, zeros (with any scale) behind the last row or block
+__device__ __forceinline__ u32x4 mx_block(const uint8_t* codes, int64_t row, int64_t rows, int b, int blocks) {
+    if (row < rows && b < blocks) return *reinterpret_cast<const u32x4*>(codes + (row * blocks + b) * 16);
+    return u32x4{0, 0, 0, 0};
+}
+__device__ __forceinline__ uint32_t mx_scale(const uint8_t* scales, int64_t row, int64_t rows, int b, int blocks) {
+    return row < rows && b < blocks ? scales[row * blocks + b] : 127u;
+}
+
+// Many rows of at most 512 values: a wave keeps its 64 features' whole weight in registers (at most 64 of them) and the
+// workgroup walks row tiles of 32, which its threads quantise into LDS on the way (four lanes per block, as above).
+// Bound by memory: rows in, results out, the weight once per workgroup.
+constexpr int MX_TILE = 32;
+
+template <int KS, int IN, int OUT>
+__global__ void __launch_bounds__(512)
+mx_rows_kernel(MxLinear P) {
+    constexpr int NB = KS * 4;             // blocks of a row, padded to whole matrix instructions
+    constexpr int PITCH = NB * 16 + 16;    // LDS bytes per row of codes; the 16 keep a wave's rows apart in the banks
+    __shared__ __align__(16) uint8_t codes[2][MX_TILE][PITCH];
+    __shared__ __align__(16) uint8_t scales[2][MX_TILE][16];  // [block % 4][block / 4]: a lane's scales are one word
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+    const int n0 = (blockIdx.y * (blockDim.x >> 6) + wave) * 64;
+    u32x4 w[4][KS];
+    int ws[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        const int n = n0 + 16 * (r >> 2) + 4 * t + (r & 3);
+        uint32_t s = 0;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            w[t][ks] = mx_block(P.w, n, P.out, ks * 4 + g, P.blocks);
+            s |= mx_scale(P.w_scales, n, P.out, ks * 4 + g, P.blocks) << (8 * ks);
+        }
+        ws[t] = (int)s;
+    }
+    float bias[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) bias[k] = P.bias && n0 + 16 * g + k < P.out ? P.bias[n0 + 16 * g + k] : 0.0f;
+
+    const int64_t tiles = (P.rows + MX_TILE - 1) / MX_TILE;
+    int buf = 0;
+    for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, buf ^= 1) {
+        if constexpr (IN == MARL_MXFP4) {
+            for (int it = threadIdx.x; it < MX_TILE * NB; it += blockDim.x) {
+                const int row = it / NB, b = it % NB;
+                const int64_t m = tile * MX_TILE + row;
+                *reinterpret_cast<u32x4*>(&codes[buf][row][b * 16]) = mx_block(static_cast<const uint8_t*>(P.x), m, P.rows, b, P.blocks);
+                scales[buf][row][(b & 3) * 4 + (b >> 2)] = (uint8_t)mx_scale(P.x_scales, m, P.rows, b, P.blocks);
+            }
+        } else {
+            for (int it = threadIdx.x; it < MX_TILE * NB * 4; it += blockDim.x) {
+                const int quarter = it & 3, b = (it >> 2) % NB, row = (it >> 2) / NB;
+                const int64_t m = tile * MX_TILE + row;
+                float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+                if (m < P.rows) load_eight<IN>(P.x, m * P.pitch + (int64_t)b * LB_BLOCK + quarter * 8, m * P.pitch + P.cols, v);
+                const uint32_t byte = mx_scale_byte(quad_max(abs_top(v)));
+                *reinterpret_cast<uint32_t*>(&codes[buf][row][b * 16 + quarter * 4]) = mx_codes(v, byte);
+                if (quarter == 0) scales[buf][row][(b & 3) * 4 + (b >> 2)] = (uint8_t)byte;
+            }
+        }
+        __syncthreads();  // one barrier a tile: the other buffer is free once every wave has come here
+#pragma unroll
+        for (int rt = 0; rt < MX_TILE / 16; ++rt) {
+            f32x4 acc[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) acc[t] = f32x4{0, 0, 0, 0};
+            const int xs = *reinterpret_cast<const int*>(&scales[buf][rt * 16 + r][g * 4]);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const u32x4 x = *reinterpret_cast<const u32x4*>(&codes[buf][rt * 16 + r][(ks * 4 + g) * 16]);
+#pragma unroll
+                for (int t = 0; t < 4; ++t) acc[t] = mx_mfma(w[t][ks], x, acc[t], ks, ws[t], xs);
+            }
+            float v[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) v[k] = acc[k >> 2][k & 3] + bias[k];
+            const int64_t m = tile * MX_TILE + rt * 16 + r;
+            mx_store<OUT>(P, m, m < P.rows, n0 + 16 * g, v);
+        }
+    }
+}
+
+// Any length: x is quantised already.  A workgroup has 64 features and 16 RM rows; its four waves take every fourth
+// step of 128 values of its share of the row and add their sums through LDS.  With few rows the row is also split over
+// workgroups (grid z): the weight, read once, is what such a call costs, and it takes many loads in flight.
+template <int RM, int OUT>
+__global__ void __launch_bounds__(256)
+mx_stream_kernel(MxLinear P) {
+    __shared__ float sums[3][RM][64][17];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+    const int n0 = blockIdx.x * 64;
+    const int64_t m0 = (int64_t)blockIdx.y * (16 * RM);
+    const int steps = (P.blocks + 3) / 4;
+    const int per = (steps + P.splits - 1) / P.splits;
+    const int first = blockIdx.z * per, last = min(steps, first + per);
+    f32x4 acc[RM][4];
+#pragma unroll
+    for (int q = 0; q < RM; ++q)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[q][t] = f32x4{0, 0, 0, 0};
+    const uint8_t* xc = static_cast<const uint8_t*>(P.x);
+    for (int s = first + wave; s < last; s += 4) {
+        const int b = s * 4 + g;
+        u32x4 w[4], x[RM];
+        int ws[4], xs[RM];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const int n = n0 + 16 * (r >> 2) + 4 * t + (r & 3);
+            w[t] = mx_block(P.w, n, P.out, b, P.blocks);
+            ws[t] = (int)mx_scale(P.w_scales, n, P.out, b, P.blocks);
+        }
+#pragma unroll
+        for (int q = 0; q < RM; ++q) {
+            x[q] = mx_block(xc, m0 + q * 16 + r, P.rows, b, P.blocks);
+            xs[q] = (int)mx_scale(P.x_scales, m0 + q * 16 + r, P.rows, b, P.blocks);
+        }
+#pragma unroll
+        for (int q = 0; q < RM; ++q)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) acc[q][t] = mx_mfma(w[t], x[q], acc[q][t], 0, ws[t], xs[q]);
+    }
+    if (wave) {
+#pragma unroll
+        for (int q = 0; q < RM; ++q)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) sums[wave - 1][q][lane][k] = acc[q][k >> 2][k & 3];
+    }
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int q = 0; q < RM; ++q) {
+        float v[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] = ((acc[q][k >> 2][k & 3] + sums[0][q][lane][k]) + sums[1][q][lane][k]) + sums[2][q][lane][k];
+        const int64_t m = m0 + q * 16 + r;
+        const int n = n0 + 16 * g;
+        if (P.splits > 1) {
+            if (m >= P.rows) continue;
+            float* part = P.part + ((int64_t)blockIdx.z * P.rows + m) * P.out;
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+                if (n + k < P.out) part[n + k] = v[k];
+        } else {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) v[k] += P.bias && n + k < P.out ? P.bias[n + k] : 0.0f;
+            mx_store<OUT>(P, m, m < P.rows, n, v);
+        }
+    }
+}
+
+// Sums of the splits in their order, then bias, ReLU and the output's type.  Four lanes per 32 features, as in quantising.
+template <int OUT>
+__global__ void __launch_bounds__(256)
+mx_join_kernel(MxLinear P) {
+    const int yb = (P.out + LB_BLOCK - 1) / LB_BLOCK;
+    int64_t m;
+    int b, quarter;
+    split_block(blockIdx.x * 256 + threadIdx.x, (uint32_t)yb, m, b, quarter);
+    if (m >= P.rows) return;
+    const int n = b * LB_BLOCK + quarter * 8;
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+    for (int s = 0; s < P.splits; ++s) {
+        const int64_t row = ((int64_t)s * P.rows + m) * P.out;
+        float p[8];
+        load_eight<MARL_F32>(P.part, row + n, row + P.out, p);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] += p[k];
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        if (n + k >= P.out) { v[k] = 0.0f; continue; }
+        if (P.bias) v[k] += P.bias[n + k];
+        if (P.relu) v[k] = v[k] < 0.0f ? 0.0f : v[k];
+    }
+    if constexpr (OUT == MARL_MXFP4) {
+        const uint32_t byte = mx_scale_byte(quad_max(abs_top(v)));
+        reinterpret_cast<uint32_t*>(P.y)[(m * yb + b) * 4 + quarter] = mx_codes(v, byte);
+        if (quarter == 0) P.y_scales[m * yb + b] = (uint8_t)byte;
+    } else {
+        store_eight<OUT>(P.y, m * P.out + n, m * P.out + P.out, v);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------ host
+
+constexpr int MX_ROWS_COLS = 512;   // longest row of mx_rows_kernel: four matrix instructions
+
+static hipError_t launch_quantize(const void* x, int type, int64_t rows, int cols, int64_t pitch, uint8_t* codes,
+                                  uint8_t* scales, hipStream_t stream) {
+    const int blocks = (int)lb_blocks(cols);
+    auto kernel = type == MARL_F32 ? mx_quantize_kernel<MARL_F32> : type == MARL_BF16 ? mx_quantize_kernel<MARL_BF16> : mx_quantize_kernel<MARL_F16>;
+    hipLaunchKernelGGL(kernel, dim3(block_grid(rows, cols)), dim3(256), 0, stream, x, rows, cols, pitch, blocks, codes, scales);
+    return hipGetLastError();
+}
+
+template <int KS, int IN>
+static void (*rows_kernel_out(int out))(MxLinear) {
+    switch (out) {
+        case MARL_F32: return mx_rows_kernel<KS, IN, MARL_F32>;
+        case MARL_BF16: return mx_rows_kernel<KS, IN, MARL_BF16>;
+        case MARL_F16: return mx_rows_kernel<KS, IN, MARL_F16>;
+        default: return mx_rows_kernel<KS, IN, MARL_MXFP4>;
+    }
+}
+template <int KS>
+static void (*rows_kernel_in(int in, int out))(MxLinear) {
+    switch (in) {
+        case MARL_F32: return rows_kernel_out<KS, MARL_F32>(out);
+        case MARL_BF16: return rows_kernel_out<KS, MARL_BF16>(out);
+        case MARL_F16: return rows_kernel_out<KS, MARL_F16>(out);
+        default: return rows_kernel_out<KS, MARL_MXFP4>(out);
+    }
+}
+static void (*rows_kernel(int ks, int in, int out))(MxLinear) {
+    switch (ks) {
+        case 1: return rows_kernel_in<1>(in, out);
+        case 2: return rows_kernel_in<2>(in, out);
+        case 3: return rows_kernel_in<3>(in, out);
+        default: return rows_kernel_in<4>(in, out);
+    }
+}
+template <int RM>
+static void (*stream_kernel(int out))(MxLinear) {
+    switch (out) {
+        case MARL_F32: return mx_stream_kernel<RM, MARL_F32>;
+        case MARL_BF16: return mx_stream_kernel<RM, MARL_BF16>;
+        case MARL_F16: return mx_stream_kernel<RM, MARL_F16>;
+        default: return mx_stream_kernel<RM, MARL_MXFP4>;
+    }
+}
+
+// How a call over rows longer than MX_ROWS_COLS is cut: row groups per workgroup and splits of the row.
+struct MxCut { int rm; int splits; };
+static MxCut mx_cut(int64_t rows, int64_t cols, int out) {
+    MxCut c;
+    c.rm = rows <= 16 ? 1 : 4;
+    const int64_t steps = ((int64_t)lb_blocks(cols) + 3) / 4;
+    const int64_t groups = ((out + 63) / 64) * ((rows + 16 * c.rm - 1) / (16 * c.rm));
+    const int64_t most = steps / 8 < 1 ? 1 : steps / 8;  // at least two steps for each of a workgroup's four waves
+    int64_t s = 1024 / groups;                           // four workgroups per compute unit
+    c.splits = (int)(s < 1 ? 1 : s > most ? most : s);
+    return c;
+}
+static size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
+
+static hipError_t launch_linear(const MxLinear& P0, int x_type, int out_type, uint8_t* ws, hipStream_t stream) {
+    MxLinear P = P0;
+    if (P.cols <= MX_ROWS_COLS) {
+        const int waves = P.out >= 512 ? 8 : (P.out + 63) / 64;
+        const int ky = (P.out + 64 * waves - 1) / (64 * waves);
+        const int64_t tiles = (P.rows + MX_TILE - 1) / MX_TILE;
+        const int64_t resident = 256 * (16 / waves);  // four waves per SIMD
+        const int64_t gx = tiles < resident ? tiles : resident;
+        hipLaunchKernelGGL(rows_kernel((P.blocks + 3) / 4, x_type, out_type), dim3((uint32_t)gx, ky), dim3(64 * waves), 0, stream, P);
+        return hipGetLastError();
+    }
+    const MxCut c = mx_cut(P.rows, P.cols, P.out);
+    if (x_type != MARL_MXFP4) {
+        uint8_t* codes = ws;
+        ws += up16((size_t)P.rows * P.blocks * 16);
+        uint8_t* scales = ws;
+        ws += up16((size_t)P.rows * P.blocks);
+        hipError_t e = launch_quantize(P.x, x_type, P.rows, P.cols, P.pitch, codes, scales, stream);
+        if (e != hipSuccess) return e;
+        P.x = codes;
+        P.x_scales = scales;
+    }
+    P.splits = c.splits;
+    P.part = reinterpret_cast<float*>(ws);
+    const dim3 grid((P.out + 63) / 64, (uint32_t)((P.rows + 16 * c.rm - 1) / (16 * c.rm)), c.splits);
+    hipLaunchKernelGGL(c.rm == 1 ? stream_kernel<1>(out_type) : stream_kernel<4>(out_type), grid, dim3(256), 0, stream, P);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || c.splits == 1) return e;
+    auto join = out_type == MARL_F32 ? mx_join_kernel<MARL_F32> : out_type == MARL_BF16 ? mx_join_kernel<MARL_BF16>
+              : out_type == MARL_F16 ? mx_join_kernel<MARL_F16> : mx_join_kernel<MARL_MXFP4>;
+    hipLaunchKernelGGL(join, dim3(block_grid(P.rows, P.out)), dim3(256), 0, stream, P);
+    return hipGetLastError();
+}
+
+static int hip_result(hipError_t e, const char* what) {
+    if (e == hipSuccess) return MARL_OK;
+    return set_error(MARL_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
+}
+
+}  // namespace oc
+
+using namespace oc;
+
+extern "C" int marl_mx_quantize(const void* d_x, int x_type, int64_t num_rows, int num_cols, int64_t row_stride,
+                                uint8_t* d_codes, uint8_t* d_scales, void* stream) {
+    if (num_rows < 0 || num_cols <= 0) return set_error(MARL_ERR_INVALID, "num_rows must not be negative and num_cols must be positive");
+    if (x_type != MARL_F32 && x_type != MARL_BF16 && x_type != MARL_F16)
+        return set_error(MARL_ERR_INVALID, "x_type must be MARL_F32, MARL_BF16 or MARL_F16");
+    if (num_rows == 0) return MARL_OK;
+    if (!d_x || !d_codes || !d_scales) return set_error(MARL_ERR_INVALID, "NULL argument to marl_mx_quantize");
+    if (row_stride == 0) row_stride = num_cols;
+    if (row_stride < num_cols) return set_error(MARL_ERR_INVALID, "row_stride is smaller than num_cols");
+    if (((uintptr_t)d_x & (lb_type_bytes(x_type) - 1)) != 0 || ((uintptr_t)d_codes & 15u) != 0)
+        return set_error(MARL_ERR_INVALID, "d_x must be aligned to its elements, d_codes to 16 bytes");
+    if (too_many_blocks(num_rows, num_cols)) return set_error(MARL_ERR_INVALID, "2^30 or more blocks of 32 values in one call");
+    return hip_result(launch_quantize(d_x, x_type, num_rows, num_cols, row_stride, d_codes, d_scales, reinterpret_cast<hipStream_t>(stream)),
+                      "MXFP4 quantisation launch");
+}
+
+extern "C" int marl_mx_dequantize(const uint8_t* d_codes, const uint8_t* d_scales, int64_t num_rows, int num_cols, int out_type,
+                                  void* d_out, void* stream) {
+    if (num_rows < 0 || num_cols <= 0) return set_error(MARL_ERR_INVALID, "num_rows must not be negative and num_cols must be positive");
+    if (out_type != MARL_F32 && out_type != MARL_BF16 && out_type != MARL_F16)
+        return set_error(MARL_ERR_INVALID, "out_type must be MARL_F32, MARL_BF16 or MARL_F16");
+    if (num_rows == 0) return MARL_OK;
+    if (!d_codes || !d_scales || !d_out) return set_error(MARL_ERR_INVALID, "NULL argument to marl_mx_dequantize");
+    if (((uintptr_t)d_codes & 15u) != 0 || ((uintptr_t)d_out & (lb_type_bytes(out_type) - 1)) != 0)
+        return set_error(MARL_ERR_INVALID, "d_codes must be 16-byte aligned, d_out aligned to its elements");
+    if (too_many_blocks(num_rows, num_cols)) return set_error(MARL_ERR_INVALID, "2^30 or more blocks of 32 values in one call");
+    const int blocks = (int)lb_blocks(num_cols);
+    auto kernel = out_type == MARL_F32 ? mx_dequantize_kernel<MARL_F32> : out_type == MARL_BF16 ? mx_dequantize_kernel<MARL_BF16> : mx_dequantize_kernel<MARL_F16>;
+    hipLaunchKernelGGL(kernel, dim3(block_grid(num_rows, num_cols)), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), d_codes, d_scales, num_rows, num_cols, blocks, d_out);
+    return hip_result(hipGetLastError(), "MXFP4 read-back launch");
+}
+
+extern "C" size_t marl_mx_linear_workspace_bytes(int x_type, int64_t num_rows, int num_cols, int num_out) {
+    if (num_rows <= 0 || num_cols <= MX_ROWS_COLS || num_out <= 0) return 0;
+    const MxCut c = mx_cut(num_rows, num_cols, num_out);
+    size_t n = 0;
+    if (x_type != MARL_MXFP4) n += up16((size_t)num_rows * lb_blocks(num_cols) * 16) + up16((size_t)num_rows * lb_blocks(num_cols));
+    if (c.splits > 1) n += (size_t)c.splits * num_rows * num_out * sizeof(float);
+    return n;
+}
+
+extern "C" int marl_mx_linear(const void* d_x, const uint8_t* d_x_scales, int x_type, int64_t num_rows, int num_cols, int64_t row_stride,
+                              const uint8_t* d_w_codes, const uint8_t* d_w_scales, int num_out, const float* d_bias, int relu,
+                              void* d_y, uint8_t* d_y_scales, int y_type, void* d_workspace, void* stream) {
+    if (num_rows < 0 || num_cols <= 0 || num_out <= 0)
+        return set_error(MARL_ERR_INVALID, "num_rows must not be negative, num_cols and num_out must be positive");
+    if (x_type < MARL_F32 || x_type > MARL_MXFP4 || y_type < MARL_F32 || y_type > MARL_MXFP4)
+        return set_error(MARL_ERR_INVALID, "x_type and y_type must be MARL_F32, MARL_BF16, MARL_F16 or MARL_MXFP4");
+    if (num_rows == 0) return MARL_OK;
+    if (!d_x || !d_w_codes || !d_w_scales || !d_y) return set_error(MARL_ERR_INVALID, "NULL argument to marl_mx_linear");
+    if ((x_type == MARL_MXFP4) != (d_x_scales != nullptr) || (y_type == MARL_MXFP4) != (d_y_scales != nullptr))
+        return set_error(MARL_ERR_INVALID, "d_x_scales / d_y_scales belong to MARL_MXFP4 operands, and only to them");
+    if (x_type == MARL_MXFP4 ? row_stride != 0 : row_stride != 0 && row_stride < num_cols)
+        return set_error(MARL_ERR_INVALID, "row_stride is smaller than num_cols (0 with MARL_MXFP4 rows, which are packed)");
+    const size_t xa = x_type == MARL_MXFP4 ? 16 : lb_type_bytes(x_type), ya = y_type == MARL_MXFP4 ? 16 : lb_type_bytes(y_type);
+    if (((uintptr_t)d_x & (xa - 1)) != 0 || ((uintptr_t)d_y & (ya - 1)) != 0 || ((uintptr_t)d_w_codes & 15u) != 0 ||
+        ((uintptr_t)d_bias & 3u) != 0 || ((uintptr_t)d_workspace & 15u) != 0)
+        return set_error(MARL_ERR_INVALID, "codes and the workspace must be 16-byte aligned, the others aligned to their elements");
+    if (too_many_blocks(num_rows, num_cols) || too_many_blocks(num_rows, num_out) || num_out > (1 << 22))
+        return set_error(MARL_ERR_INVALID, "fewer than 2^30 blocks of 32 values on either side and at most 2^22 output features in one call");
+    if (num_cols > MX_ROWS_COLS && num_rows > (int64_t)65535 * 64)
+        return set_error(MARL_ERR_INVALID, "of rows of more than 512 values at most 4,194,240 in one call");
+    if (marl_mx_linear_workspace_bytes(x_type, num_rows, num_cols, num_out) != 0 && !d_workspace)
+        return set_error(MARL_ERR_INVALID, "this size needs d_workspace (marl_mx_linear_workspace_bytes bytes)");
+    MxLinear P;
+    P.x = d_x; P.x_scales = d_x_scales;
+    P.rows = num_rows; P.pitch = row_stride ? row_stride : num_cols;
+    P.cols = num_cols; P.blocks = (int)lb_blocks(num_cols);
+    P.w = d_w_codes; P.w_scales = d_w_scales; P.out = num_out;
+    P.bias = d_bias; P.relu = relu != 0;
+    P.y = d_y; P.y_scales = d_y_scales;
+    P.part = nullptr; P.splits = 1;
+    return hip_result(launch_linear(P, x_type, y_type, static_cast<uint8_t*>(d_workspace), reinterpret_cast<hipStream_t>(stream)),
+                      "MXFP4 linear launch");
+}
