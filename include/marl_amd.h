@@ -309,6 +309,43 @@ int marl_mx_linear(const void *d_x, const uint8_t *d_x_scales, int x_type, int64
                    void *d_workspace, void *stream);
 size_t marl_mx_linear_workspace_bytes(int x_type, int64_t num_rows, int num_cols, int num_out);
 
+/*
+ * Activations kept in 8 bits from the forward to the backward pass of an update (no counterpart in
+ * the reference, whose autograd keeps them in float32: agents/MAPPO.py:167-209).
+ *
+ * A row is cut into blocks of 32 as above.  A block has
+ *   one scale byte  e + 127 with e the smallest for which no rounded |x| / 2^e passes 127 (nonnegative:
+ *                   255), at least -126, at most 121 (120: 127 or 255 of them are still finite, and
+ *                   what is above them is cut to them); 255 if the block holds an infinity or a NaN: it then reads
+ *                   as NaN throughout;
+ *   one code a value  round(x / 2^e) + 128, ties to even; nonnegative: round(x / 2^e), where a negative
+ *                   value counts as 0 and a positive one never gets code 0.
+ *   d_codes   uint8 [num_rows][num_cols];   d_scales   uint8 [num_rows][B]
+ * Whole numbers up to 127 are kept exactly.  d_x as for marl_mx_quantize.
+ */
+int marl_act_compress(const void *d_x, int x_type, int64_t num_rows, int num_cols, int64_t row_stride,
+                      int nonnegative, uint8_t *d_codes, uint8_t *d_scales, void *stream);
+
+/* the values that codes and scales stand for: out_type [num_rows][num_cols] */
+int marl_act_dequantize(const uint8_t *d_codes, const uint8_t *d_scales, int64_t num_rows, int num_cols,
+                        int nonnegative, int out_type, void *d_out, void *stream);
+
+/*
+ * The parameter gradients of y = relu?(x W^T + b) from the gradient of y and the kept x:
+ *   g = d_grad, cut to 0 where d_mask_codes (the codes of y, kept in the nonnegative form; NULL: no
+ *       ReLU) is 0; what is cut does not count, whatever it holds
+ *   d_grad_weight float32 [num_out][num_cols] = g^T x,  d_grad_bias float32 [num_out] = column sums of g
+ *   d_masked_grad grad_type [num_rows][num_out] = g (with d_mask_codes only, and not d_grad itself)
+ * d_grad: grad_type [num_rows][num_out]; d_codes, d_scales, nonnegative: x as marl_act_compress wrote it.
+ * Sums in float32, each product exact to float32 whatever grad_type; the same call gives the same bits
+ * every time.  d_workspace: marl_act_weight_grad_workspace_bytes() bytes, 16-byte aligned.
+ */
+int marl_act_weight_grad(const void *d_grad, int grad_type, int64_t num_rows, int num_out,
+                         const uint8_t *d_codes, const uint8_t *d_scales, int num_cols, int nonnegative,
+                         const uint8_t *d_mask_codes, void *d_masked_grad, float *d_grad_weight,
+                         float *d_grad_bias, void *d_workspace, void *stream);
+size_t marl_act_weight_grad_workspace_bytes(int64_t num_rows, int num_out, int num_cols);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,6 +21,7 @@ EXPORTS = (
     "marl_reward_events", "marl_reward_events_workspace_bytes", "marl_reward_events_noalloc", "marl_reward_events_many", "marl_reward_events_many_workspace_bytes", "marl_sample_categorical",
     "marl_ppo_loss", "marl_ppo_loss_workspace_bytes",
     "marl_mx_quantize", "marl_mx_dequantize", "marl_mx_linear", "marl_mx_linear_workspace_bytes",
+    "marl_act_compress", "marl_act_dequantize", "marl_act_weight_grad", "marl_act_weight_grad_workspace_bytes",
 )
 
 _lib = None
@@ -104,6 +105,14 @@ def lib() -> ctypes.CDLL:
     L.marl_mx_linear.argtypes = [vp, vp, ci, i64, ci, i64, vp, vp, ci, vp, ci, vp, vp, ci, vp, vp]
     L.marl_mx_linear_workspace_bytes.restype = ctypes.c_size_t
     L.marl_mx_linear_workspace_bytes.argtypes = [ci, i64, ci, ci]
+    L.marl_act_compress.restype = ci
+    L.marl_act_compress.argtypes = [vp, ci, i64, ci, i64, ci, vp, vp, vp]
+    L.marl_act_dequantize.restype = ci
+    L.marl_act_dequantize.argtypes = [vp, vp, i64, ci, ci, ci, vp, vp]
+    L.marl_act_weight_grad.restype = ci
+    L.marl_act_weight_grad.argtypes = [vp, ci, i64, ci, vp, vp, ci, ci, vp, vp, vp, vp, vp, vp]
+    L.marl_act_weight_grad_workspace_bytes.restype = ctypes.c_size_t
+    L.marl_act_weight_grad_workspace_bytes.argtypes = [i64, ci, ci]
     _lib = L
     return L
 

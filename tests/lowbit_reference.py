@@ -52,10 +52,10 @@ def act8(x, positive):
     e = _floor_log2(top) - (7 if positive else 6)
     with np.errstate(invalid="ignore"):
         e = np.where(np.rint(np.where(bad, 0.0, top) / np.exp2(e.astype(np.float64))) > most, e + 1, e)
-    e = np.maximum(e, -126)
+    e = np.clip(e, -126, 120 if positive else 121)  # the largest scale of which `most` are finite in float32
     scale = np.exp2(e.astype(np.float64))[..., None]
     with np.errstate(invalid="ignore", over="ignore"):
-        code = np.rint(np.where(np.isfinite(b), b, 0.0) / scale)
+        code = np.clip(np.rint(np.where(np.isfinite(b), b, 0.0) / scale), -most, most)
     if positive:
         code = np.where(b > 0, np.maximum(code, 1), code)
     values = np.where(bad[..., None], np.nan, code * scale)
