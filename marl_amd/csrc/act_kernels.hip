@@ -94,7 +94,7 @@ act_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restri
 // The sum runs over the rows, 32 of them a step of v_mfma_f32_16x16x32_bf16.  x is a bfloat16 exactly.  A float32 g is
 // the sum of three bfloat16 numbers exactly (its 24 bits cut into eights), so three products with float32 sums give
 // float32's accuracy; a float16 g needs two and a bfloat16 g one.
-// Both operands are wanted with the rows innermost: a thread takes 8 rows of two (g) or four (x) columns, and writes 16
+// Both operands are wanted with the rows innermost: a thread takes 4 (g) or 8 rows (x) of four columns and writes 8 or 16
 // bytes per column and part to LDS, which is the transposition.
 
 struct ActGrad {
@@ -121,218 +121,403 @@ __device__ __forceinline__ uint32_t high_halves(float a, float b) {  // a's uppe
     return __builtin_amdgcn_perm(f_bits(b), f_bits(a), 0x07060302u);
 }
 
-template <int TYPE>
-__device__ __forceinline__ void load_two(const void* p, int64_t at, bool two, float& a, float& b) {
+// Four neighbouring values of a row as they come from memory (16-bit types: two words).  The last group of a row that is no
+// multiple of four is the row's last four values, moved down by `back` places when they are used: what then stands behind
+// the row's end does not matter, and memory behind it is not touched.  Where one of the operands has rows of fewer than four values, all are read one by one.
+template <int TYPE, bool NARROW>
+__device__ __forceinline__ u32x4 load_four(const void* p, uint32_t at, int have) {
+    if constexpr (NARROW) {
+        u32x4 u = {0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) u[k] = f_bits(load_one<TYPE>(p, at + min(k, have - 1)));
+        return u;
+    }
     if constexpr (TYPE == MARL_F32) {
-        typedef f32x2 f32x2_a4 __attribute__((aligned(4)));
-        if (two) {
-            const f32x2 v = *reinterpret_cast<const f32x2_a4*>(static_cast<const float*>(p) + at);
-            a = v.x; b = v.y;
-        } else {
-            a = static_cast<const float*>(p)[at]; b = 0.0f;
-        }
+        typedef u32x4 u32x4_a4 __attribute__((aligned(4)));
+        return *reinterpret_cast<const u32x4_a4*>(static_cast<const uint32_t*>(p) + at);
     } else {
-        a = load_one<TYPE>(p, at);
-        b = two ? load_one<TYPE>(p, at + 1) : 0.0f;
+        typedef u32x2 u32x2_a2 __attribute__((aligned(2)));
+        const u32x2 q = *reinterpret_cast<const u32x2_a2*>(static_cast<const uint16_t*>(p) + at);
+        return u32x4{q.x, q.y, 0, 0};
     }
 }
-
-template <int TYPE>
-__device__ __forceinline__ void store_two(void* p, int64_t at, bool two, float a, float b) {
-    if constexpr (TYPE == MARL_F32) {
-        static_cast<float*>(p)[at] = a;
-        if (two) static_cast<float*>(p)[at + 1] = b;
+template <int TYPE, bool NARROW>
+__device__ __forceinline__ void use_four(u32x4 q, int back, float (&v)[4]) {
+    float a, b, c, d;
+    if constexpr (TYPE == MARL_F32 || NARROW) {
+        a = bits_f(q.x); b = bits_f(q.y); c = bits_f(q.z); d = bits_f(q.w);
+    } else if constexpr (TYPE == MARL_BF16) {
+        a = bits_f(q.x << 16); b = bits_f(q.x & 0xFFFF0000u); c = bits_f(q.y << 16); d = bits_f(q.y & 0xFFFF0000u);
     } else {
-        static_cast<uint16_t*>(p)[at] = to_half_type<TYPE>(a);
-        if (two) static_cast<uint16_t*>(p)[at + 1] = to_half_type<TYPE>(b);
+        a = half_lo(q.x); b = half_hi(q.x); c = half_lo(q.y); d = half_hi(q.y);
     }
+    if (back) {
+        a = back == 1 ? b : back == 2 ? c : d;
+        b = back == 1 ? c : d;
+        c = d;
+    }
+    v[0] = a; v[1] = b; v[2] = c; v[3] = d;
+}
+template <bool NARROW>
+__device__ __forceinline__ uint32_t load_four_bytes(const uint8_t* p, uint32_t at, int have) {
+    if constexpr (NARROW) {
+        uint32_t u = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) u |= (uint32_t)p[at + min(k, have - 1)] << (8 * k);
+        return u;
+    }
+    return *reinterpret_cast<const u32_a1*>(p + at);
 }
 
-// A workgroup of four waves has BO output features and BI input features, each wave BO/WO by BI/WI of them.
-template <int TYPE, int BO, int BI, int WO, int WI>
-__global__ void __launch_bounds__(256)
-act_weight_grad_kernel(ActGrad P) {
-    static_assert(WO * WI == 4, "four waves");
-    constexpr int PARTS = grad_parts<TYPE>();
-    constexpr int TO = BO / WO / 16, TI = BI / WI / 16;
-    __shared__ __align__(16) uint8_t A[PARTS][BO][WG_PITCH];
-    __shared__ __align__(16) uint8_t B[BI][WG_PITCH];
-    __shared__ float bias_sum[BO][4];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
-    const int o0 = blockIdx.y * BO, i0 = blockIdx.x * BI;
-    const int wo = (wave / WI) * (BO / WO), wi = (wave % WI) * (BI / WI);
-    const int64_t first = (int64_t)blockIdx.z * P.per, last = min(P.rows, first + P.per);
-    const bool leader = blockIdx.x == 0;  // also writes the cut gradient and sums it
+// A workgroup has BO output features and BI input features, its waves (WO x WI of them) BO/WO by 64 each.  LDS holds two
+// steps: while the waves multiply one, they convert the next, whose loads went out two steps earlier; one barrier a step.
+// Some waves convert x and the others g, the latter before they multiply and the former after it, so that on each SIMD
+// the matrix unit and the vector unit have work at the same time.
+// A column of the tile lies in LDS at (column % 4) * (columns / 4) + column / 4, so that the lanes of a wave, which take
+// four neighbouring columns each, write to neighbouring places, and a lane's results are four neighbouring inputs.
+template <int TYPE, int BO, int BI, int WO, int WI, bool MASK, bool NARROW>
+struct WeightGrad {
+    static constexpr int PARTS = grad_parts<TYPE>(), BYTES = TYPE == MARL_F32 ? 4 : 2;
+    static constexpr int THREADS = 64 * WO * WI, TO = BO / WO / 16, GITEMS = 2 * BO, XITEMS = BI;
+    static_assert(BI == 64 * WI && GITEMS <= THREADS && XITEMS <= THREADS, "a wave has 64 input features, a thread one item of each kind");
 
-    constexpr int GITEMS = BO * 2, XITEMS = BI;  // (group of 8 rows, 2 columns), (group of 8 rows, 4 columns)
-    constexpr int GN = (GITEMS + 255) / 256, XN = (XITEMS + 255) / 256;
-    float bsum[GN][2];
-#pragma unroll
-    for (int q = 0; q < GN; ++q) bsum[q][0] = bsum[q][1] = 0.0f;
-    f32x4 acc[TO][TI];
-#pragma unroll
-    for (int a = 0; a < TO; ++a)
-#pragma unroll
-        for (int b = 0; b < TI; ++b) acc[a][b] = f32x4{0, 0, 0, 0};
+    struct Lds {
+        uint8_t A[2][PARTS][BO][WG_PITCH];
+        uint8_t B[2][BI][WG_PITCH];
+    };
+    struct RawX { uint32_t x[8], s[2]; };  // 8 rows of 4 columns and two of the rows' scales
+    struct RawG { u32x4 g[4]; uint32_t m[4]; };  // 4 rows of 4 columns
 
-    for (int64_t m0 = first; m0 < last; m0 += WG_STEP) {
+    const ActGrad& P;
+    Lds& S;
+    int64_t first, last;
+    int o0, i0, lane, wo, wi;
+    bool leader;  // also writes the cut gradient and sums it
+    int xc, xr, xi, xback, xhave, gc, gr, go, gback, ghave;
+    bool has_g;
+    float bsum[4] = {0, 0, 0, 0};
+    f32x4 acc[TO][4];
+
+    // Rows behind the last are the last one again (their g counts as 0).  A step's place is the same for the whole
+    // workgroup, what differs from thread to thread is a 32-bit offset (at most 32 rows of 2^20 values).
+    template <bool X, bool G>
+    __device__ __forceinline__ void fetch(RawX& x, RawG& g, int64_t m0) const {
+        if (m0 >= last) return;
+        const int lim = (int)min(last - 1 - m0, (int64_t)WG_STEP - 1);
+        if constexpr (X) {
+            const uint8_t* codes = P.codes + m0 * P.cols;
+            const uint8_t* scales = P.scales + m0 * P.blocks;
 #pragma unroll
-        for (int q = 0; q < GN; ++q) {
-            const int it = tid + q * 256;
-            if (GITEMS % 256 != 0 && it >= GITEMS) break;
-            const int pair = it % (BO / 2), mg = it / (BO / 2), o = o0 + 2 * pair;
-            float a[8], b[8];
-            uint32_t top = 0;
+            for (int k = 0; k < 8; ++k) x.x[k] = load_four_bytes<NARROW>(codes, __umul24(min(xr + k, lim), P.cols) + (xi - xback), xhave);
+            // a quad's four lanes have the same block of 32: each takes the scales of two of the eight rows
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int64_t m = m0 + mg * 8 + k;
-                a[k] = b[k] = 0.0f;
-                if (m < last && o < P.out) {
-                    const bool two = o + 1 < P.out;
-                    load_two<TYPE>(P.grad, m * P.out + o, two, a[k], b[k]);
-                    if (P.mask) {
-                        a[k] = P.mask[m * P.out + o] ? a[k] : 0.0f;
-                        b[k] = two && P.mask[m * P.out + o + 1] ? b[k] : 0.0f;
-                        if (leader) store_two<TYPE>(P.masked, m * P.out + o, two, a[k], b[k]);
-                    }
-                }
-                top = max(top, max(f_bits(a[k]) & 0x7FFFFFFFu, f_bits(b[k]) & 0x7FFFFFFFu));
-            }
-            bsum[q][0] += ((a[0] + a[1]) + (a[2] + a[3])) + ((a[4] + a[5]) + (a[6] + a[7]));
-            bsum[q][1] += ((b[0] + b[1]) + (b[2] + b[3])) + ((b[4] + b[5]) + (b[6] + b[7]));
-            const bool wild = top >= 0x7F800000u;  // an infinity minus itself is no number: it has no lower parts
-#pragma unroll
-            for (int p = 0; p < PARTS; ++p) {
-                u32x4 ua, ub;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    ua[k] = high_halves(a[2 * k], a[2 * k + 1]);
-                    ub[k] = high_halves(b[2 * k], b[2 * k + 1]);
-                }
-                *reinterpret_cast<u32x4*>(&A[p][2 * pair][mg * 16]) = ua;
-                *reinterpret_cast<u32x4*>(&A[p][2 * pair + 1][mg * 16]) = ub;
-                if (p + 1 < PARTS) {
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        a[k] = wild && isinf(a[k]) ? 0.0f : a[k] - bits_f(f_bits(a[k]) & 0xFFFF0000u);
-                        b[k] = wild && isinf(b[k]) ? 0.0f : b[k] - bits_f(f_bits(b[k]) & 0xFFFF0000u);
-                    }
-                }
-            }
+            for (int k = 0; k < 2; ++k) x.s[k] = scales[__umul24(min(xr + 4 * k + (lane & 3), lim), P.blocks) + xi / LB_BLOCK];
         }
-#pragma unroll
-        for (int q = 0; q < XN; ++q) {
-            const int it = tid + q * 256;
-            if (XITEMS % 256 != 0 && it >= XITEMS) break;
-            const int four = it % (BI / 4), mg = it / (BI / 4), i = i0 + 4 * four;
-            float v[4][8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int64_t m = m0 + mg * 8 + k;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) v[c][k] = 0.0f;
-                if (m < last && i < P.cols) {
-                    const uint8_t* at = P.codes + m * P.cols + i;
-                    const float s = scale_value(P.scales[m * P.blocks + i / LB_BLOCK]);
-                    uint32_t u;
-                    if (i + 4 <= P.cols) u = *reinterpret_cast<const u32_a1*>(at);
-                    else {
-                        u = at[0];
-                        if (i + 1 < P.cols) u |= (uint32_t)at[1] << 8;
-                        if (i + 2 < P.cols) u |= (uint32_t)at[2] << 16;
-                    }
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) v[c][k] = ((float)((u >> (8 * c)) & 255u) - P.zero) * s;
-                }
-            }
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                u32x4 u;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) u[k] = high_halves(v[c][2 * k], v[c][2 * k + 1]);
-                *reinterpret_cast<u32x4*>(&B[4 * four + c][mg * 16]) = u;
-            }
-        }
-        __syncthreads();
-        bf16x8 x[TI];
-#pragma unroll
-        for (int b = 0; b < TI; ++b) x[b] = *reinterpret_cast<const bf16x8*>(&B[wi + b * 16 + r][g * 16]);
-#pragma unroll
-        for (int p = PARTS - 1; p >= 0; --p)
-#pragma unroll
-            for (int a = 0; a < TO; ++a) {
-                const bf16x8 y = *reinterpret_cast<const bf16x8*>(&A[p][wo + a * 16 + r][g * 16]);
-#pragma unroll
-                for (int b = 0; b < TI; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y, x[b], acc[a][b], 0, 0, 0);
-            }
-        __syncthreads();
-    }
-
-    float* gw = P.gw + (size_t)blockIdx.z * P.out * P.cols;
-#pragma unroll
-    for (int a = 0; a < TO; ++a)
-#pragma unroll
-        for (int b = 0; b < TI; ++b)
+        if constexpr (G) {
+            const uint8_t* grad = static_cast<const uint8_t*>(P.grad) + m0 * P.out * BYTES;
+            const uint8_t* mask = MASK ? P.mask + m0 * P.out : nullptr;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const int o = o0 + wo + a * 16 + g * 4 + k, i = i0 + wi + b * 16 + r;
-                if (o < P.out && i < P.cols) gw[(size_t)o * P.cols + i] = acc[a][b][k];
+                const uint32_t at = __umul24(min(gr + k, lim), P.out) + (go - gback);
+                g.g[k] = load_four<TYPE, NARROW>(grad, at, ghave);
+                if constexpr (MASK) g.m[k] = load_four_bytes<NARROW>(mask, at, ghave);
             }
-    if (leader) {
-#pragma unroll
-        for (int q = 0; q < GN; ++q) {
-            const int it = tid + q * 256;
-            if (GITEMS % 256 != 0 && it >= GITEMS) break;
-            const int pair = it % (BO / 2), mg = it / (BO / 2);
-            bias_sum[2 * pair][mg] = bsum[q][0];
-            bias_sum[2 * pair + 1][mg] = bsum[q][1];
         }
-        __syncthreads();
-        for (int o = tid; o < BO; o += 256)
-            if (o0 + o < P.out)
-                P.gb[(size_t)blockIdx.z * P.out + o0 + o] = (bias_sum[o][0] + bias_sum[o][1]) + (bias_sum[o][2] + bias_sum[o][3]);
     }
+
+    __device__ __forceinline__ void convert_x(const RawX& raw, int buf) const {
+        float s[8], z[8];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int v = (int)f_bits(scale_value(raw.s[k]));
+            s[4 * k] = bits_f(__builtin_amdgcn_update_dpp(0, v, 0x00, 0xF, 0xF, true));  // quad_perm: lane 0's
+            s[4 * k + 1] = bits_f(__builtin_amdgcn_update_dpp(0, v, 0x55, 0xF, 0xF, true));
+            s[4 * k + 2] = bits_f(__builtin_amdgcn_update_dpp(0, v, 0xAA, 0xF, 0xF, true));
+            s[4 * k + 3] = bits_f(__builtin_amdgcn_update_dpp(0, v, 0xFF, 0xF, 0xF, true));
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) z[k] = -P.zero * s[k];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            u32x4 u;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {  // (code - zero) * scale: every step of it is exact
+                const uint32_t xa = raw.x[2 * k] >> (8 * xback), xb = raw.x[2 * k + 1] >> (8 * xback);
+                u[k] = high_halves(fmaf((float)(xa >> (8 * c) & 255u), s[2 * k], z[2 * k]),
+                                   fmaf((float)(xb >> (8 * c) & 255u), s[2 * k + 1], z[2 * k + 1]));
+            }
+            *reinterpret_cast<u32x4*>(&S.B[buf][c * (BI / 4) + xc][xr * 2]) = u;
+        }
+    }
+
+    __device__ __forceinline__ void convert_g(const RawG& raw, int64_t m0, int buf) {
+        float v[4][4];
+        float odd = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            use_four<TYPE, NARROW>(raw.g[k], gback, v[k]);
+            const bool there = m0 + gr + k < last;
+            const uint32_t m = MASK ? (there ? raw.m[k] >> (8 * gback) : 0u) : there ? 0xFFFFFFFFu : 0u;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                v[k][c] = m & (255u << (8 * c)) ? v[k][c] : 0.0f;
+                if (PARTS > 1) odd = fmaf(v[k][c], 0.0f, odd);
+            }
+        }
+        if (leader) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) bsum[c] += (v[0][c] + v[1][c]) + (v[2][c] + v[3][c]);
+            if (MASK) write_masked(v, m0);
+        }
+        const bool wild = odd != 0.0f;  // an infinity or a NaN among them
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                *reinterpret_cast<u32x2*>(&S.A[buf][p][c * (BO / 4) + gc][gr * 2]) =
+                    u32x2{high_halves(v[0][c], v[1][c]), high_halves(v[2][c], v[3][c])};
+            if (p + 1 == PARTS) break;
+            if (p == 0 && wild) {  // an infinity minus itself is no number: it has no lower parts
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) v[k][c] = isinf(v[k][c]) ? 0.0f : v[k][c];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) v[k][c] -= bits_f(f_bits(v[k][c]) & 0xFFFF0000u);
+                continue;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) v[k][c] -= bits_f(f_bits(v[k][c]) & 0xFFFF0000u);
+        }
+    }
+    __device__ __forceinline__ void write_masked(const float (&v)[4][4], int64_t m0) const {
+        const int c0 = o0 + 4 * gc;
+        if (c0 >= P.out) return;
+        uint8_t* masked = static_cast<uint8_t*>(P.masked) + m0 * P.out * BYTES;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (m0 + gr + k >= last) continue;
+            const uint32_t at = (uint32_t)((gr + k) * P.out + c0);
+            if (c0 + 4 <= P.out) {
+                if constexpr (TYPE == MARL_F32) {
+                    *reinterpret_cast<f32x4_a4*>(reinterpret_cast<float*>(masked) + at) = f32x4{v[k][0], v[k][1], v[k][2], v[k][3]};
+                } else {
+                    typedef u32x2 u32x2_a2 __attribute__((aligned(2)));
+                    *reinterpret_cast<u32x2_a2*>(reinterpret_cast<uint16_t*>(masked) + at) =
+                        u32x2{(uint32_t)to_half_type<TYPE>(v[k][0]) | (uint32_t)to_half_type<TYPE>(v[k][1]) << 16,
+                              (uint32_t)to_half_type<TYPE>(v[k][2]) | (uint32_t)to_half_type<TYPE>(v[k][3]) << 16};
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < 3; ++c) {
+                    if (c0 + c >= P.out) continue;
+                    if constexpr (TYPE == MARL_F32) reinterpret_cast<float*>(masked)[at + c] = v[k][c];
+                    else reinterpret_cast<uint16_t*>(masked)[at + c] = to_half_type<TYPE>(v[k][c]);
+                }
+            }
+        }
+    }
+
+    __device__ __forceinline__ void multiply(int buf) {
+        const int r = lane & 15, g = lane >> 4;
+        bf16x8 x[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) x[b] = *reinterpret_cast<const bf16x8*>(&S.B[buf][b * (BI / 4) + wi + r][g * 16]);
+        // the next 16 output features' fragments are on their way while these multiply, and no more: registers are short
+        bf16x8 y[2][PARTS];
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) y[0][p] = *reinterpret_cast<const bf16x8*>(&S.A[buf][p][wo + r][g * 16]);
+#pragma unroll
+        for (int a = 0; a < TO; ++a) {
+            if (a + 1 < TO) {
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p)
+                    y[(a + 1) & 1][p] = *reinterpret_cast<const bf16x8*>(&S.A[buf][p][wo + (a + 1) * 16 + r][g * 16]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int p = PARTS - 1; p >= 0; --p)
+#pragma unroll
+                for (int b = 0; b < 4; ++b) acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(y[a & 1][p], x[b], acc[a][b], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+
+    template <bool X, bool G>
+    __device__ __forceinline__ void convert(const RawX& x, const RawG& g, int64_t m0, int buf) {
+        if (m0 >= last) return;
+        if constexpr (X) convert_x(x, buf);
+        if constexpr (G)
+            if (has_g) convert_g(g, m0, buf);
+    }
+
+    template <bool X, bool G>
+    __device__ __forceinline__ void step(RawX& x, RawG& g, int64_t m0, int buf) {
+        if constexpr (X) multiply(buf);
+        convert<X, G>(x, g, m0 + WG_STEP, buf ^ 1);
+        fetch<X, G>(x, g, m0 + 3 * WG_STEP);
+        if constexpr (!X) multiply(buf);
+        __syncthreads();
+    }
+
+    template <bool X, bool G>
+    __device__ __forceinline__ void walk() {
+        RawX x0, x1;
+        RawG g0, g1;
+        fetch<X, G>(x0, g0, first);
+        fetch<X, G>(x1, g1, first + WG_STEP);
+        convert<X, G>(x0, g0, first, 0);
+        fetch<X, G>(x0, g0, first + 2 * WG_STEP);
+        __syncthreads();
+        for (int64_t m0 = first; m0 < last; m0 += 2 * WG_STEP) {
+            step<X, G>(x1, g1, m0, 0);
+            if (m0 + WG_STEP < last) step<X, G>(x0, g0, m0 + WG_STEP, 1);
+        }
+    }
+
+    __device__ __forceinline__ void run(int split, int tile) {
+        const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        lane = tid & 63;
+        const int ti = (P.cols + BI - 1) / BI;
+        o0 = tile / ti * BO;
+        i0 = tile % ti * BI;
+        wo = wave / WI * (BO / WO);
+        wi = wave % WI * 16;
+        first = (int64_t)split * P.per;
+        last = min(P.rows, first + P.per);
+        leader = i0 == 0;
+        xc = tid % (BI / 4);
+        xr = tid / (BI / 4) * 8;
+        const int git = tid - (THREADS - GITEMS);  // the last threads have g
+        has_g = git >= 0;
+        gc = git & (BO / 4 - 1);
+        gr = has_g ? git / (BO / 4) * 4 : 0;
+        // Columns behind the end: any that exist, their results are not stored.  With fewer than four columns (NARROW) a
+        // group is the columns that there are from its first on.
+        xi = min(i0 + 4 * xc, P.cols - 1);
+        go = min(o0 + 4 * gc, P.out - 1);
+        xback = NARROW ? 0 : max(xi + 4 - P.cols, 0);
+        gback = NARROW ? 0 : max(go + 4 - P.out, 0);
+        xhave = P.cols - xi;
+        ghave = P.out - go;
+#pragma unroll
+        for (int a = 0; a < TO; ++a)
+#pragma unroll
+            for (int b = 0; b < 4; ++b) acc[a][b] = f32x4{0, 0, 0, 0};
+
+        const bool wave_x = wave * 64 < XITEMS, wave_g = wave * 64 + 63 >= THREADS - GITEMS;  // every wave passes the same barriers
+        if (wave_x && wave_g) walk<true, true>();
+        else if (wave_x) walk<true, false>();
+        else if (wave_g) walk<false, true>();
+        else walk<false, false>();
+
+        const int r = lane & 15, g = lane >> 4, ic = i0 + 4 * (wi + r);
+        float* gw = P.gw + (size_t)split * P.out * P.cols;
+#pragma unroll
+        for (int a = 0; a < TO; ++a)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int place = wo + a * 16 + g * 4 + k, oc = o0 + 4 * (place & (BO / 4 - 1)) + place / (BO / 4);
+                if (oc >= P.out) continue;
+                float* to = gw + (size_t)oc * P.cols + ic;
+                if (ic + 4 <= P.cols) {
+                    *reinterpret_cast<f32x4_a4*>(to) = f32x4{acc[a][0][k], acc[a][1][k], acc[a][2][k], acc[a][3][k]};
+                } else {
+#pragma unroll
+                    for (int b = 0; b < 3; ++b)
+                        if (ic + b < P.cols) to[b] = acc[a][b][k];
+                }
+            }
+        if (leader) {
+            float* sums = reinterpret_cast<float*>(&S.A[0][0][0][0]);  // [BO][8 groups of rows]; every wave is past its last step
+            if (has_g) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) sums[(4 * gc + c) * 8 + gr / 4] = bsum[c];
+            }
+            __syncthreads();
+            for (int q = tid; q < BO && o0 + q < P.out; q += THREADS) {
+                const float* s = sums + q * 8;
+                P.gb[(size_t)split * P.out + o0 + q] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+            }
+        }
+    }
+};
+
+template <int TYPE, int BO, int BI, int WO, int WI, bool MASK, bool NARROW>
+__global__ void __launch_bounds__(64 * WO * WI, 2)
+act_weight_grad_kernel(ActGrad P) {
+    typedef WeightGrad<TYPE, BO, BI, WO, WI, MASK, NARROW> Pass;
+    __shared__ __align__(16) typename Pass::Lds lds;
+    // workgroups go to the eight XCDs in turn: the tiles of one split, which read the same rows, stay on one of them
+    const int tiles = ((P.cols + BI - 1) / BI) * ((P.out + BO - 1) / BO);
+    const int turn = blockIdx.x >> 3, split = (turn / tiles) * 8 + (blockIdx.x & 7);
+    if (split >= P.splits) return;
+    Pass pass{P, lds};
+    pass.run(split, turn % tiles);
 }
 
-// Sums of the splits in their order, in double (hundreds of them, one after the other): the weight's entries, then the
-// bias's
+// Sums of the splits in double: the weight's entries, then the bias's.  A workgroup has 64 entries, its four waves every
+// fourth split each, and their four sums are added in order.
 __global__ void __launch_bounds__(256)
 act_join_kernel(const float* __restrict__ part_w, const float* __restrict__ part_b, int64_t nw, int nb, int splits,
                 float* __restrict__ gw, float* __restrict__ gb) {
-    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const bool bias = at >= nw;
-    if (at >= nw + nb) return;
+    __shared__ double sums[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t at = (int64_t)blockIdx.x * 64 + lane;
+    const bool bias = at >= nw, live = at < nw + nb;
     const float* p = bias ? part_b + (at - nw) : part_w + at;
     const int64_t step = bias ? nb : nw;
     double s = 0.0;
-    for (int k = 0; k < splits; ++k) s += (double)p[k * step];
-    if (bias) gb[at - nw] = (float)s;
-    else gw[at] = (float)s;
+    if (live)
+#pragma unroll 8
+        for (int k = wave; k < splits; k += 4) s += (double)p[k * step];
+    sums[wave][lane] = s;
+    __syncthreads();
+    if (wave || !live) return;
+    const float v = (float)((sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]));
+    if (bias) gb[at - nw] = v;
+    else gw[at] = v;
 }
 
 // ------------------------------------------------------------------------------------------------------------ host
 
-struct ActCut { int bo, bi, splits; int64_t per; };
+struct ActCut { int bo, bi, splits; int64_t per, grid; };
 static ActCut act_cut(int64_t rows, int out, int cols) {
     ActCut c;
-    c.bo = out <= 16 ? 16 : 64;
-    c.bi = out <= 16 ? 256 : 64;
-    const int64_t tiles = (int64_t)((out + c.bo - 1) / c.bo) * ((cols + c.bi - 1) / c.bi);
     const int64_t steps = (rows + WG_STEP - 1) / WG_STEP;
-    int64_t s = 1024 / tiles;
+    const auto tiles = [&](int bo, int bi) { return (int64_t)((out + bo - 1) / bo) * ((cols + bi - 1) / bi); };
+    if (out <= 16 || cols < 4) { c.bo = 16; c.bi = 256; }
+    else if (tiles(128, 256) * (steps / 8) >= 256) { c.bo = 128; c.bi = 256; }
+    else { c.bo = 64; c.bi = 64; }
+    const int64_t t = tiles(c.bo, c.bi);
+    int64_t s = (c.bo == 128 ? 256 : 512) / t;
     s = s < 1 ? 1 : s;
     const int64_t most = (steps + 3) / 4;  // at least four steps each
     s = s > most ? most : s;
     const int64_t each = (steps + s - 1) / s;
     c.per = each * WG_STEP;
     c.splits = (int)((steps + each - 1) / each);
+    c.grid = (int64_t)(c.splits + 7) / 8 * 8 * t;
     return c;
 }
 
+template <int TYPE, bool MASK>
+static void launch_weight_grad_mask(const ActGrad& P, const ActCut& c, hipStream_t stream) {
+    const dim3 grid((uint32_t)c.grid);
+    if (c.bo == 16 && (P.out < 4 || P.cols < 4))
+        hipLaunchKernelGGL((act_weight_grad_kernel<TYPE, 16, 256, 1, 4, MASK, true>), grid, dim3(256), 0, stream, P);
+    else if (c.bo == 16) hipLaunchKernelGGL((act_weight_grad_kernel<TYPE, 16, 256, 1, 4, MASK, false>), grid, dim3(256), 0, stream, P);
+    else if (c.bo == 64) hipLaunchKernelGGL((act_weight_grad_kernel<TYPE, 64, 64, 4, 1, MASK, false>), grid, dim3(256), 0, stream, P);
+    else hipLaunchKernelGGL((act_weight_grad_kernel<TYPE, 128, 256, 2, 4, MASK, false>), grid, dim3(512), 0, stream, P);
+}
 template <int TYPE>
-static void launch_weight_grad_type(const ActGrad& P, const ActCut& c, dim3 grid, hipStream_t stream) {
-    if (c.bo == 16) hipLaunchKernelGGL((act_weight_grad_kernel<TYPE, 16, 256, 1, 4>), grid, dim3(256), 0, stream, P);
-    else hipLaunchKernelGGL((act_weight_grad_kernel<TYPE, 64, 64, 2, 2>), grid, dim3(256), 0, stream, P);
+static void launch_weight_grad_type(const ActGrad& P, const ActCut& c, hipStream_t stream) {
+    if (P.mask) launch_weight_grad_mask<TYPE, true>(P, c, stream);
+    else launch_weight_grad_mask<TYPE, false>(P, c, stream);
 }
 
 static int act_hip(hipError_t e, const char* what) {
@@ -419,14 +604,13 @@ extern "C" int marl_act_weight_grad(const void* d_grad, int grad_type, int64_t n
     P.splits = c.splits; P.per = c.per;
     P.gw = c.splits == 1 ? d_grad_weight : static_cast<float*>(d_workspace);
     P.gb = c.splits == 1 ? d_grad_bias : static_cast<float*>(d_workspace) + c.splits * nw;
-    const dim3 grid((num_cols + c.bi - 1) / c.bi, (num_out + c.bo - 1) / c.bo, c.splits);
-    if (grad_type == MARL_F32) launch_weight_grad_type<MARL_F32>(P, c, grid, s);
-    else if (grad_type == MARL_BF16) launch_weight_grad_type<MARL_BF16>(P, c, grid, s);
-    else launch_weight_grad_type<MARL_F16>(P, c, grid, s);
+    if (grad_type == MARL_F32) launch_weight_grad_type<MARL_F32>(P, c, s);
+    else if (grad_type == MARL_BF16) launch_weight_grad_type<MARL_BF16>(P, c, s);
+    else launch_weight_grad_type<MARL_F16>(P, c, s);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || c.splits == 1) return act_hip(e, "weight gradient launch");
     const int64_t threads = nw + num_out;
-    hipLaunchKernelGGL(act_join_kernel, dim3((uint32_t)((threads + 255) / 256)), dim3(256), 0, s, P.gw, P.gb, nw, num_out, c.splits,
+    hipLaunchKernelGGL(act_join_kernel, dim3((uint32_t)((threads + 63) / 64)), dim3(256), 0, s, P.gw, P.gb, nw, num_out, c.splits,
                        d_grad_weight, d_grad_bias);
     return act_hip(hipGetLastError(), "weight gradient join launch");
 }
