@@ -117,6 +117,21 @@ def lib() -> ctypes.CDLL:
     return L
 
 
+def call(fn, what: str, device, *args) -> None:
+    """fn(*args, stream) with `device` current and its current stream: an entry point's call for tensors on `device`.
+    Small passes are bound by the host, so nothing is switched that is right already."""
+    import torch
+
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != 0:
+        check(rc, what)
+
+
 def check(rc: int, what: str) -> None:
     if rc != 0:
         msg = lib().marl_last_error()

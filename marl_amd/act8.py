@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .mxfp4 import BLOCK, _TYPES, _p, _rows, _stream
+from .mxfp4 import BLOCK, _TYPES, _bytes_on_gpu, _p, _rows
 
 
 class Act8:
@@ -19,31 +19,22 @@ class Act8:
     the block reads as NaN), blocks = ceil(cols / 32).  `nonnegative`: codes are 0 .. 255 and 0 only for zero; otherwise
     128 is zero."""
 
+    __slots__ = ("codes", "scales", "nonnegative", "shape", "device")
+
     def __init__(self, codes, scales, nonnegative):
-        for t, name in ((codes, "codes"), (scales, "scales")):
-            if not isinstance(t, torch.Tensor) or t.dtype != torch.uint8 or t.dim() != 2 or not t.is_contiguous() or not t.is_cuda:
-                raise ValueError(f"{name} must be a contiguous 2-d uint8 tensor on the GPU")
-        if codes.shape[1] == 0 or scales.shape != (codes.shape[0], -(-codes.shape[1] // BLOCK)) or scales.device != codes.device:
+        rows, cols = _bytes_on_gpu(codes, "codes")
+        if cols == 0 or _bytes_on_gpu(scales, "scales") != (rows, -(-cols // BLOCK)) or scales.device != codes.device:
             raise ValueError("scales must be [rows, ceil(cols / 32)] beside the codes' [rows, cols], on the same device")
         self.codes, self.scales, self.nonnegative = codes, scales, bool(nonnegative)
-
-    @property
-    def shape(self):
-        return self.codes.shape
-
-    @property
-    def device(self):
-        return self.codes.device
+        self.shape, self.device = codes.shape, codes.device
 
     def dequantize(self, dtype=torch.float32):
         """the values, as a [rows, cols] tensor (exact also in bfloat16)"""
         if dtype not in _TYPES:
             raise ValueError("dtype must be torch.float32, torch.bfloat16 or torch.float16")
-        out = torch.empty(tuple(self.shape), dtype=dtype, device=self.device)
-        with torch.cuda.device(self.device):
-            _lib.check(_lib.lib().marl_act_dequantize(_p(self.codes), _p(self.scales), self.shape[0], self.shape[1],
-                                                      int(self.nonnegative), _TYPES[dtype], _p(out), _stream(self.device)),
-                       "marl_act_dequantize")
+        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        _lib.call(_lib.lib().marl_act_dequantize, "marl_act_dequantize", self.device, self.codes.data_ptr(), self.scales.data_ptr(),
+                  self.shape[0], self.shape[1], 1 if self.nonnegative else 0, _TYPES[dtype], out.data_ptr())
         return out
 
 
@@ -51,13 +42,13 @@ def compress(x, nonnegative=False):
     """x: float32, bfloat16 or float16 [rows, cols] on the GPU (rows may lie apart).  `nonnegative`: x has no negative
     values (it comes from a ReLU); any there are count as 0.  One step of a block is at most 1/64 (nonnegative: 1/128) of
     its largest value, so a value is off by at most half that; a positive one that would round to 0 becomes one step."""
-    x, stride = _rows(x.detach() if isinstance(x, torch.Tensor) else x, "x")
-    rows, cols = x.shape
-    out = Act8(torch.empty((rows, cols), dtype=torch.uint8, device=x.device),
-               torch.empty((rows, -(-cols // BLOCK)), dtype=torch.uint8, device=x.device), nonnegative)
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.lib().marl_act_compress(_p(x), _TYPES[x.dtype], rows, cols, stride, int(out.nonnegative), _p(out.codes),
-                                                _p(out.scales), _stream(x.device)), "marl_act_compress")
+    x, rows, cols, stride = _rows(x, "x")
+    out = Act8.__new__(Act8)
+    out.codes = torch.empty((rows, cols), dtype=torch.uint8, device=x.device)
+    out.scales = torch.empty((rows, -(-cols // BLOCK)), dtype=torch.uint8, device=x.device)
+    out.nonnegative, out.shape, out.device = bool(nonnegative), x.shape, x.device
+    _lib.call(_lib.lib().marl_act_compress, "marl_act_compress", x.device, x.data_ptr(), _TYPES[x.dtype], rows, cols, stride,
+              1 if nonnegative else 0, out.codes.data_ptr(), out.scales.data_ptr())
     return out
 
 
@@ -66,15 +57,16 @@ def weight_grad(grad, act, mask=None):
     float16) and the kept x (`act`).  `mask`: y as it was kept (nonnegative) where a ReLU stood behind the layer.
     Returns (grad_weight float32 [out, cols], grad_bias float32 [out], the gradient behind the ReLU in grad's type, or None
     without a mask)."""
-    grad, _ = _rows(grad.detach() if isinstance(grad, torch.Tensor) else grad, "grad")
-    grad = grad.contiguous()
-    if not isinstance(act, Act8) or act.shape[0] != grad.shape[0] or act.device != grad.device:
+    grad, rows, out, stride = _rows(grad, "grad")
+    if stride != out:
+        grad = grad.contiguous()
+    device = grad.device
+    if not isinstance(act, Act8) or act.shape[0] != rows or act.device != device:
         raise ValueError("act must be an Act8 with the rows and the device of grad")
-    if mask is not None and (not isinstance(mask, Act8) or not mask.nonnegative or mask.shape != grad.shape or mask.device != grad.device):
+    if mask is not None and (not isinstance(mask, Act8) or not mask.nonnegative or mask.shape != grad.shape or mask.device != device):
         raise ValueError("mask must be a nonnegative Act8 of grad's shape, on its device")
-    rows, out = grad.shape
-    cols, device = act.shape[1], grad.device
-    masked = torch.empty_like(grad) if mask is not None else None
+    cols = act.shape[1]
+    masked = torch.empty((rows, out), dtype=grad.dtype, device=device) if mask is not None else None
     if rows == 0:
         return torch.zeros((out, cols), device=device), torch.zeros(out, device=device), masked
     gw = torch.empty((out, cols), dtype=torch.float32, device=device)
@@ -82,8 +74,7 @@ def weight_grad(grad, act, mask=None):
     L = _lib.lib()
     need = L.marl_act_weight_grad_workspace_bytes(rows, out, cols)
     work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    with torch.cuda.device(device):
-        _lib.check(L.marl_act_weight_grad(_p(grad), _TYPES[grad.dtype], rows, out, _p(act.codes), _p(act.scales), cols,
-                                          int(act.nonnegative), _p(mask.codes) if mask is not None else None, _p(masked), _p(gw),
-                                          _p(gb), _p(work), _stream(device)), "marl_act_weight_grad")
+    _lib.call(L.marl_act_weight_grad, "marl_act_weight_grad", device, grad.data_ptr(), _TYPES[grad.dtype], rows, out,
+              act.codes.data_ptr(), act.scales.data_ptr(), cols, 1 if act.nonnegative else 0,
+              mask.codes.data_ptr() if mask is not None else None, _p(masked), gw.data_ptr(), gb.data_ptr(), _p(work))
     return gw, gb, masked

@@ -7,8 +7,6 @@ here has a gradient.  (The whole numbers of the two-agent observations, -3 to 4,
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
@@ -19,74 +17,75 @@ _MXFP4 = 3
 
 
 def _p(t):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
-
-
-def _stream(device):
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    return None if t is None else t.data_ptr()
 
 
 def _rows(x, name):
-    """a 2-d float tensor on the GPU whose rows are contiguous (they may lie apart): (tensor, row stride)"""
-    if not isinstance(x, torch.Tensor) or x.dim() != 2 or not x.is_cuda or x.dtype not in _TYPES:
+    """a 2-d float tensor on the GPU whose rows are contiguous (they may lie apart): (tensor, rows, cols, row stride)"""
+    if not isinstance(x, torch.Tensor) or x.dtype not in _TYPES or x.dim() != 2 or not x.is_cuda:
         raise ValueError(f"{name} must be a float32, bfloat16 or float16 [rows, cols] tensor on the GPU")
-    if x.shape[1] == 0:
-        raise ValueError(f"{name} has no columns")
-    if x.shape[0] > 1 and (x.stride(1) != 1 or x.stride(0) < x.shape[1]) or x.shape[0] == 1 and x.shape[1] > 1 and x.stride(1) != 1:
-        x = x.contiguous()
-    return x, (x.stride(0) if x.shape[0] > 1 else x.shape[1])
+    rows, cols = x.shape
+    if x.is_contiguous():
+        if cols == 0:
+            raise ValueError(f"{name} has no columns")
+        return x, rows, cols, cols
+    if x.stride(1) != 1 or x.stride(0) < cols:
+        return x.contiguous(), rows, cols, cols
+    return x, rows, cols, x.stride(0)
+
+
+def _bytes_on_gpu(t, name):
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.uint8 or t.dim() != 2 or not t.is_cuda or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous 2-d uint8 tensor on the GPU")
+    return t.shape
 
 
 class MXFP4:
     """A [rows, cols] tensor in 4 bits: `codes` uint8 [rows, 16 * blocks] (two codes a byte, the lower half first) and
     `scales` uint8 [rows, blocks] (2^(byte - 127); 255: the block reads as NaN), blocks = ceil(cols / 32)."""
 
+    __slots__ = ("codes", "scales", "shape", "device")
+
     def __init__(self, codes, scales, cols):
-        cols = int(cols)
+        rows, width = _bytes_on_gpu(codes, "codes")
         blocks = -(-cols // BLOCK)
-        for t, width, name in ((codes, 16 * blocks, "codes"), (scales, blocks, "scales")):
-            if not isinstance(t, torch.Tensor) or t.dtype != torch.uint8 or t.dim() != 2 or not t.is_contiguous() or not t.is_cuda:
-                raise ValueError(f"{name} must be a contiguous 2-d uint8 tensor on the GPU")
-            if cols <= 0 or t.shape[1] != width or t.shape[0] != codes.shape[0] or t.device != codes.device:
-                raise ValueError(f"{name} of {cols} columns must be [rows, {width}], the same rows and device as the codes")
-        self.codes, self.scales, self.cols = codes, scales, cols
+        if cols <= 0 or width != 16 * blocks or _bytes_on_gpu(scales, "scales") != (rows, blocks) or scales.device != codes.device:
+            raise ValueError(f"codes and scales of {cols} columns must be [rows, {16 * blocks}] and [rows, {blocks}] on one device")
+        self.codes, self.scales, self.shape, self.device = codes, scales, torch.Size((rows, cols)), codes.device
 
     @property
-    def shape(self):
-        return torch.Size((self.codes.shape[0], self.cols))
-
-    @property
-    def device(self):
-        return self.codes.device
+    def cols(self):
+        return self.shape[1]
 
     def dequantize(self, dtype=torch.float32):
         """the values, as a [rows, cols] tensor (rounded once more for the 16-bit types)"""
         if dtype not in _TYPES:
             raise ValueError("dtype must be torch.float32, torch.bfloat16 or torch.float16")
-        out = torch.empty(tuple(self.shape), dtype=dtype, device=self.device)
-        with torch.cuda.device(self.device):
-            _lib.check(_lib.lib().marl_mx_dequantize(_p(self.codes), _p(self.scales), self.shape[0], self.cols, _TYPES[dtype],
-                                                     _p(out), _stream(self.device)), "marl_mx_dequantize")
+        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        _lib.call(_lib.lib().marl_mx_dequantize, "marl_mx_dequantize", self.device, self.codes.data_ptr(), self.scales.data_ptr(),
+                  self.shape[0], self.shape[1], _TYPES[dtype], out.data_ptr())
         return out
 
 
 def _empty(rows, cols, device):
     blocks = -(-cols // BLOCK)
-    return MXFP4(torch.empty((rows, 16 * blocks), dtype=torch.uint8, device=device),
-                 torch.empty((rows, blocks), dtype=torch.uint8, device=device), cols)
+    new = MXFP4.__new__(MXFP4)
+    new.codes = torch.empty((rows, 16 * blocks), dtype=torch.uint8, device=device)
+    new.scales = torch.empty((rows, blocks), dtype=torch.uint8, device=device)
+    new.shape, new.device = torch.Size((rows, cols)), device
+    return new
 
 
 def quantize(x, out=None):
     """x: float32, bfloat16 or float16 [rows, cols] on the GPU (rows may lie apart).  `out`: an MXFP4 of the same shape
     to write into (a weight that captured launches read) instead of a new one."""
-    x, stride = _rows(x.detach() if isinstance(x, torch.Tensor) else x, "x")
+    x, rows, cols, stride = _rows(x, "x")
     if out is None:
-        out = _empty(x.shape[0], x.shape[1], x.device)
+        out = _empty(rows, cols, x.device)
     elif not isinstance(out, MXFP4) or out.shape != x.shape or out.device != x.device:
         raise ValueError(f"out must be an MXFP4 of shape {tuple(x.shape)} on the device of x")
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.lib().marl_mx_quantize(_p(x), _TYPES[x.dtype], x.shape[0], x.shape[1], stride, _p(out.codes), _p(out.scales),
-                                               _stream(x.device)), "marl_mx_quantize")
+    _lib.call(_lib.lib().marl_mx_quantize, "marl_mx_quantize", x.device, x.data_ptr(), _TYPES[x.dtype], rows, cols, stride,
+              out.codes.data_ptr(), out.scales.data_ptr())
     return out
 
 
@@ -96,19 +95,22 @@ def linear(x, weight, bias=None, relu=False, out_dtype=torch.float32):
     out_dtype="mxfp4", an MXFP4 (the next layer's x)."""
     if not isinstance(weight, MXFP4):
         raise ValueError("weight must be an MXFP4 (mxfp4.quantize)")
-    quantised = isinstance(x, MXFP4)
-    if not quantised:
+    n, cols = weight.shape
+    if isinstance(x, MXFP4):
+        rows, xcols = x.shape
+        x_data, x_scales, x_type, stride = x.codes, x.scales, _MXFP4, 0
+    else:
         if isinstance(x, torch.Tensor) and x.requires_grad and torch.is_grad_enabled():
             raise ValueError("mxfp4.linear has no gradient: call it under torch.no_grad()")
-        x, stride = _rows(x, "x")
-    if x.shape[1] != weight.cols or x.device != weight.device:
-        raise ValueError(f"x has {x.shape[1]} columns on {x.device}, the weight {weight.cols} on {weight.device}")
-    rows, n = x.shape[0], weight.shape[0]
+        x, rows, xcols, stride = _rows(x, "x")
+        x_data, x_scales, x_type = x, None, _TYPES[x.dtype]
+    device = x.device
+    if xcols != cols or device != weight.device:
+        raise ValueError(f"x has {xcols} columns on {device}, the weight {cols} on {weight.device}")
     if n == 0:
         raise ValueError("weight has no rows")
-    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or not bias.is_contiguous() or bias.device != x.device):
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or not bias.is_contiguous() or bias.device != device):
         raise ValueError(f"bias must be a contiguous float32 tensor of {n} entries on the device of x")
-    device = x.device
     if out_dtype == "mxfp4":
         y = _empty(rows, n, device)
         y_data, y_scales, y_type = y.codes, y.scales, _MXFP4
@@ -118,11 +120,9 @@ def linear(x, weight, bias=None, relu=False, out_dtype=torch.float32):
     else:
         raise ValueError('out_dtype must be torch.float32, torch.bfloat16, torch.float16 or "mxfp4"')
     L = _lib.lib()
-    x_data, x_scales, x_type, stride = (x.codes, x.scales, _MXFP4, 0) if quantised else (x, None, _TYPES[x.dtype], stride)
-    need = L.marl_mx_linear_workspace_bytes(x_type, rows, weight.cols, n)
+    need = L.marl_mx_linear_workspace_bytes(x_type, rows, cols, n)
     work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    with torch.cuda.device(device):
-        _lib.check(L.marl_mx_linear(_p(x_data), _p(x_scales), x_type, rows, weight.cols, stride, _p(weight.codes), _p(weight.scales),
-                                    n, _p(bias), int(bool(relu)), _p(y_data), _p(y_scales), y_type, _p(work), _stream(device)),
-                   "marl_mx_linear")
+    _lib.call(L.marl_mx_linear, "marl_mx_linear", device, x_data.data_ptr(), _p(x_scales), x_type, rows, cols, stride,
+              weight.codes.data_ptr(), weight.scales.data_ptr(), n, _p(bias), 1 if relu else 0, y_data.data_ptr(), _p(y_scales), y_type,
+              _p(work))
     return y

@@ -173,7 +173,7 @@ def test_largest_gradients_do_not_overflow_in_their_parts():
 
 def test_every_output_is_written_and_nothing_else():
     from marl_amd import _lib, act8
-    from marl_amd.mxfp4 import _p, _stream
+    from marl_amd.mxfp4 import _p
 
     L = _lib.lib()
     for rows, out, cols in ((37, 65, 202), (700, 9, 33), (3000, 130, 70)):
@@ -182,7 +182,7 @@ def test_every_output_is_written_and_nothing_else():
         bufs = [torch.full((n + 128,), 7.0, device="cuda") for n in (out * cols, out, rows * out)]
         work = torch.full((need + 64,), 9, dtype=torch.uint8, device="cuda")
         _lib.check(L.marl_act_weight_grad(_p(grad), 0, rows, out, _p(act.codes), _p(act.scales), cols, 1, _p(mask.codes), _p(bufs[2][64:]),
-                                          _p(bufs[0][64:]), _p(bufs[1][64:]), _p(work), _stream(grad.device)), "marl_act_weight_grad")
+                                          _p(bufs[0][64:]), _p(bufs[1][64:]), _p(work), torch.cuda.current_stream().cuda_stream), "marl_act_weight_grad")
         for buf, want in zip(bufs, (gw, gb, masked)):
             assert torch.equal(buf[64:-64], want.flatten()) and (buf[:64] == 7).all() and (buf[-64:] == 7).all()
         assert (work[need:] == 9).all()

@@ -179,7 +179,7 @@ def test_every_output_is_written_and_nothing_else():
         need = L.marl_mx_linear_workspace_bytes(0, rows, cols, out)
         work = torch.full((need + 256,), 9, dtype=torch.uint8, device="cuda")
         _lib.check(L.marl_mx_linear(p(x), None, 0, rows, cols, 0, p(wq.codes), p(wq.scales), out, None, 0, p(room[256:]), None, 0,
-                                    p(work), mxfp4._stream(x.device)), "marl_mx_linear")
+                                    p(work), torch.cuda.current_stream().cuda_stream), "marl_mx_linear")
         assert torch.equal(room[256:256 + rows * out].view(rows, out), mxfp4.linear(x, wq))
         assert (room[:256] == 7).all() and (room[256 + rows * out:] == 7).all() and (work[need:] == 9).all()
 
