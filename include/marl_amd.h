@@ -298,10 +298,10 @@ int marl_mx_dequantize(const uint8_t *d_codes, const uint8_t *d_scales, int64_t 
  *   d_bias    float32 [num_out] or NULL
  *   d_y       y_type [num_rows][num_out]; MARL_MXFP4: the result is quantised as marl_mx_quantize would
  *             quantise its float32 values, codes to d_y (16-byte aligned), scales to d_y_scales
- *   d_workspace   marl_mx_linear_workspace_bytes() bytes, 16-byte aligned; that is 0 for num_cols up to
- *             512 (d_workspace may then be NULL)
- * The same call gives the same bits every time.  At most 2^22 output features; of rows of more than 512
- * values at most 4,194,240.
+ *   d_workspace   marl_mx_linear_workspace_bytes() bytes, 16-byte aligned; that is 0 for num_cols
+ *             from 8 to 512 (d_workspace may then be NULL)
+ * The same call gives the same bits every time.  At most 2^22 output features; of rows of fewer than 8
+ * or more than 512 values at most 4,194,240.
  */
 int marl_mx_linear(const void *d_x, const uint8_t *d_x_scales, int x_type, int64_t num_rows, int num_cols,
                    int64_t row_stride, const uint8_t *d_w_codes, const uint8_t *d_w_scales, int num_out,

@@ -80,8 +80,9 @@ mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restric
 // v_mfma_scale_f32_16x16x128_f8f6f4 takes 16 rows of 128 values from each operand; lane l holds row l % 16, block l / 16
 // of the four 32-value blocks, so a lane's 16 bytes of codes and its scale byte are exactly one stored block: fragments
 // need no rearrangement, neither from memory nor from LDS.  The weight is the first operand, so a lane's four results
-// are four output features of one row.  Rows of the weight are dealt to a wave's four tiles such that a lane's 4 x 4
-// results are 16 consecutive features: feature = 16 (lane / 16) + 4 tile + i.
+// are four output features of one row.  Rows of the weight are dealt to a wave's four tiles such that a lane has `span`
+// neighbouring features, 16 bytes of float32 (4) or of a 16-bit type (8), half a block of MXFP4 (16), and the four lanes
+// of a row write 64 neighbouring bytes with one store.
 
 struct MxLinear {
     const void* x;            // float rows, or codes
@@ -99,6 +100,13 @@ struct MxLinear {
     int splits;
 };
 
+template <int OUT> constexpr int mx_span() { return OUT == MARL_F32 ? 4 : OUT == MARL_MXFP4 ? 16 : 8; }
+// first of the four neighbouring features that lane group g has from tile t
+template <int OUT> __device__ __forceinline__ int mx_feature(int t, int g) {
+    constexpr int SPAN = mx_span<OUT>(), TILES = SPAN / 4;
+    return t / TILES * (4 * SPAN) + g * SPAN + t % TILES * 4;
+}
+
 __device__ __forceinline__ f32x4 mx_mfma(u32x4 a, u32x4 b, f32x4 c, int ks, int sa, int sb) {
     const i32x8 A = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};
     const i32x8 B = {(int)b.x, (int)b.y, (int)b.z, (int)b.w, 0, 0, 0, 0};
@@ -110,15 +118,16 @@ __device__ __forceinline__ f32x4 mx_mfma(u32x4 a, u32x4 b, f32x4 c, int ks, int 
     }
 }
 
-// Results of one lane: row m, features n .. n + 15 (v[4 t + i] is feature n + 4 t + i).  All lanes of the wave come
-// here together (the MXFP4 form exchanges maxima between lanes); `live` says whether row m exists.
+// Results of one lane: row m, v[4 t + i] is feature n0 + mx_feature(t, g) + i.  All lanes of the wave come here together
+// (the MXFP4 form exchanges maxima between lanes); `live` says whether row m exists.
 template <int OUT>
-__device__ __forceinline__ void mx_store(const MxLinear& P, int64_t m, bool live, int n, float (&v)[16]) {
+__device__ __forceinline__ void mx_store(const MxLinear& P, int64_t m, bool live, int n0, int g, float (&v)[16]) {
     if (P.relu) {
 #pragma unroll
         for (int k = 0; k < 16; ++k) v[k] = v[k] < 0.0f ? 0.0f : v[k];  // a NaN stays
     }
     if constexpr (OUT == MARL_MXFP4) {
+        const int n = n0 + 16 * g;
         uint32_t top = 0;
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
@@ -135,13 +144,31 @@ __device__ __forceinline__ void mx_store(const MxLinear& P, int64_t m, bool live
         *reinterpret_cast<u32x2*>(static_cast<uint8_t*>(P.y) + (m * yb + b) * 16 + (n & 16) / 2) = u32x2{mx_codes(lo, byte), mx_codes(hi, byte)};
         if ((n & 16) == 0) P.y_scales[m * yb + b] = (uint8_t)byte;
     } else {
-        if (!live || n >= P.out) return;
-        const int64_t at = m * P.out + n, end = m * P.out + P.out;
-        float lo[8], hi[8];
+        if (!live) return;
+        const int64_t row = m * P.out;
+        constexpr int SPAN = mx_span<OUT>();
 #pragma unroll
-        for (int k = 0; k < 8; ++k) { lo[k] = v[k]; hi[k] = v[8 + k]; }
-        store_eight<OUT>(P.y, at, end, lo);
-        store_eight<OUT>(P.y, at + 8, end, hi);
+        for (int s = 0; s < 16 / SPAN; ++s) {
+            const int n = n0 + mx_feature<OUT>(s * SPAN / 4, g);
+            if (n + SPAN <= P.out) {
+                if constexpr (OUT == MARL_F32) {
+                    *reinterpret_cast<f32x4_a4*>(static_cast<float*>(P.y) + row + n) = f32x4{v[4 * s], v[4 * s + 1], v[4 * s + 2], v[4 * s + 3]};
+                } else {
+                    u32x4 u;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        u[k] = (uint32_t)to_half_type<OUT>(v[8 * s + 2 * k]) | (uint32_t)to_half_type<OUT>(v[8 * s + 2 * k + 1]) << 16;
+                    *reinterpret_cast<u32x4_a2*>(static_cast<uint16_t*>(P.y) + row + n) = u;
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < SPAN; ++k) {
+                    if (n + k >= P.out) continue;
+                    if constexpr (OUT == MARL_F32) static_cast<float*>(P.y)[row + n + k] = v[SPAN * s + k];
+                    else static_cast<uint16_t*>(P.y)[row + n + k] = to_half_type<OUT>(v[SPAN * s + k]);
+                }
+            }
+        }
     }
 }
 
@@ -154,25 +181,56 @@ __device__ __forceinline__ uint32_t mx_scale(const uint8_t* scales, int64_t row,
     return row < rows && b < blocks ? scales[row * blocks + b] : 127u;
 }
 
-// Many rows of at most 512 values: a wave keeps its 64 features' whole weight in registers (at most 64 of them) and the
-// workgroup walks row tiles of 32, which its threads quantise into LDS on the way (four lanes per block, as above).
-// Bound by memory: rows in, results out, the weight once per workgroup.
-constexpr int MX_TILE = 32;
+// Rows of 8 to 512 values.  A workgroup has eight waves, WN of them side by side (64 features each) and 8 / WN below one
+// another, and walks row tiles; a wave keeps its 64 features' whole weight in registers (at most 64 of them).  The threads
+// quantise a tile's rows into LDS (four lanes per block, as above); the next tile's values are on their way from memory
+// meanwhile.  Bound by memory: rows in, results out, the weight once per workgroup.
+template <int WN>
+struct MxTile {
+    static constexpr int WM = 8 / WN, GROUPS = WN == 8 ? 2 : 1;  // waves along the rows; groups of 16 rows each of them has
+    static constexpr int ROWS = 16 * WM * GROUPS;
+};
 
-template <int KS, int IN, int OUT>
+// eight values of a row as they come from memory; `n` of them exist
+template <int TYPE> struct MxRaw { u32x4 u[TYPE == MARL_F32 ? 2 : 1]; };
+template <int TYPE>
+__device__ __forceinline__ void raw_load(MxRaw<TYPE>& raw, const void* x, int64_t at) {
+    if constexpr (TYPE == MARL_F32) {
+        typedef u32x4 u32x4_a4 __attribute__((aligned(4)));
+        const u32x4_a4* p = reinterpret_cast<const u32x4_a4*>(static_cast<const uint32_t*>(x) + at);
+        raw.u[0] = p[0];
+        raw.u[1] = p[1];
+    } else {
+        raw.u[0] = *reinterpret_cast<const u32x4_a2*>(static_cast<const uint16_t*>(x) + at);
+    }
+}
+template <int TYPE>
+__device__ __forceinline__ void raw_use(const MxRaw<TYPE>& raw, float (&v)[8]) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        if constexpr (TYPE == MARL_F32) v[k] = bits_f(raw.u[k >> 2][k & 3]);
+        else if constexpr (TYPE == MARL_BF16) v[k] = bits_f(k & 1 ? raw.u[0][k >> 1] & 0xFFFF0000u : raw.u[0][k >> 1] << 16);
+        else v[k] = k & 1 ? half_hi(raw.u[0][k >> 1]) : half_lo(raw.u[0][k >> 1]);
+    }
+}
+
+template <int KS, int IN, int OUT, int WN>
 __global__ void __launch_bounds__(512)
 mx_rows_kernel(MxLinear P) {
+    typedef MxTile<WN> T;
     constexpr int NB = KS * 4;             // blocks of a row, padded to whole matrix instructions
     constexpr int PITCH = NB * 16 + 16;    // LDS bytes per row of codes; the 16 keep a wave's rows apart in the banks
-    __shared__ __align__(16) uint8_t codes[2][MX_TILE][PITCH];
-    __shared__ __align__(16) uint8_t scales[2][MX_TILE][16];  // [block % 4][block / 4]: a lane's scales are one word
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-    const int n0 = (blockIdx.y * (blockDim.x >> 6) + wave) * 64;
+    constexpr int ITEMS = T::ROWS * NB * (IN == MARL_MXFP4 ? 1 : 4) / 512 > 0 ? T::ROWS * NB * (IN == MARL_MXFP4 ? 1 : 4) / 512 : 1;
+    constexpr bool AHEAD = ITEMS <= 4;     // whether the next tile's values fit in registers meanwhile
+    __shared__ __align__(16) uint8_t codes[2][T::ROWS][PITCH];
+    __shared__ __align__(16) uint8_t scales[2][T::ROWS][16];  // [block % 4][block / 4]: a lane's scales are one word
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
+    const int n0 = (blockIdx.y * WN + wave % WN) * 64, wm = wave / WN * 16 * T::GROUPS;
     u32x4 w[4][KS];
     int ws[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-        const int n = n0 + 16 * (r >> 2) + 4 * t + (r & 3);
+        const int n = n0 + mx_feature<OUT>(t, r >> 2) + (r & 3);
         uint32_t s = 0;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
@@ -183,47 +241,85 @@ mx_rows_kernel(MxLinear P) {
     }
     float bias[16];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) bias[k] = P.bias && n0 + 16 * g + k < P.out ? P.bias[n0 + 16 * g + k] : 0.0f;
+    for (int k = 0; k < 16; ++k) {
+        const int n = n0 + mx_feature<OUT>(k >> 2, g) + (k & 3);
+        bias[k] = P.bias && n < P.out ? P.bias[n] : 0.0f;
+    }
 
-    const int64_t tiles = (P.rows + MX_TILE - 1) / MX_TILE;
+    // An item: 8 values of a block (float rows) or a whole block (codes).  Rows and blocks behind the end read what there is
+    // at the end (every path makes the same loads), rows give results that are not stored, blocks count as zeros.
+    MxRaw<IN == MARL_MXFP4 ? MARL_BF16 : IN> raw[AHEAD ? ITEMS : 1];
+    uint32_t raw_s[AHEAD ? ITEMS : 1];
+    const auto load = [&](int64_t tile, int q, int slot) {
+        const int it = tid + q * 512;
+        if constexpr (IN == MARL_MXFP4) {
+            const int64_t m = min(tile * T::ROWS + it / NB, P.rows - 1) * P.blocks + min(it % NB, P.blocks - 1);
+            raw[slot].u[0] = reinterpret_cast<const u32x4*>(P.x)[m];
+            raw_s[slot] = P.x_scales[m];
+        } else {
+            const int64_t m = min(tile * T::ROWS + (it >> 2) / NB, P.rows - 1);
+            raw_load<IN>(raw[slot], P.x, m * P.pitch + min((it >> 2) % NB * LB_BLOCK + (it & 3) * 8, P.cols - 8));
+        }
+    };
+    const auto quantise = [&](int q, int slot, int buf) {
+        const int it = tid + q * 512;
+        if (T::ROWS * NB * (IN == MARL_MXFP4 ? 1 : 4) < 512 && it >= T::ROWS * NB * (IN == MARL_MXFP4 ? 1 : 4)) return;
+        if constexpr (IN == MARL_MXFP4) {
+            const int row = it / NB, b = it % NB;
+            const bool there = b < P.blocks;
+            *reinterpret_cast<u32x4*>(&codes[buf][row][b * 16]) = there ? raw[slot].u[0] : u32x4{0, 0, 0, 0};
+            scales[buf][row][(b & 3) * 4 + (b >> 2)] = (uint8_t)(there ? raw_s[slot] : 127u);
+        } else {
+            const int quarter = it & 3, b = (it >> 2) % NB, row = (it >> 2) / NB;
+            float v[8];
+            raw_use<IN>(raw[slot], v);
+            const int n = P.cols - b * LB_BLOCK - quarter * 8;  // how many of the eight exist
+            if (n < 8) {  // what was read are the row's last eight: move them down
+#pragma unroll
+                for (int step = 4; step >= 1; step >>= 1)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) v[k] = (8 - n) & step ? (k + step < 8 ? v[k + step] : 0.0f) : v[k];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] = n <= 0 ? 0.0f : v[k];
+            }
+            const uint32_t byte = mx_scale_byte(quad_max(abs_top(v)));
+            *reinterpret_cast<uint32_t*>(&codes[buf][row][b * 16 + quarter * 4]) = mx_codes(v, byte);
+            if (quarter == 0) scales[buf][row][(b & 3) * 4 + (b >> 2)] = (uint8_t)byte;
+        }
+    };
+
+    const int64_t tiles = (P.rows + T::ROWS - 1) / T::ROWS;
+    if constexpr (AHEAD) {
+#pragma unroll
+        for (int q = 0; q < ITEMS; ++q) load(blockIdx.x, q, q);
+    }
     int buf = 0;
     for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, buf ^= 1) {
-        if constexpr (IN == MARL_MXFP4) {
-            for (int it = threadIdx.x; it < MX_TILE * NB; it += blockDim.x) {
-                const int row = it / NB, b = it % NB;
-                const int64_t m = tile * MX_TILE + row;
-                *reinterpret_cast<u32x4*>(&codes[buf][row][b * 16]) = mx_block(static_cast<const uint8_t*>(P.x), m, P.rows, b, P.blocks);
-                scales[buf][row][(b & 3) * 4 + (b >> 2)] = (uint8_t)mx_scale(P.x_scales, m, P.rows, b, P.blocks);
-            }
-        } else {
-            for (int it = threadIdx.x; it < MX_TILE * NB * 4; it += blockDim.x) {
-                const int quarter = it & 3, b = (it >> 2) % NB, row = (it >> 2) / NB;
-                const int64_t m = tile * MX_TILE + row;
-                float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-                if (m < P.rows) load_eight<IN>(P.x, m * P.pitch + (int64_t)b * LB_BLOCK + quarter * 8, m * P.pitch + P.cols, v);
-                const uint32_t byte = mx_scale_byte(quad_max(abs_top(v)));
-                *reinterpret_cast<uint32_t*>(&codes[buf][row][b * 16 + quarter * 4]) = mx_codes(v, byte);
-                if (quarter == 0) scales[buf][row][(b & 3) * 4 + (b >> 2)] = (uint8_t)byte;
-            }
+#pragma unroll
+        for (int q = 0; q < ITEMS; ++q) {
+            if constexpr (!AHEAD) load(tile, q, 0);
+            quantise(q, AHEAD ? q : 0, buf);
+            if constexpr (AHEAD) load(tile + gridDim.x, q, q);
         }
         __syncthreads();  // one barrier a tile: the other buffer is free once every wave has come here
 #pragma unroll
-        for (int rt = 0; rt < MX_TILE / 16; ++rt) {
+        for (int rt = 0; rt < T::GROUPS; ++rt) {
             f32x4 acc[4];
 #pragma unroll
             for (int t = 0; t < 4; ++t) acc[t] = f32x4{0, 0, 0, 0};
-            const int xs = *reinterpret_cast<const int*>(&scales[buf][rt * 16 + r][g * 4]);
+            const int row = wm + rt * 16 + r;
+            const int xs = *reinterpret_cast<const int*>(&scales[buf][row][g * 4]);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                const u32x4 x = *reinterpret_cast<const u32x4*>(&codes[buf][rt * 16 + r][(ks * 4 + g) * 16]);
+                const u32x4 x = *reinterpret_cast<const u32x4*>(&codes[buf][row][(ks * 4 + g) * 16]);
 #pragma unroll
                 for (int t = 0; t < 4; ++t) acc[t] = mx_mfma(w[t][ks], x, acc[t], ks, ws[t], xs);
             }
             float v[16];
 #pragma unroll
             for (int k = 0; k < 16; ++k) v[k] = acc[k >> 2][k & 3] + bias[k];
-            const int64_t m = tile * MX_TILE + rt * 16 + r;
-            mx_store<OUT>(P, m, m < P.rows, n0 + 16 * g, v);
+            const int64_t m = tile * T::ROWS + row;
+            mx_store<OUT>(P, m, m < P.rows, n0, g, v);
         }
     }
 }
@@ -253,7 +349,7 @@ mx_stream_kernel(MxLinear P) {
         int ws[4], xs[RM];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            const int n = n0 + 16 * (r >> 2) + 4 * t + (r & 3);
+            const int n = n0 + mx_feature<OUT>(t, r >> 2) + (r & 3);
             w[t] = mx_block(P.w, n, P.out, b, P.blocks);
             ws[t] = (int)mx_scale(P.w_scales, n, P.out, b, P.blocks);
         }
@@ -281,17 +377,21 @@ mx_stream_kernel(MxLinear P) {
 #pragma unroll
         for (int k = 0; k < 16; ++k) v[k] = ((acc[q][k >> 2][k & 3] + sums[0][q][lane][k]) + sums[1][q][lane][k]) + sums[2][q][lane][k];
         const int64_t m = m0 + q * 16 + r;
-        const int n = n0 + 16 * g;
         if (P.splits > 1) {
             if (m >= P.rows) continue;
             float* part = P.part + ((int64_t)blockIdx.z * P.rows + m) * P.out;
 #pragma unroll
-            for (int k = 0; k < 16; ++k)
-                if (n + k < P.out) part[n + k] = v[k];
+            for (int k = 0; k < 16; ++k) {
+                const int n = n0 + mx_feature<OUT>(k >> 2, g) + (k & 3);
+                if (n < P.out) part[n] = v[k];
+            }
         } else {
 #pragma unroll
-            for (int k = 0; k < 16; ++k) v[k] += P.bias && n + k < P.out ? P.bias[n + k] : 0.0f;
-            mx_store<OUT>(P, m, m < P.rows, n, v);
+            for (int k = 0; k < 16; ++k) {
+                const int n = n0 + mx_feature<OUT>(k >> 2, g) + (k & 3);
+                v[k] += P.bias && n < P.out ? P.bias[n] : 0.0f;
+            }
+            mx_store<OUT>(P, m, m < P.rows, n0, g, v);
         }
     }
 }
@@ -333,7 +433,8 @@ mx_join_kernel(MxLinear P) {
 
 // ------------------------------------------------------------------------------------------------------------ host
 
-constexpr int MX_ROWS_COLS = 512;   // longest row of mx_rows_kernel: four matrix instructions
+// rows that mx_rows_kernel takes: its loads are eight values wide, its weight registers hold four matrix instructions
+static bool mx_short_rows(int64_t cols) { return cols >= 8 && cols <= 512; }
 
 static hipError_t launch_quantize(const void* x, int type, int64_t rows, int cols, int64_t pitch, uint8_t* codes,
                                   uint8_t* scales, hipStream_t stream) {
@@ -343,31 +444,30 @@ static hipError_t launch_quantize(const void* x, int type, int64_t rows, int col
     return hipGetLastError();
 }
 
-template <int KS, int IN>
+template <int KS, int WN, int IN>
 static void (*rows_kernel_out(int out))(MxLinear) {
     switch (out) {
-        case MARL_F32: return mx_rows_kernel<KS, IN, MARL_F32>;
-        case MARL_BF16: return mx_rows_kernel<KS, IN, MARL_BF16>;
-        case MARL_F16: return mx_rows_kernel<KS, IN, MARL_F16>;
-        default: return mx_rows_kernel<KS, IN, MARL_MXFP4>;
+        case MARL_F32: return mx_rows_kernel<KS, IN, MARL_F32, WN>;
+        case MARL_BF16: return mx_rows_kernel<KS, IN, MARL_BF16, WN>;
+        case MARL_F16: return mx_rows_kernel<KS, IN, MARL_F16, WN>;
+        default: return mx_rows_kernel<KS, IN, MARL_MXFP4, WN>;
     }
+}
+template <int KS, int WN>
+static void launch_rows(const MxLinear& P, int in, int out, hipStream_t stream) {
+    auto kernel = in == MARL_F32 ? rows_kernel_out<KS, WN, MARL_F32>(out) : in == MARL_BF16 ? rows_kernel_out<KS, WN, MARL_BF16>(out)
+                : in == MARL_F16 ? rows_kernel_out<KS, WN, MARL_F16>(out) : rows_kernel_out<KS, WN, MARL_MXFP4>(out);
+    const int64_t tiles = (P.rows + MxTile<WN>::ROWS - 1) / MxTile<WN>::ROWS;
+    const int64_t resident = 512;  // two workgroups a compute unit
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)(tiles < resident ? tiles : resident), (P.out + 64 * WN - 1) / (64 * WN)), dim3(512), 0, stream, P);
 }
 template <int KS>
-static void (*rows_kernel_in(int in, int out))(MxLinear) {
-    switch (in) {
-        case MARL_F32: return rows_kernel_out<KS, MARL_F32>(out);
-        case MARL_BF16: return rows_kernel_out<KS, MARL_BF16>(out);
-        case MARL_F16: return rows_kernel_out<KS, MARL_F16>(out);
-        default: return rows_kernel_out<KS, MARL_MXFP4>(out);
-    }
-}
-static void (*rows_kernel(int ks, int in, int out))(MxLinear) {
-    switch (ks) {
-        case 1: return rows_kernel_in<1>(in, out);
-        case 2: return rows_kernel_in<2>(in, out);
-        case 3: return rows_kernel_in<3>(in, out);
-        default: return rows_kernel_in<4>(in, out);
-    }
+static void launch_rows_wide(const MxLinear& P, int in, int out, hipStream_t stream) {
+    // Side by side as many waves as there are features for, so that a row is quantised once; with few rows, where that
+    // would leave most of the chip without work, two.
+    if (P.out <= 128 || P.rows <= 1024) launch_rows<KS, 2>(P, in, out, stream);
+    else if (P.out <= 256) launch_rows<KS, 4>(P, in, out, stream);
+    else launch_rows<KS, 8>(P, in, out, stream);
 }
 template <int RM>
 static void (*stream_kernel(int out))(MxLinear) {
@@ -379,7 +479,7 @@ static void (*stream_kernel(int out))(MxLinear) {
     }
 }
 
-// How a call over rows longer than MX_ROWS_COLS is cut: row groups per workgroup and splits of the row.
+// How a call over other rows is cut: row groups per workgroup and splits of the row.
 struct MxCut { int rm; int splits; };
 static MxCut mx_cut(int64_t rows, int64_t cols, int out) {
     MxCut c;
@@ -395,13 +495,9 @@ static size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 
 static hipError_t launch_linear(const MxLinear& P0, int x_type, int out_type, uint8_t* ws, hipStream_t stream) {
     MxLinear P = P0;
-    if (P.cols <= MX_ROWS_COLS) {
-        const int waves = P.out >= 512 ? 8 : (P.out + 63) / 64;
-        const int ky = (P.out + 64 * waves - 1) / (64 * waves);
-        const int64_t tiles = (P.rows + MX_TILE - 1) / MX_TILE;
-        const int64_t resident = 256 * (16 / waves);  // four waves per SIMD
-        const int64_t gx = tiles < resident ? tiles : resident;
-        hipLaunchKernelGGL(rows_kernel((P.blocks + 3) / 4, x_type, out_type), dim3((uint32_t)gx, ky), dim3(64 * waves), 0, stream, P);
+    if (mx_short_rows(P.cols)) {
+        if (P.blocks <= 8) launch_rows_wide<2>(P, x_type, out_type, stream);
+        else launch_rows_wide<4>(P, x_type, out_type, stream);
         return hipGetLastError();
     }
     const MxCut c = mx_cut(P.rows, P.cols, P.out);
@@ -469,7 +565,7 @@ extern "C" int marl_mx_dequantize(const uint8_t* d_codes, const uint8_t* d_scale
 }
 
 extern "C" size_t marl_mx_linear_workspace_bytes(int x_type, int64_t num_rows, int num_cols, int num_out) {
-    if (num_rows <= 0 || num_cols <= MX_ROWS_COLS || num_out <= 0) return 0;
+    if (num_rows <= 0 || num_cols <= 0 || mx_short_rows(num_cols) || num_out <= 0) return 0;
     const MxCut c = mx_cut(num_rows, num_cols, num_out);
     size_t n = 0;
     if (x_type != MARL_MXFP4) n += up16((size_t)num_rows * lb_blocks(num_cols) * 16) + up16((size_t)num_rows * lb_blocks(num_cols));
@@ -496,8 +592,8 @@ extern "C" int marl_mx_linear(const void* d_x, const uint8_t* d_x_scales, int x_
         return set_error(MARL_ERR_INVALID, "codes and the workspace must be 16-byte aligned, the others aligned to their elements");
     if (too_many_blocks(num_rows, num_cols) || too_many_blocks(num_rows, num_out) || num_out > (1 << 22))
         return set_error(MARL_ERR_INVALID, "fewer than 2^30 blocks of 32 values on either side and at most 2^22 output features in one call");
-    if (num_cols > MX_ROWS_COLS && num_rows > (int64_t)65535 * 64)
-        return set_error(MARL_ERR_INVALID, "of rows of more than 512 values at most 4,194,240 in one call");
+    if (!mx_short_rows(num_cols) && num_rows > (int64_t)65535 * 64)
+        return set_error(MARL_ERR_INVALID, "of rows of fewer than 8 or more than 512 values at most 4,194,240 in one call");
     if (marl_mx_linear_workspace_bytes(x_type, num_rows, num_cols, num_out) != 0 && !d_workspace)
         return set_error(MARL_ERR_INVALID, "this size needs d_workspace (marl_mx_linear_workspace_bytes bytes)");
     MxLinear P;
