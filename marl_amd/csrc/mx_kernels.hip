@@ -246,8 +246,9 @@ mx_rows_kernel(MxLinear P) {
         bias[k] = P.bias && n < P.out ? P.bias[n] : 0.0f;
     }
 
-    // An item: 8 values of a block (float rows) or a whole block (codes).  Rows and blocks behind the end read what there is
-    // at the end (every path makes the same loads), rows give results that are not stored, blocks count as zeros.
+    // An item: 8 values of a block (float rows) or a whole block (codes).  Rows behind the last are the last again, their
+    // results are not stored; every path makes the same loads.
+    const int64_t all = (P.rows - 1) * P.pitch + P.cols;  // elements from the first row's start to the last one's end
     MxRaw<IN == MARL_MXFP4 ? MARL_BF16 : IN> raw[AHEAD ? ITEMS : 1];
     uint32_t raw_s[AHEAD ? ITEMS : 1];
     const auto load = [&](int64_t tile, int q, int slot) {
@@ -258,10 +259,10 @@ mx_rows_kernel(MxLinear P) {
             raw_s[slot] = P.x_scales[m];
         } else {
             const int64_t m = min(tile * T::ROWS + (it >> 2) / NB, P.rows - 1);
-            raw_load<IN>(raw[slot], P.x, m * P.pitch + min((it >> 2) % NB * LB_BLOCK + (it & 3) * 8, P.cols - 8));
+            raw_load<IN>(raw[slot], P.x, min(m * P.pitch + (it >> 2) % NB * LB_BLOCK + (it & 3) * 8, all - 8));
         }
     };
-    const auto quantise = [&](int q, int slot, int buf) {
+    const auto quantise = [&](int64_t tile, int q, int slot, int buf) {
         const int it = tid + q * 512;
         if (T::ROWS * NB * (IN == MARL_MXFP4 ? 1 : 4) < 512 && it >= T::ROWS * NB * (IN == MARL_MXFP4 ? 1 : 4)) return;
         if constexpr (IN == MARL_MXFP4) {
@@ -273,15 +274,18 @@ mx_rows_kernel(MxLinear P) {
             const int quarter = it & 3, b = (it >> 2) % NB, row = (it >> 2) / NB;
             float v[8];
             raw_use<IN>(raw[slot], v);
-            const int n = P.cols - b * LB_BLOCK - quarter * 8;  // how many of the eight exist
-            if (n < 8) {  // what was read are the row's last eight: move them down
+            // What lies behind a row's end is the next row, and counts as 0; only behind the last row there is nothing, and
+            // its last values were read as the tensor's last eight: move them down.
+            const int64_t back = min(tile * T::ROWS + row, P.rows - 1) * P.pitch + b * LB_BLOCK + quarter * 8 - (all - 8);
+            if (back > 0) {
 #pragma unroll
                 for (int step = 4; step >= 1; step >>= 1)
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) v[k] = (8 - n) & step ? (k + step < 8 ? v[k + step] : 0.0f) : v[k];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) v[k] = n <= 0 ? 0.0f : v[k];
+                    for (int k = 0; k < 8; ++k) v[k] = back & step ? (k + step < 8 ? v[k + step] : 0.0f) : v[k];
             }
+            const int n = P.cols - b * LB_BLOCK - quarter * 8;  // how many of the eight exist
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = k < n ? v[k] : 0.0f;
             const uint32_t byte = mx_scale_byte(quad_max(abs_top(v)));
             *reinterpret_cast<uint32_t*>(&codes[buf][row][b * 16 + quarter * 4]) = mx_codes(v, byte);
             if (quarter == 0) scales[buf][row][(b & 3) * 4 + (b >> 2)] = (uint8_t)byte;
@@ -298,7 +302,7 @@ mx_rows_kernel(MxLinear P) {
 #pragma unroll
         for (int q = 0; q < ITEMS; ++q) {
             if constexpr (!AHEAD) load(tile, q, 0);
-            quantise(q, AHEAD ? q : 0, buf);
+            quantise(tile, q, AHEAD ? q : 0, buf);
             if constexpr (AHEAD) load(tile + gridDim.x, q, q);
         }
         __syncthreads();  // one barrier a tile: the other buffer is free once every wave has come here
@@ -325,43 +329,78 @@ mx_rows_kernel(MxLinear P) {
 }
 
 // Any length: x is quantised already.  A workgroup has 64 features and 16 RM rows; its four waves take every fourth
-// step of 128 values of its share of the row and add their sums through LDS.  With few rows the row is also split over
+// stretch of 512 values of its share of the row and add their sums through LDS.  With few rows the row is also split over
 // workgroups (grid z): the weight, read once, is what such a call costs, and it takes many loads in flight.
+// Which block goes to which of a stretch's four instructions is free as long as both operands agree: lane group g has
+// blocks 4 g .. 4 g + 3, so that a lane reads 64 neighbouring bytes of codes and its four scales as one word, and the
+// lanes of a row 256 bytes.
 template <int RM, int OUT>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 2)
 mx_stream_kernel(MxLinear P) {
     __shared__ float sums[3][RM][64][17];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
     const int n0 = blockIdx.x * 64;
     const int64_t m0 = (int64_t)blockIdx.y * (16 * RM);
-    const int steps = (P.blocks + 3) / 4;
-    const int per = (steps + P.splits - 1) / P.splits;
-    const int first = blockIdx.z * per, last = min(steps, first + per);
+    const int stretches = (P.blocks + 15) / 16;
+    const int per = (stretches + P.splits - 1) / P.splits;
+    const int first = blockIdx.z * per, last = min(stretches, first + per);
     f32x4 acc[RM][4];
 #pragma unroll
     for (int q = 0; q < RM; ++q)
 #pragma unroll
         for (int t = 0; t < 4; ++t) acc[q][t] = f32x4{0, 0, 0, 0};
+    // rows and features behind the last are the last again, their results are not stored
+    int64_t wrow[4], xrow[RM];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) wrow[t] = (int64_t)min(n0 + mx_feature<OUT>(t, r >> 2) + (r & 3), P.out - 1) * P.blocks + 4 * g;
+#pragma unroll
+    for (int q = 0; q < RM; ++q) xrow[q] = min(m0 + q * 16 + r, P.rows - 1) * P.blocks + 4 * g;
     const uint8_t* xc = static_cast<const uint8_t*>(P.x);
     for (int s = first + wave; s < last; s += 4) {
-        const int b = s * 4 + g;
-        u32x4 w[4], x[RM];
-        int ws[4], xs[RM];
+        const int b = s * 16;
+        u32x4 w[4][4], x[RM][4];
+        uint32_t ws[4], xs[RM];
+        if (b + 16 <= P.blocks) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const int n = n0 + mx_feature<OUT>(t, r >> 2) + (r & 3);
-            w[t] = mx_block(P.w, n, P.out, b, P.blocks);
-            ws[t] = (int)mx_scale(P.w_scales, n, P.out, b, P.blocks);
+            for (int q = 0; q < RM; ++q) {
+                xs[q] = *reinterpret_cast<const u32_a1*>(P.x_scales + xrow[q] + b);
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks) x[q][ks] = *reinterpret_cast<const u32x4*>(xc + (xrow[q] + b + ks) * 16);
+            }
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                ws[t] = *reinterpret_cast<const u32_a1*>(P.w_scales + wrow[t] + b);
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks) w[t][ks] = *reinterpret_cast<const u32x4*>(P.w + (wrow[t] + b + ks) * 16);
+            }
+        } else {  // the last stretch of a row: blocks behind its end are its last one again, and zeros in x
+#pragma unroll
+            for (int q = 0; q < RM; ++q) xs[q] = 0;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) ws[t] = 0;
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+                const bool there = b + 4 * g + ks < P.blocks;
+                const int64_t at = min(b + 4 * g + ks, P.blocks - 1) - 4 * g;
+#pragma unroll
+                for (int q = 0; q < RM; ++q) {
+                    const u32x4 v = *reinterpret_cast<const u32x4*>(xc + (xrow[q] + at) * 16);
+                    x[q][ks] = there ? v : u32x4{0, 0, 0, 0};
+                    xs[q] |= (there ? (uint32_t)P.x_scales[xrow[q] + at] : 127u) << (8 * ks);
+                }
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    w[t][ks] = *reinterpret_cast<const u32x4*>(P.w + (wrow[t] + at) * 16);
+                    ws[t] |= (uint32_t)P.w_scales[wrow[t] + at] << (8 * ks);
+                }
+            }
         }
 #pragma unroll
-        for (int q = 0; q < RM; ++q) {
-            x[q] = mx_block(xc, m0 + q * 16 + r, P.rows, b, P.blocks);
-            xs[q] = (int)mx_scale(P.x_scales, m0 + q * 16 + r, P.rows, b, P.blocks);
-        }
+        for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
-        for (int q = 0; q < RM; ++q)
+            for (int q = 0; q < RM; ++q)
 #pragma unroll
-            for (int t = 0; t < 4; ++t) acc[q][t] = mx_mfma(w[t], x[q], acc[q][t], 0, ws[t], xs[q]);
+                for (int t = 0; t < 4; ++t) acc[q][t] = mx_mfma(w[t][ks], x[q][ks], acc[q][t], ks, (int)ws[t], (int)xs[q]);
     }
     if (wave) {
 #pragma unroll
@@ -396,28 +435,40 @@ mx_stream_kernel(MxLinear P) {
     }
 }
 
-// Sums of the splits in their order, then bias, ReLU and the output's type.  Four lanes per 32 features, as in quantising.
+// Sums of the splits, then bias, ReLU and the output's type.  Four lanes per 32 features, as in quantising; a workgroup's
+// four waves have every fourth split each, and their four sums are added in order.
 template <int OUT>
 __global__ void __launch_bounds__(256)
 mx_join_kernel(MxLinear P) {
-    const int yb = (P.out + LB_BLOCK - 1) / LB_BLOCK;
+    __shared__ float sums[3][8][64];
+    const int yb = (P.out + LB_BLOCK - 1) / LB_BLOCK, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int64_t m;
     int b, quarter;
-    split_block(blockIdx.x * 256 + threadIdx.x, (uint32_t)yb, m, b, quarter);
-    if (m >= P.rows) return;
+    split_block(blockIdx.x * 64 + lane, (uint32_t)yb, m, b, quarter);
     const int n = b * LB_BLOCK + quarter * 8;
+    const bool live = m < P.rows && n < P.out;
     float v[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = 0.0f;
-    for (int s = 0; s < P.splits; ++s) {
-        const int64_t row = ((int64_t)s * P.rows + m) * P.out;
-        float p[8];
-        load_eight<MARL_F32>(P.part, row + n, row + P.out, p);
+    if (live) {
+        const int64_t step = P.rows * P.out;
+#pragma unroll 4
+        for (int s = wave; s < P.splits; s += 4) {
+            float p[8];
+            load_eight<MARL_F32>(P.part, s * step + m * P.out + n, s * step + m * P.out + P.out, p);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] += p[k];
+            for (int k = 0; k < 8; ++k) v[k] += p[k];
+        }
     }
+    if (wave) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sums[wave - 1][k][lane] = v[k];
+    }
+    __syncthreads();
+    if (wave || m >= P.rows) return;  // whole quads leave together
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
+        v[k] = (v[k] + sums[0][k][lane]) + (sums[1][k][lane] + sums[2][k][lane]);
         if (n + k >= P.out) { v[k] = 0.0f; continue; }
         if (P.bias) v[k] += P.bias[n + k];
         if (P.relu) v[k] = v[k] < 0.0f ? 0.0f : v[k];
@@ -426,7 +477,7 @@ mx_join_kernel(MxLinear P) {
         const uint32_t byte = mx_scale_byte(quad_max(abs_top(v)));
         reinterpret_cast<uint32_t*>(P.y)[(m * yb + b) * 4 + quarter] = mx_codes(v, byte);
         if (quarter == 0) P.y_scales[m * yb + b] = (uint8_t)byte;
-    } else {
+    } else if (n < P.out) {
         store_eight<OUT>(P.y, m * P.out + n, m * P.out + P.out, v);
     }
 }
@@ -458,7 +509,10 @@ static void launch_rows(const MxLinear& P, int in, int out, hipStream_t stream) 
     auto kernel = in == MARL_F32 ? rows_kernel_out<KS, WN, MARL_F32>(out) : in == MARL_BF16 ? rows_kernel_out<KS, WN, MARL_BF16>(out)
                 : in == MARL_F16 ? rows_kernel_out<KS, WN, MARL_F16>(out) : rows_kernel_out<KS, WN, MARL_MXFP4>(out);
     const int64_t tiles = (P.rows + MxTile<WN>::ROWS - 1) / MxTile<WN>::ROWS;
-    const int64_t resident = 512;  // two workgroups a compute unit
+    // One workgroup a compute unit: two read the weight twice and are slower where results are written out in full (131072
+    // x 512 -> 256 in float32: 87 against 90 us; 21847 x 420 -> 250 in bfloat16: 15 against 18); MXFP4 results are small
+    // and leave the conversions, which two overlap (131072 x 202 -> 512: 48 against 41 us).
+    const int64_t resident = out == MARL_MXFP4 ? 512 : 256;
     hipLaunchKernelGGL(kernel, dim3((uint32_t)(tiles < resident ? tiles : resident), (P.out + 64 * WN - 1) / (64 * WN)), dim3(512), 0, stream, P);
 }
 template <int KS>
@@ -479,16 +533,20 @@ static void (*stream_kernel(int out))(MxLinear) {
     }
 }
 
+constexpr int64_t MX_SPLIT_GROUPS = 512;  // two workgroups a compute unit
+
 // How a call over other rows is cut: row groups per workgroup and splits of the row.
 struct MxCut { int rm; int splits; };
 static MxCut mx_cut(int64_t rows, int64_t cols, int out) {
     MxCut c;
     c.rm = rows <= 16 ? 1 : 4;
-    const int64_t steps = ((int64_t)lb_blocks(cols) + 3) / 4;
+    const int64_t stretches = ((int64_t)lb_blocks(cols) + 15) / 16;
     const int64_t groups = ((out + 63) / 64) * ((rows + 16 * c.rm - 1) / (16 * c.rm));
-    const int64_t most = steps / 8 < 1 ? 1 : steps / 8;  // at least two steps for each of a workgroup's four waves
-    int64_t s = 1024 / groups;                           // four workgroups per compute unit
-    c.splits = (int)(s < 1 ? 1 : s > most ? most : s);
+    const int64_t most = stretches / 8 < 1 ? 1 : stretches / 8;  // two stretches for each of a workgroup's four waves
+    int64_t s = MX_SPLIT_GROUPS / groups;
+    s = s < 1 ? 1 : s > most ? most : s;
+    const int64_t per = (stretches + s - 1) / s;
+    c.splits = (int)((stretches + per - 1) / per);
     return c;
 }
 static size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
@@ -519,7 +577,7 @@ static hipError_t launch_linear(const MxLinear& P0, int x_type, int out_type, ui
     if (e != hipSuccess || c.splits == 1) return e;
     auto join = out_type == MARL_F32 ? mx_join_kernel<MARL_F32> : out_type == MARL_BF16 ? mx_join_kernel<MARL_BF16>
               : out_type == MARL_F16 ? mx_join_kernel<MARL_F16> : mx_join_kernel<MARL_MXFP4>;
-    hipLaunchKernelGGL(join, dim3(block_grid(P.rows, P.out)), dim3(256), 0, stream, P);
+    hipLaunchKernelGGL(join, dim3((uint32_t)((P.rows * lb_blocks(P.out) * 4 + 63) / 64)), dim3(256), 0, stream, P);
     return hipGetLastError();
 }
 
