@@ -96,7 +96,7 @@ struct MxLinear {
     int relu;
     void* y;
     uint8_t* y_scales;        // MXFP4 output only
-    float* part;              // [splits][rows][out] partial sums (mx_stream_kernel with splits > 1)
+    float* part;              // [splits][rows][out] sums of the row's shares
     int splits;
 };
 
@@ -328,21 +328,87 @@ mx_rows_kernel(MxLinear P) {
     }
 }
 
-// Any length: x is quantised already.  A workgroup has 64 features and 16 RM rows; its four waves take every fourth
-// stretch of 512 values of its share of the row and add their sums through LDS.  With few rows the row is also split over
-// workgroups (grid z): the weight, read once, is what such a call costs, and it takes many loads in flight.
-// Which block goes to which of a stretch's four instructions is free as long as both operands agree: lane group g has
-// blocks 4 g .. 4 g + 3, so that a lane reads 64 neighbouring bytes of codes and its four scales as one word, and the
-// lanes of a row 256 bytes.
-template <int RM, int OUT>
+// Up to 16 rows of any length (a joint observation): the weight, read once, is what such a call costs.  A workgroup has 16
+// features and a share of the row (grid y), its four waves every fourth chunk of 2048 values each, whose 64 loads of 1 KiB
+// are under way together; the sums of the shares are joined by mx_join_kernel.
+// Which block goes to which matrix instruction is free as long as both operands agree: of a stretch of 512 values lane group
+// g has blocks 4 g .. 4 g + 3, so that a lane reads 64 neighbouring bytes of codes and its four scales as one word, and the
+// four lanes of a row 256 bytes, a wave 1 KiB of each of its 16 rows.  (With 64 features to a wave and 256 bytes of each row
+// at a time, 1 x 827392 -> 512 took 57 us.)
+struct MxStretch { u32x4 c[4]; uint32_t s; };
+__device__ __forceinline__ void load_stretch(MxStretch& v, const uint8_t* codes, const uint8_t* scales, int64_t at) {
+    v.s = *reinterpret_cast<const u32_a1*>(scales + at);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) v.c[ks] = *reinterpret_cast<const u32x4*>(codes + (at + ks) * 16);
+}
+// a row's last stretch: block b + ks of `blocks`, those behind the end are the last one again, and zeros if `zero`
+__device__ __forceinline__ void load_last_stretch(MxStretch& v, const uint8_t* codes, const uint8_t* scales, int64_t row, int b, int blocks, bool zero) {
+    v.s = 0;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+        const bool there = b + ks < blocks || !zero;
+        const int64_t at = row + min(b + ks, blocks - 1);
+        const u32x4 c = *reinterpret_cast<const u32x4*>(codes + at * 16);
+        v.c[ks] = there ? c : u32x4{0, 0, 0, 0};
+        v.s |= (there ? (uint32_t)scales[at] : 127u) << (8 * ks);
+    }
+}
+
+__global__ void __launch_bounds__(256, 2)
+mx_few_rows_kernel(MxLinear P) {
+    __shared__ f32x4 sums[3][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+    const int n0 = blockIdx.x * 16;
+    const int chunks = (P.blocks + 63) / 64, per = (chunks + P.splits - 1) / P.splits;
+    const int first = blockIdx.y * per, last = min(chunks, first + per);
+    const int64_t wrow = (int64_t)min(n0 + r, P.out - 1) * P.blocks, xrow = min((int64_t)r, P.rows - 1) * P.blocks;
+    const uint8_t* xc = static_cast<const uint8_t*>(P.x);
+    f32x4 acc[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) acc[u] = f32x4{0, 0, 0, 0};
+    for (int c = first + wave; c < last; c += 4) {
+        MxStretch w[4], x[4];
+        const int b = c * 64 + 4 * g;
+        if (c * 64 + 64 <= P.blocks) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) load_stretch(w[u], P.w, P.w_scales, wrow + b + 16 * u);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) load_stretch(x[u], xc, P.x_scales, xrow + b + 16 * u);
+        } else {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                load_last_stretch(w[u], P.w, P.w_scales, wrow, b + 16 * u, P.blocks, false);
+                load_last_stretch(x[u], xc, P.x_scales, xrow, b + 16 * u, P.blocks, true);
+            }
+        }
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) acc[u] = mx_mfma(w[u].c[ks], x[u].c[ks], acc[u], ks, (int)w[u].s, (int)x[u].s);
+    }
+    f32x4 v = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+    if (wave) sums[wave - 1][lane] = v;
+    __syncthreads();
+    if (wave || r >= P.rows) return;
+    v = (v + sums[0][lane]) + (sums[1][lane] + sums[2][lane]);
+    float* part = P.part + ((int64_t)blockIdx.y * P.rows + r) * P.out + n0 + 4 * g;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (n0 + 4 * g + k < P.out) part[k] = v[k];
+}
+
+// More rows of any length: 64 features and 64 rows to a workgroup, whose four waves take every fourth stretch of 512 values
+// each and add their sums through LDS; with few workgroups the row is split over them too (grid z).
+constexpr int MX_RM = 4;  // groups of 16 rows
+template <int OUT>
 __global__ void __launch_bounds__(256, 2)
 mx_stream_kernel(MxLinear P) {
+    constexpr int RM = MX_RM;
     __shared__ float sums[3][RM][64][17];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
     const int n0 = blockIdx.x * 64;
     const int64_t m0 = (int64_t)blockIdx.y * (16 * RM);
-    const int stretches = (P.blocks + 15) / 16;
-    const int per = (stretches + P.splits - 1) / P.splits;
+    const int stretches = (P.blocks + 15) / 16, per = (stretches + P.splits - 1) / P.splits;
     const int first = blockIdx.z * per, last = min(stretches, first + per);
     f32x4 acc[RM][4];
 #pragma unroll
@@ -352,55 +418,30 @@ mx_stream_kernel(MxLinear P) {
     // rows and features behind the last are the last again, their results are not stored
     int64_t wrow[4], xrow[RM];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) wrow[t] = (int64_t)min(n0 + mx_feature<OUT>(t, r >> 2) + (r & 3), P.out - 1) * P.blocks + 4 * g;
+    for (int t = 0; t < 4; ++t) wrow[t] = (int64_t)min(n0 + mx_feature<OUT>(t, r >> 2) + (r & 3), P.out - 1) * P.blocks;
 #pragma unroll
-    for (int q = 0; q < RM; ++q) xrow[q] = min(m0 + q * 16 + r, P.rows - 1) * P.blocks + 4 * g;
+    for (int q = 0; q < RM; ++q) xrow[q] = min(m0 + q * 16 + r, P.rows - 1) * P.blocks;
     const uint8_t* xc = static_cast<const uint8_t*>(P.x);
     for (int s = first + wave; s < last; s += 4) {
-        const int b = s * 16;
-        u32x4 w[4][4], x[RM][4];
-        uint32_t ws[4], xs[RM];
-        if (b + 16 <= P.blocks) {
+        MxStretch w[4], x[RM];
+        const int b = s * 16 + 4 * g;
+        if (s * 16 + 16 <= P.blocks) {
 #pragma unroll
-            for (int q = 0; q < RM; ++q) {
-                xs[q] = *reinterpret_cast<const u32_a1*>(P.x_scales + xrow[q] + b);
+            for (int q = 0; q < RM; ++q) load_stretch(x[q], xc, P.x_scales, xrow[q] + b);
 #pragma unroll
-                for (int ks = 0; ks < 4; ++ks) x[q][ks] = *reinterpret_cast<const u32x4*>(xc + (xrow[q] + b + ks) * 16);
-            }
+            for (int t = 0; t < 4; ++t) load_stretch(w[t], P.w, P.w_scales, wrow[t] + b);
+        } else {
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                ws[t] = *reinterpret_cast<const u32_a1*>(P.w_scales + wrow[t] + b);
+            for (int q = 0; q < RM; ++q) load_last_stretch(x[q], xc, P.x_scales, xrow[q], b, P.blocks, true);
 #pragma unroll
-                for (int ks = 0; ks < 4; ++ks) w[t][ks] = *reinterpret_cast<const u32x4*>(P.w + (wrow[t] + b + ks) * 16);
-            }
-        } else {  // the last stretch of a row: blocks behind its end are its last one again, and zeros in x
-#pragma unroll
-            for (int q = 0; q < RM; ++q) xs[q] = 0;
-#pragma unroll
-            for (int t = 0; t < 4; ++t) ws[t] = 0;
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks) {
-                const bool there = b + 4 * g + ks < P.blocks;
-                const int64_t at = min(b + 4 * g + ks, P.blocks - 1) - 4 * g;
-#pragma unroll
-                for (int q = 0; q < RM; ++q) {
-                    const u32x4 v = *reinterpret_cast<const u32x4*>(xc + (xrow[q] + at) * 16);
-                    x[q][ks] = there ? v : u32x4{0, 0, 0, 0};
-                    xs[q] |= (there ? (uint32_t)P.x_scales[xrow[q] + at] : 127u) << (8 * ks);
-                }
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    w[t][ks] = *reinterpret_cast<const u32x4*>(P.w + (wrow[t] + at) * 16);
-                    ws[t] |= (uint32_t)P.w_scales[wrow[t] + at] << (8 * ks);
-                }
-            }
+            for (int t = 0; t < 4; ++t) load_last_stretch(w[t], P.w, P.w_scales, wrow[t], b, P.blocks, false);
         }
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
             for (int q = 0; q < RM; ++q)
 #pragma unroll
-                for (int t = 0; t < 4; ++t) acc[q][t] = mx_mfma(w[t][ks], x[q][ks], acc[q][t], ks, (int)ws[t], (int)xs[q]);
+                for (int t = 0; t < 4; ++t) acc[q][t] = mx_mfma(w[t].c[ks], x[q].c[ks], acc[q][t], ks, (int)w[t].s, (int)x[q].s);
     }
     if (wave) {
 #pragma unroll
@@ -523,30 +564,28 @@ static void launch_rows_wide(const MxLinear& P, int in, int out, hipStream_t str
     else if (P.out <= 256) launch_rows<KS, 4>(P, in, out, stream);
     else launch_rows<KS, 8>(P, in, out, stream);
 }
-template <int RM>
 static void (*stream_kernel(int out))(MxLinear) {
     switch (out) {
-        case MARL_F32: return mx_stream_kernel<RM, MARL_F32>;
-        case MARL_BF16: return mx_stream_kernel<RM, MARL_BF16>;
-        case MARL_F16: return mx_stream_kernel<RM, MARL_F16>;
-        default: return mx_stream_kernel<RM, MARL_MXFP4>;
+        case MARL_F32: return mx_stream_kernel<MARL_F32>;
+        case MARL_BF16: return mx_stream_kernel<MARL_BF16>;
+        case MARL_F16: return mx_stream_kernel<MARL_F16>;
+        default: return mx_stream_kernel<MARL_MXFP4>;
     }
 }
 
-constexpr int64_t MX_SPLIT_GROUPS = 512;  // two workgroups a compute unit
-
-// How a call over other rows is cut: row groups per workgroup and splits of the row.
-struct MxCut { int rm; int splits; };
+// How a call over other rows is cut: whether mx_few_rows_kernel takes it, and into how many shares of the row.
+struct MxCut { bool few; int splits; };
+constexpr int64_t MX_GROUPS = 512;  // two workgroups a compute unit
 static MxCut mx_cut(int64_t rows, int64_t cols, int out) {
     MxCut c;
-    c.rm = rows <= 16 ? 1 : 4;
-    const int64_t stretches = ((int64_t)lb_blocks(cols) + 15) / 16;
-    const int64_t groups = ((out + 63) / 64) * ((rows + 16 * c.rm - 1) / (16 * c.rm));
-    const int64_t most = stretches / 8 < 1 ? 1 : stretches / 8;  // two stretches for each of a workgroup's four waves
-    int64_t s = MX_SPLIT_GROUPS / groups;
+    c.few = rows <= 16;
+    const int64_t unit = c.few ? 64 : 16, units = ((int64_t)lb_blocks(cols) + unit - 1) / unit;  // chunks, stretches
+    const int64_t groups = c.few ? (out + 15) / 16 : ((out + 63) / 64) * ((rows + 16 * MX_RM - 1) / (16 * MX_RM));
+    const int64_t most = units / 8 < 1 ? 1 : units / 8;  // at least two for each of a workgroup's four waves
+    int64_t s = MX_GROUPS / groups;
     s = s < 1 ? 1 : s > most ? most : s;
-    const int64_t per = (stretches + s - 1) / s;
-    c.splits = (int)((stretches + per - 1) / per);
+    const int64_t per = (units + s - 1) / s;
+    c.splits = (int)((units + per - 1) / per);
     return c;
 }
 static size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
@@ -571,10 +610,13 @@ static hipError_t launch_linear(const MxLinear& P0, int x_type, int out_type, ui
     }
     P.splits = c.splits;
     P.part = reinterpret_cast<float*>(ws);
-    const dim3 grid((P.out + 63) / 64, (uint32_t)((P.rows + 16 * c.rm - 1) / (16 * c.rm)), c.splits);
-    hipLaunchKernelGGL(c.rm == 1 ? stream_kernel<1>(out_type) : stream_kernel<4>(out_type), grid, dim3(256), 0, stream, P);
+    if (c.few)
+        hipLaunchKernelGGL(mx_few_rows_kernel, dim3((P.out + 15) / 16, c.splits), dim3(256), 0, stream, P);
+    else
+        hipLaunchKernelGGL(stream_kernel(out_type), dim3((P.out + 63) / 64, (uint32_t)((P.rows + 16 * MX_RM - 1) / (16 * MX_RM)), c.splits),
+                           dim3(256), 0, stream, P);
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess || c.splits == 1) return e;
+    if (e != hipSuccess || (!c.few && c.splits == 1)) return e;
     auto join = out_type == MARL_F32 ? mx_join_kernel<MARL_F32> : out_type == MARL_BF16 ? mx_join_kernel<MARL_BF16>
               : out_type == MARL_F16 ? mx_join_kernel<MARL_F16> : mx_join_kernel<MARL_MXFP4>;
     hipLaunchKernelGGL(join, dim3((uint32_t)((P.rows * lb_blocks(P.out) * 4 + 63) / 64)), dim3(256), 0, stream, P);
@@ -627,7 +669,7 @@ extern "C" size_t marl_mx_linear_workspace_bytes(int x_type, int64_t num_rows, i
     const MxCut c = mx_cut(num_rows, num_cols, num_out);
     size_t n = 0;
     if (x_type != MARL_MXFP4) n += up16((size_t)num_rows * lb_blocks(num_cols) * 16) + up16((size_t)num_rows * lb_blocks(num_cols));
-    if (c.splits > 1) n += (size_t)c.splits * num_rows * num_out * sizeof(float);
+    if (c.few || c.splits > 1) n += (size_t)c.splits * num_rows * num_out * sizeof(float);
     return n;
 }
 
