@@ -115,7 +115,11 @@ struct ActGrad {
 template <int TYPE> constexpr int grad_parts() { return TYPE == MARL_F32 ? 3 : TYPE == MARL_F16 ? 2 : 1; }
 
 constexpr int WG_STEP = 32;                 // rows a step
-constexpr int WG_PITCH = WG_STEP * 2 + 16;  // LDS bytes per column: the 16 spread columns over the banks
+constexpr int WG_PITCH = WG_STEP * 2;       // LDS bytes per column, four pieces of 8 rows
+
+// Where the piece of rows 8 p .. 8 p + 7 of a column lies within it: turned by the column's place, so that the 16 columns
+// that a fragment's lanes read lie in different banks (4.2 cycles a read of a wave; 8.0 without, or with padded columns).
+__device__ __forceinline__ int piece(int place, int p) { return (p ^ (place >> 1 & 3)) * 16; }
 
 __device__ __forceinline__ uint32_t high_halves(float a, float b) {  // a's upper 16 bits below b's
     return __builtin_amdgcn_perm(f_bits(b), f_bits(a), 0x07060302u);
@@ -246,7 +250,7 @@ struct WeightGrad {
                 u[k] = high_halves(fmaf((float)(xa >> (8 * c) & 255u), s[2 * k], z[2 * k]),
                                    fmaf((float)(xb >> (8 * c) & 255u), s[2 * k + 1], z[2 * k + 1]));
             }
-            *reinterpret_cast<u32x4*>(&S.B[buf][c * (BI / 4) + xc][xr * 2]) = u;
+            *reinterpret_cast<u32x4*>(&S.B[buf][c * (BI / 4) + xc][piece(c * (BI / 4) + xc, xr >> 3)]) = u;
         }
     }
 
@@ -274,7 +278,7 @@ struct WeightGrad {
         for (int p = 0; p < PARTS; ++p) {
 #pragma unroll
             for (int c = 0; c < 4; ++c)
-                *reinterpret_cast<u32x2*>(&S.A[buf][p][c * (BO / 4) + gc][gr * 2]) =
+                *reinterpret_cast<u32x2*>(&S.A[buf][p][c * (BO / 4) + gc][piece(c * (BO / 4) + gc, gr >> 3) + (gr & 4) * 2]) =
                     u32x2{high_halves(v[0][c], v[1][c]), high_halves(v[2][c], v[3][c])};
             if (p + 1 == PARTS) break;
             if (p == 0 && wild) {  // an infinity minus itself is no number: it has no lower parts
@@ -326,17 +330,17 @@ struct WeightGrad {
         const int r = lane & 15, g = lane >> 4;
         bf16x8 x[4];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) x[b] = *reinterpret_cast<const bf16x8*>(&S.B[buf][b * (BI / 4) + wi + r][g * 16]);
+        for (int b = 0; b < 4; ++b) x[b] = *reinterpret_cast<const bf16x8*>(&S.B[buf][b * (BI / 4) + wi + r][piece(wi + r, g)]);
         // the next 16 output features' fragments are on their way while these multiply, and no more: registers are short
         bf16x8 y[2][PARTS];
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p) y[0][p] = *reinterpret_cast<const bf16x8*>(&S.A[buf][p][wo + r][g * 16]);
+        for (int p = 0; p < PARTS; ++p) y[0][p] = *reinterpret_cast<const bf16x8*>(&S.A[buf][p][wo + r][piece(r, g)]);
 #pragma unroll
         for (int a = 0; a < TO; ++a) {
             if (a + 1 < TO) {
 #pragma unroll
                 for (int p = 0; p < PARTS; ++p)
-                    y[(a + 1) & 1][p] = *reinterpret_cast<const bf16x8*>(&S.A[buf][p][wo + (a + 1) * 16 + r][g * 16]);
+                    y[(a + 1) & 1][p] = *reinterpret_cast<const bf16x8*>(&S.A[buf][p][wo + (a + 1) * 16 + r][piece(r, g)]);
             }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll

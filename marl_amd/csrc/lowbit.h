@@ -82,9 +82,9 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t t) {
     return max(t, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)t, 0x4E, 0xF, 0xF, true));  // quad_perm 2,3,0,1
 }
 
-// value of a scale byte: 2^(byte - 127), NaN for 255
+// value of a scale byte: 2^(byte - 127), NaN for 255 (and the denormal 2^-127 for 0)
 __device__ __forceinline__ float scale_value(uint32_t byte) {
-    return byte == 255u ? bits_f(0x7FC00000u) : byte == 0u ? bits_f(0x00400000u) : bits_f(byte << 23);
+    return bits_f(max(byte << 23 | (byte == 255u ? 0x00400000u : 0u), 0x00400000u));
 }
 
 template <int TYPE>
