@@ -109,7 +109,6 @@ struct ActGrad {
     float* gw;                   // [splits][out][cols] (the result itself if splits is 1)
     float* gb;                   // [splits][out]
     int splits;
-    int64_t per;                 // rows of a split, a multiple of 32
 };
 
 template <int TYPE> constexpr int grad_parts() { return TYPE == MARL_F32 ? 3 : TYPE == MARL_F16 ? 2 : 1; }
@@ -194,7 +193,7 @@ struct WeightGrad {
 
     const ActGrad& P;
     Lds& S;
-    int64_t first, last;
+    int64_t first, stride, last;
     int o0, i0, lane, wo, wi;
     bool leader;  // also writes the cut gradient and sums it
     int xc, xr, xi, xback, xhave, gc, gr, go, gback, ghave;
@@ -362,8 +361,8 @@ struct WeightGrad {
     template <bool X, bool G>
     __device__ __forceinline__ void step(RawX& x, RawG& g, int64_t m0, int buf) {
         if constexpr (X) multiply(buf);
-        convert<X, G>(x, g, m0 + WG_STEP, buf ^ 1);
-        fetch<X, G>(x, g, m0 + 3 * WG_STEP);
+        convert<X, G>(x, g, m0 + stride, buf ^ 1);
+        fetch<X, G>(x, g, m0 + 3 * stride);
         if constexpr (!X) multiply(buf);
         __syncthreads();
     }
@@ -373,13 +372,13 @@ struct WeightGrad {
         RawX x0, x1;
         RawG g0, g1;
         fetch<X, G>(x0, g0, first);
-        fetch<X, G>(x1, g1, first + WG_STEP);
+        fetch<X, G>(x1, g1, first + stride);
         convert<X, G>(x0, g0, first, 0);
-        fetch<X, G>(x0, g0, first + 2 * WG_STEP);
+        fetch<X, G>(x0, g0, first + 2 * stride);
         __syncthreads();
-        for (int64_t m0 = first; m0 < last; m0 += 2 * WG_STEP) {
+        for (int64_t m0 = first; m0 < last; m0 += 2 * stride) {
             step<X, G>(x1, g1, m0, 0);
-            if (m0 + WG_STEP < last) step<X, G>(x0, g0, m0 + WG_STEP, 1);
+            if (m0 + stride < last) step<X, G>(x0, g0, m0 + stride, 1);
         }
     }
 
@@ -391,8 +390,10 @@ struct WeightGrad {
         i0 = tile % ti * BI;
         wo = wave / WI * (BO / WO);
         wi = wave % WI * 16;
-        first = (int64_t)split * P.per;
-        last = min(P.rows, first + P.per);
+        // the splits take turns at the steps: what runs at the same time reads one stretch of memory
+        first = (int64_t)split * WG_STEP;
+        stride = (int64_t)P.splits * WG_STEP;
+        last = P.rows;
         leader = i0 == 0;
         xc = tid % (BI / 4);
         xr = tid / (BI / 4) * 8;
@@ -489,7 +490,7 @@ act_join_kernel(const float* __restrict__ part_w, const float* __restrict__ part
 
 // ------------------------------------------------------------------------------------------------------------ host
 
-struct ActCut { int bo, bi, splits; int64_t per, grid; };
+struct ActCut { int bo, bi, splits; int64_t grid; };
 static ActCut act_cut(int64_t rows, int out, int cols) {
     ActCut c;
     const int64_t steps = (rows + WG_STEP - 1) / WG_STEP;
@@ -500,10 +501,9 @@ static ActCut act_cut(int64_t rows, int out, int cols) {
     const int64_t t = tiles(c.bo, c.bi);
     int64_t s = (c.bo == 128 ? 256 : 512) / t;
     s = s < 1 ? 1 : s;
-    const int64_t most = (steps + 3) / 4;  // at least four steps each
+    const int64_t least = c.bo == 16 ? 8 : 4, most = (steps + least - 1) / least;  // steps a split
     s = s > most ? most : s;
     const int64_t each = (steps + s - 1) / s;
-    c.per = each * WG_STEP;
     c.splits = (int)((steps + each - 1) / each);
     c.grid = (int64_t)(c.splits + 7) / 8 * 8 * t;
     return c;
@@ -605,7 +605,7 @@ extern "C" int marl_act_weight_grad(const void* d_grad, int grad_type, int64_t n
     P.grad = d_grad; P.mask = d_mask_codes; P.rows = num_rows; P.out = num_out; P.cols = num_cols;
     P.blocks = (int)lb_blocks(num_cols);
     P.codes = d_codes; P.scales = d_scales; P.zero = nonnegative ? 0.0f : 128.0f; P.masked = d_masked_grad;
-    P.splits = c.splits; P.per = c.per;
+    P.splits = c.splits;
     P.gw = c.splits == 1 ? d_grad_weight : static_cast<float*>(d_workspace);
     P.gb = c.splits == 1 ? d_grad_bias : static_cast<float*>(d_workspace) + c.splits * nw;
     if (grad_type == MARL_F32) launch_weight_grad_type<MARL_F32>(P, c, s);
