@@ -61,12 +61,16 @@ def main(argv=None):
     p.add_argument("--max-steps", type=int, default=1000)
     p.add_argument("--seed", type=int, default=0)
     p.add_argument("--greedy", action="store_true", help="argmax actions instead of sampling (the reference samples)")
+    p.add_argument("--precision", choices=["float32", "mxfp4"], default="float32",
+                   help="the policy's trunk in float32, or in 4-bit floating point (marl_amd.mxfp4)")
     args = p.parse_args(argv)
     device = torch.device("cuda", torch.cuda.current_device())
     torch.manual_seed(args.seed)
     env = make_env(args.num_agents, layout=args.layout, feature=args.feature, max_steps=args.max_steps)
     vec = make_vector_env(args.num_envs, env, seed=args.seed, device=device)
     net = load_policy(args.model_path, vec.single_observation_space, vec.single_action_space, args.num_agents, device)
+    if args.precision == "mxfp4":
+        net.use_mxfp4_rollouts()
     result = run_inference(net, vec, episodes=args.episodes, greedy=args.greedy)
     for k, r in enumerate(result):
         print(json.dumps({"episode": k, "envs": args.num_envs, **r}))

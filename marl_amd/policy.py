@@ -3,8 +3,10 @@
 ReLU), ``actor`` (256 -> n_actions), ``critic`` (256 -> 1) and ``centralised_critics.{0,2,4}``
 (obs_dim * num_agents * num_envs -> 512 -> 256 -> 1).  All layers start orthogonal with gain
 sqrt(2) and zero bias (model.py:6-9).  The matrix products run on PyTorch-ROCm (rocBLAS /
-hipBLASLt); nothing here is hand-written HIP; which library call computes a layer of a small
-batch is a fixed function of its shape (`_table_form`)."""
+hipBLASLt); which library call computes a layer of a small batch is a fixed function of its
+shape (`_table_form`).  On request the trunk acts in 4-bit floating point (`use_mxfp4_rollouts`, the
+HIP passes of `mxfp4`) and keeps its activations for the backward pass in 8 bits
+(`use_activation_checkpoints`, those of `act8`)."""
 from __future__ import annotations
 
 import math
@@ -15,6 +17,8 @@ import warnings
 import torch
 from torch import nn
 from torch.distributions import Categorical
+
+from . import act8, mxfp4
 
 
 def _ortho(linear: nn.Linear, gain: float = math.sqrt(2.0), bias: float = 0.0) -> nn.Linear:
@@ -187,6 +191,32 @@ class _LinearReLU(torch.autograd.Function):
         return gx, _weight_grad(gy, x), gy.sum(0), None
 
 
+class _KeptLinear(torch.autograd.Function):
+    """`_LinearReLU` that keeps its input, and behind a ReLU its output, in 8 bits for the backward pass instead of in
+    float32.  The input comes with its kept form (codes, scales, whether nonnegative); the output's goes on to the next layer, so that
+    what lies between two layers is kept once.  The gradient of the weight is formed from the kept input, the ReLU's mask is the
+    kept output's and exact; the forward pass and the gradient of the input are those of `_LinearReLU`."""
+
+    @staticmethod
+    def forward(ctx, x, codes, scales, nonnegative, weight, bias, relu):
+        out = _FORMS[_small_gemm_form(x, weight, bias, relu)](x, weight, bias, relu)
+        kept = act8.compress(out, nonnegative=True) if relu else None
+        ctx.nonnegative = nonnegative
+        ctx.save_for_backward(codes, scales, weight, kept.codes if relu else None, kept.scales if relu else None)
+        if not relu:
+            return out
+        ctx.mark_non_differentiable(kept.codes, kept.scales)
+        return out, kept.codes, kept.scales
+
+    @staticmethod
+    def backward(ctx, gy, *_kept):
+        codes, scales, weight, out_codes, out_scales = ctx.saved_tensors
+        mask = None if out_codes is None else act8.Act8(out_codes, out_scales, True)
+        gw, gb, masked = act8.weight_grad(gy, act8.Act8(codes, scales, ctx.nonnegative), mask)
+        gx = (gy if mask is None else masked) @ weight if ctx.needs_input_grad[0] else None
+        return gx, None, None, None, gw, gb, None
+
+
 def _linear(layer: nn.Linear, x, relu):
     if x.is_cuda and x.dim() == 2:
         if x.shape[0] < _SMALL_ROWS:
@@ -220,6 +250,8 @@ class Agent(nn.Module):
         # decentralised learner never evaluates it and may leave it out.
         self.sampler = None  # set by use_fused_sampling(); plain torch.distributions otherwise
         self._head_w = self._head_b = None  # stacked heads of rollout_step
+        self._acting = None  # 4-bit weights of the layers that act in 4 bits, set by use_mxfp4_rollouts()
+        self._keep_in_8_bits = False  # set by use_activation_checkpoints()
         self.centralised_critics = (_mlp([d * self.num_agents * self.num_envs, 512, 256, 1], final_activation=False)
                                     if build_centralised else None)
 
@@ -228,6 +260,63 @@ class Agent(nn.Module):
         ReLU in its epilogue: the same float32 result bit for bit, one pass less over the
         activations (250 us instead of 365 us for 131,072 x 202 -> 512)."""
         return _linear(self.network[2], _linear(self.network[0], x, True), True)
+
+    def use_mxfp4_rollouts(self):
+        """Acting (rollouts, evaluation: no autograd) computes the trunk in 4-bit floating point (`mxfp4.linear`), and of the
+        centralised critic its first layer, whose weight is most of what a rollout step reads.  Heads, updates and the bootstrap
+        value stay in float32.  The log-probabilities that a rollout stores are those of the policy that acted, so the PPO
+        ratio starts from it.  `rollout_step` reads the weights as `refresh_rollout_heads` last quantised them; every other call
+        quantises them anew."""
+        self._acting = {}
+        return self
+
+    def use_activation_checkpoints(self):
+        """Updates keep the trunk's activations in 8 bits between the forward and the backward pass (`act8`), a quarter of what
+        autograd keeps: an input of whole numbers up to 127 (the observations) exactly, the hidden layers to half a step of
+        a 1/128 of their block's largest value.  Values, log-probabilities and the loss are unchanged; the gradients of
+        the weights are those of the kept activations."""
+        self._keep_in_8_bits = True
+        return self
+
+    def _acting_weight(self, name, layer, fresh):
+        """`layer`'s weight in 4 bits, in the same storage every time; quantised anew unless `fresh` says that it is current"""
+        held = self._acting.get(name)
+        if held is None or held.device != layer.weight.device:
+            held = self._acting[name] = mxfp4.quantize(layer.weight.detach())
+        elif not fresh:
+            mxfp4.quantize(layer.weight.detach(), out=held)
+        return held
+
+    def _acting_trunk(self, x, fresh=False):
+        """network(x) for acting: in 4 bits if `use_mxfp4_rollouts` asked for it, as `_trunk` otherwise"""
+        if self._acting is None or not x.is_cuda or torch.is_grad_enabled():
+            return self._trunk(x)
+        l0, l1 = self.network[0], self.network[2]
+        h = mxfp4.linear(x, self._acting_weight("network.0", l0, fresh), l0.bias.detach(), relu=True, out_dtype="mxfp4")
+        return mxfp4.linear(h, self._acting_weight("network.2", l1, fresh), l1.bias.detach(), relu=True)
+
+    def _acting_central(self, joint_obs, fresh=False):
+        if self._acting is None or not joint_obs.is_cuda or torch.is_grad_enabled() or self.centralised_critics is None:
+            return self._central(joint_obs)
+        c = self.centralised_critics
+        h = mxfp4.linear(joint_obs, self._acting_weight("centralised_critics.0", c[0], fresh), c[0].bias.detach(), relu=True)
+        return _linear(c[4], _linear(c[2], h, True), False)
+
+    def _kept_heads(self, x):
+        """logits and value with every activation kept in 8 bits: both heads as one layer, so that the hidden layer is read once"""
+        kept = act8.compress(x)
+        codes, scales, nonnegative, h = kept.codes, kept.scales, False, x.contiguous()
+        if x.shape[0] < _SMALL_ROWS:
+            _announce_blas_switch_quietly(x)
+        for layer in (self.network[0], self.network[2]):
+            h, codes, scales = _KeptLinear.apply(h, codes, scales, nonnegative, layer.weight, layer.bias, True)
+            nonnegative = True
+        heads = _KeptLinear.apply(h, codes, scales, True, torch.cat([self.actor.weight, self.critic.weight]),
+                                  torch.cat([self.actor.bias, self.critic.bias]), False)
+        return heads.split([self.actor.out_features, 1], dim=1)
+
+    def _keeps(self, x):
+        return self._keep_in_8_bits and torch.is_grad_enabled() and x.is_cuda and x.dim() == 2 and x.shape[0] > 0
 
     def use_fused_sampling(self, seed, row_index_base=0):
         """Rollout actions (no autograd, action=None) come from `sampling.CategoricalSampler`: one
@@ -252,19 +341,25 @@ class Agent(nn.Module):
         return _linear(self.critic, self._trunk(x), False)
 
     def get_action_and_value(self, x, action=None, joint_obs=None):
-        hidden = self._trunk(x)
         # validate_args=False: the argument check reads a device flag back on the host, one
         # synchronisation per call, and cannot run under hipGraph capture; it changes no result
-        logits = _linear(self.actor, hidden, False)
-        if action is None and self.sampler is not None and logits.is_cuda and not torch.is_grad_enabled():
+        if action is None and self.sampler is not None and x.is_cuda and not torch.is_grad_enabled():
             # rollout: sample, log-probability and entropy in one launch
-            value = self._central(joint_obs) if joint_obs is not None else _linear(self.critic, hidden, False)
+            hidden = self._acting_trunk(x)
+            logits = _linear(self.actor, hidden, False)
+            value = self._acting_central(joint_obs) if joint_obs is not None else _linear(self.critic, hidden, False)
             action, logprob, entropy = self.sampler.sample(logits)
             return action, logprob, entropy, value
+        if joint_obs is None and self._keeps(x):
+            logits, value = self._kept_heads(x)
+        else:
+            hidden = self._acting_trunk(x) if action is None else self._trunk(x)
+            logits, value = _linear(self.actor, hidden, False), None
         dist = Categorical(logits=logits, validate_args=False)
         if action is None:
             action = dist.sample()
-        value = self._central(joint_obs) if joint_obs is not None else _linear(self.critic, hidden, False)
+        if value is None:
+            value = self._central(joint_obs) if joint_obs is not None else _linear(self.critic, hidden, False)
         return action, dist.log_prob(action), dist.entropy(), value
 
     def refresh_rollout_heads(self):
@@ -278,6 +373,11 @@ class Agent(nn.Module):
         with torch.no_grad():
             torch.cat([self.actor.weight, self.critic.weight], out=self._head_w)
             torch.cat([self.actor.bias, self.critic.bias], out=self._head_b)
+        if self._acting is not None:  # the 4-bit weights that rollout_step reads
+            self._acting_weight("network.0", self.network[0], False)
+            self._acting_weight("network.2", self.network[2], False)
+            if self.centralised_critics is not None and "centralised_critics.0" in self._acting:
+                self._acting_weight("centralised_critics.0", self.centralised_critics[0], False)
 
     def rollout_step(self, x, logprob_out, value_out, actions_out=None, slot=None, joint=False, row_offset=0):
         """The rollout half of `get_action_and_value` for the decentralised critic, writing the
@@ -297,15 +397,15 @@ class Agent(nn.Module):
             raise RuntimeError("rollout_step needs use_fused_sampling()")
         if joint:
             with torch.no_grad():
-                logits = _linear(self.actor, self._trunk(x), False)
+                logits = _linear(self.actor, self._acting_trunk(x, fresh=True), False)
                 actions, _, _ = self.sampler.sample(logits, want_entropy=False, actions_out=actions_out,
                                                     logprob_out=logprob_out, slot=slot)
-                value_out.copy_(self._central(x.view(1, -1)).view(1).expand_as(value_out))
+                value_out.copy_(self._acting_central(x.view(1, -1), fresh=True).view(1).expand_as(value_out))
             return actions
         if getattr(self, "_head_w", None) is None:
             self.refresh_rollout_heads()
         with torch.no_grad():
-            heads = torch.addmm(self._head_b, self._trunk(x), self._head_w.t())
+            heads = torch.addmm(self._head_b, self._acting_trunk(x, fresh=True), self._head_w.t())
             actions, _, _ = self.sampler.sample(heads, want_entropy=False, actions_out=actions_out, logprob_out=logprob_out,
                                                 slot=slot, num_actions=self.actor.out_features, next_column_out=value_out,
                                                 row_offset=row_offset)
@@ -313,8 +413,10 @@ class Agent(nn.Module):
 
     def logits_and_value(self, x):
         """both heads on the shared trunk (model.py:49-61 without the distribution object)"""
+        if self._keeps(x):
+            return self._kept_heads(x)
         hidden = self._trunk(x)
         return _linear(self.actor, hidden, False), _linear(self.critic, hidden, False)
 
     def get_prob(self, x):
-        return Categorical(logits=_linear(self.actor, self._trunk(x), False), validate_args=False)
+        return Categorical(logits=_linear(self.actor, self._acting_trunk(x), False), validate_args=False)

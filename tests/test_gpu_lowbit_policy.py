@@ -1,0 +1,302 @@
+"""The policy that acts in 4 bits and keeps its activations in 8 for the update, as the rollout driver, the learners and the
+commands use them together."""
+import copy
+
+import numpy as np
+import pytest
+import torch
+
+import lowbit_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def _agent(seed=5, num_envs=1, central=True, layout="overcooked_cramped_room_v0", A=2, feature="global_obs"):
+    from marl_amd.env import make_env, make_vector_env
+    from marl_amd.policy import Agent
+
+    dev = torch.device("cuda:0")
+    env = make_env(A, layout, feature)
+    vec = make_vector_env(max(num_envs, 1), env, device=dev)
+    torch.manual_seed(seed)
+    return Agent(vec.single_observation_space, vec.single_action_space, A, num_envs, build_centralised=central).to(dev), vec
+
+
+def _obs(rows, d, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(rows, d, device="cuda", generator=g)
+    return (x.abs() > 0.9).float() * (x * 1.3).round()
+
+
+def _acting_logits(net, x):
+    """the acting policy's logits composed from the formats' definition, in 64 bits but for the float32 sums in between"""
+    l0, l1 = net.network[0], net.network[2]
+    h = x.double().cpu().numpy()
+    for layer in (l0, l1):
+        w = ref.mxfp4(layer.weight.detach().double().cpu().numpy())[2]
+        h = np.maximum(ref.mxfp4(h)[2] @ w.T + layer.bias.detach().double().cpu().numpy(), 0.0).astype(np.float32).astype(np.float64)
+    return h @ net.actor.weight.detach().double().cpu().numpy().T + net.actor.bias.detach().double().cpu().numpy()
+
+
+@pytest.mark.parametrize("rows", [1, 32, 2000])
+def test_every_acting_call_computes_the_trunk_in_4_bits(rows):
+    net, _ = _agent()
+    x = _obs(rows, 202, rows)
+    net.use_fused_sampling(3)
+    with torch.no_grad():
+        plain = net.get_prob(x).logits
+    net.use_mxfp4_rollouts()
+    want = _acting_logits(net, x)
+    want = want - np.log(np.exp(want).sum(1, keepdims=True))
+    with torch.no_grad():
+        got = net.get_prob(x).logits
+        # sums of whole multiples of a scale: exact in the trunk; heads and log-softmax in float32
+        np.testing.assert_allclose(got.double().cpu().numpy(), want, rtol=0, atol=2e-5)
+        action, logprob, _, value = net.get_action_and_value(x)
+        np.testing.assert_allclose(logprob.cpu().numpy(), want[np.arange(rows), action.cpu().numpy()], rtol=0, atol=2e-5)
+        lp, v = torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda")
+        a2 = net.rollout_step(x, lp, v)
+        np.testing.assert_allclose(lp.cpu().numpy(), want[np.arange(rows), a2.cpu().numpy()], rtol=0, atol=2e-5)
+        torch.testing.assert_close(v, value.squeeze(1), rtol=1e-5, atol=1e-5)
+    assert not torch.equal(got, plain)  # it is another policy
+    # with autograd on, and for the bootstrap value, nothing changes
+    assert torch.equal(net.get_prob(x).logits.detach(), plain)
+
+
+def test_changed_weights_reach_the_acting_policy():
+    net, _ = _agent()
+    x = _obs(64, 202)
+    net.use_fused_sampling(3).use_mxfp4_rollouts()
+    lp, v = torch.empty(64, device="cuda"), torch.empty(64, device="cuda")
+    net.refresh_rollout_heads()
+    net.rollout_step(x, lp, v)
+    held = {k: w.codes.data_ptr() for k, w in net._acting.items()}
+    before = v.clone()
+    with torch.no_grad():
+        for p in net.network.parameters():
+            p.mul_(1.5)
+        expected = net.get_prob(x).logits  # quantised anew by itself
+    net.refresh_rollout_heads()
+    net.rollout_step(x, lp, v)
+    assert not torch.equal(v, before)
+    assert {k: w.codes.data_ptr() for k, w in net._acting.items()} == held  # captured launches read the same places
+    np.testing.assert_allclose(expected.double().cpu().numpy(),
+                               (lambda l: l - np.log(np.exp(l).sum(1, keepdims=True)))(_acting_logits(net, x)), rtol=0, atol=2e-5)
+
+
+def test_a_rollout_step_replayed_from_a_graph_follows_the_refreshed_weights():
+    net, _ = _agent()
+    x = _obs(32, 202)
+    net.use_fused_sampling(3).use_mxfp4_rollouts()
+    lp, v = torch.empty(32, device="cuda"), torch.empty(32, device="cuda")
+    net.refresh_rollout_heads()
+    net.rollout_step(x, lp, v)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, capture_error_mode="thread_local"):
+        net.rollout_step(x, lp, v)
+    for step in range(3):
+        with torch.no_grad():
+            for p in net.parameters():
+                p.mul_(1.1)
+        x.copy_(_obs(32, 202, step + 1))
+        net.refresh_rollout_heads()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        got = v.clone()
+        with torch.no_grad():
+            want = net.get_action_and_value(x)[3].squeeze(1)
+        torch.testing.assert_close(got, want, rtol=1e-5, atol=1e-5)
+
+
+def test_the_centralised_critic_acts_in_4_bits():
+    net, _ = _agent(num_envs=16)
+    x = _obs(32, 202)
+    net.use_fused_sampling(3).use_mxfp4_rollouts()
+    lp, v = torch.empty(32, device="cuda"), torch.empty(32, device="cuda")
+    net.rollout_step(x, lp, v, joint=True)
+    c = net.centralised_critics
+    h = np.maximum(ref.mxfp4(x.view(1, -1).double().cpu().numpy())[2] @ ref.mxfp4(c[0].weight.detach().double().cpu().numpy())[2].T
+                   + c[0].bias.detach().double().cpu().numpy(), 0.0)
+    for layer, relu in ((c[2], True), (c[4], False)):
+        h = h @ layer.weight.detach().double().cpu().numpy().T + layer.bias.detach().double().cpu().numpy()
+        h = np.maximum(h, 0.0) if relu else h
+    # two float32 layers of 512 and 256 terms behind it
+    np.testing.assert_allclose(v.double().cpu().numpy(), np.full(32, h[0, 0]), rtol=0, atol=2e-5 * max(1.0, abs(h[0, 0])))
+    with torch.no_grad():
+        value = net.get_action_and_value(x, joint_obs=x.view(1, -1))[3]
+    torch.testing.assert_close(value.view(1), v[:1], rtol=1e-6, atol=1e-6)
+
+
+def _reference_gradients(net, x, g_heads):
+    """float64 gradients of sum(heads * g_heads) from the formula with the kept activations: what every weight gradient reads is
+    the kept value, what the ReLU let through is where the float32 output is positive"""
+    d = lambda t: t.detach().double().cpu().numpy()  # noqa: E731
+    w0, w1 = d(net.network[0].weight), d(net.network[2].weight)
+    with torch.no_grad():
+        h0 = torch._addmm_activation(net.network[0].bias, x, net.network[0].weight.t(), use_gelu=False)
+        h1 = torch._addmm_activation(net.network[2].bias, h0, net.network[2].weight.t(), use_gelu=False)
+    kx, k0, k1 = ref.act8(d(x), False)[2], ref.act8(d(h0), True)[2], ref.act8(d(h1), True)[2]
+    wh = np.concatenate([d(net.actor.weight), d(net.critic.weight)])
+    gh = g_heads.double().cpu().numpy()
+    out = {"heads.weight": gh.T @ k1, "heads.bias": gh.sum(0)}
+    g1 = (gh @ wh) * (d(h1) > 0)
+    out["network.2.weight"], out["network.2.bias"] = g1.T @ k0, g1.sum(0)
+    g0 = (g1 @ w1) * (d(h0) > 0)
+    out["network.0.weight"], out["network.0.bias"] = g0.T @ kx, g0.sum(0)
+    return out
+
+
+@pytest.mark.parametrize("rows", [5, 600, 8192])
+def test_gradients_of_the_kept_activations(rows):
+    net, _ = _agent(central=False)
+    x = _obs(rows, 202, rows)
+    with torch.no_grad():
+        plain_logits, plain_value = net.logits_and_value(x)
+    plain = copy.deepcopy(net)
+    net.use_activation_checkpoints()
+    logits, value = net.logits_and_value(x)
+    # the same trunk; the two heads in one product
+    torch.testing.assert_close(logits, plain_logits, rtol=1e-5, atol=1e-5)
+    torch.testing.assert_close(value, plain_value, rtol=1e-5, atol=1e-5)
+    g = torch.randn(rows, 8, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)) / rows
+    torch.autograd.backward([logits, value], [g[:, :7], g[:, 7:]])
+    want = _reference_gradients(net, x, g)
+    got = {k: p.grad.double().cpu().numpy() for k, p in net.named_parameters()}
+    got["heads.weight"] = np.concatenate([got.pop("actor.weight"), got.pop("critic.weight")])
+    got["heads.bias"] = np.concatenate([got.pop("actor.bias"), got.pop("critic.bias")])
+    for name, w in want.items():
+        # sums in float32, through at most two float32 products of up to 256 terms
+        assert np.linalg.norm(got[name] - w) <= 4e-6 * np.linalg.norm(w) + 1e-12, name
+    # Against float32 activations: observations are kept exactly and the masks are exact, so the first layer's gradients and
+    # every bias's are the same numbers but for the order of sums.  The others are off by what 8 bits leave out: a step is at
+    # most 2^-7 of a block's largest value (128 to 255 of them reach it), a rounding is off by step / sqrt(12) in the mean
+    # square, and the largest of 32 values is at most sqrt(32) times their root mean square; with g independent of the
+    # roundings, error and gradient add up alike: 2^-7 sqrt(32 / 12) = 1.64 * 2^-7 of the gradient, below 2^-6.
+    logits, value = plain.logits_and_value(x)
+    torch.autograd.backward([logits, value], [g[:, :7], g[:, 7:]])
+    for name, p in plain.named_parameters():
+        w = p.grad.double().cpu().numpy()
+        mine = dict(net.named_parameters())[name].grad.double().cpu().numpy()
+        close = 4e-6 if name.endswith("bias") or name == "network.0.weight" else 2.0 ** -6
+        assert np.linalg.norm(mine - w) <= close * np.linalg.norm(w) + 1e-12, name
+
+
+def test_a_weight_gradient_against_differences():
+    """f(W, b) = sum(G * relu(x W^T + b)) in 64 bits over the kept x, differenced along random directions small enough that no
+    ReLU changes sides"""
+    from marl_amd import act8
+
+    rng = np.random.default_rng(0)
+    rows, cols, out = 300, 70, 33
+    x = torch.from_numpy(rng.standard_normal((rows, cols))).float().cuda()
+    kept = act8.compress(x)
+    xv = kept.dequantize().double().cpu().numpy()
+    w, b, G = rng.standard_normal((out, cols)), rng.standard_normal(out), rng.standard_normal((rows, out)).astype(np.float32)
+    pre = xv @ w.T + b
+    y = torch.from_numpy(np.maximum(pre, 0.0)).float().cuda()
+    gw, gb, _ = act8.weight_grad(torch.from_numpy(G).cuda(), kept, act8.compress(y, nonnegative=True))
+    for k in range(4):
+        dw, db = rng.standard_normal(w.shape), rng.standard_normal(b.shape)
+        eps = 0.25 * np.abs(pre).min() / np.abs(xv @ dw.T + db).max()
+        f = lambda s: (G.astype(np.float64) * np.maximum(xv @ (w + s * dw).T + b + s * db, 0.0)).sum()  # noqa: E731
+        slope = (f(eps) - f(-eps)) / (2 * eps)
+        mine = (gw.double().cpu().numpy() * dw).sum() + (gb.double().cpu().numpy() * db).sum()
+        scale = np.sqrt((gw.double().cpu().numpy() ** 2).sum())
+        assert abs(slope - mine) <= 1e-5 * scale * np.sqrt(dw.size) / 10 + 1e-9 * abs(f(0)) / eps
+
+
+def test_the_update_keeps_less():
+    net, _ = _agent(central=False)
+    rows = 65536
+
+    def peak():
+        x = _obs(rows, 202)
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        torch.cuda.reset_peak_memory_stats()
+        base = torch.cuda.memory_allocated()
+        logits, value = net.logits_and_value(x)
+        return torch.cuda.memory_allocated() - base, (logits.sum() + value.sum()).item()
+
+    kept32, s32 = peak()
+    net.use_activation_checkpoints()
+    kept8, s8 = peak()
+    # float32: the two hidden layers (the observations are the caller's); 8 bits: 33/32 of a byte a value, observations too,
+    # and the heads' outputs in both
+    assert kept32 >= rows * (512 + 256) * 4
+    assert kept8 <= rows * ((202 + 512 + 256) * 34 / 32 + 3 * 8 * 4) + (8 << 20)
+    assert abs(s8 - s32) <= 1e-4 * rows
+
+
+def _learner(cls, bits, graph, seed=3, **kw):
+    from marl_amd.rollout_buffer import Buffer
+
+    E, A, T = 8, 2, 32
+    net, vec = _agent(seed, num_envs=E, central=cls.__name__ == "CMAPPO")
+    if bits == 8:
+        net.use_activation_checkpoints()
+    buf = Buffer(202, A, E, max_size=T, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    buf.obs_buff.copy_(_obs(T * E * A, 202, 2).view(T, E * A, 202))
+    buf.actions_buff.copy_(torch.randint(0, 7, (T, E * A), device="cuda", generator=g).float())
+    buf.rewards_buff.copy_(torch.randn(T, E * A, device="cuda", generator=g))
+    buf.logprobs_buff.fill_(-1.9459)
+    buf.values_buff.copy_(torch.randn(T, E * A, device="cuda", generator=g) * 0.1)
+    opt = torch.optim.SGD(net.parameters(), lr=1e-2)
+    learner = cls(vec, opt, net, buf, (202,), 7, batch_size=T * E * A, num_mini_batches=4, num_agents=A, ppo_epoch=2,
+                  graph_update="on" if graph else "off", **kw)
+    return learner, net
+
+
+@pytest.mark.parametrize("name", ["MAPPO", "CMAPPO"])
+@pytest.mark.parametrize("fused", [True, False])
+def test_updates_with_kept_activations_follow_the_float32_ones(name, fused):
+    from marl_amd import agents
+
+    cls = getattr(agents, name)
+    after = {}
+    for bits in (32, 8):
+        learner, net = _learner(cls, bits, False, fused_loss=fused)
+        before = {k: p.detach().clone() for k, p in net.named_parameters()}
+        torch.manual_seed(11)
+        learner.update(_obs(16, 202, 9))
+        after[bits] = {k: (p.detach() - before[k]) for k, p in net.named_parameters()}
+    for k, d in after[32].items():
+        # eight clipped steps, each weight gradient off by at most half a step of 8 bits
+        assert (after[8][k] - d).norm() <= 2.0 ** -6 * d.norm() + 1e-9, k
+
+
+def test_captured_updates_equal_eager_ones():
+    from marl_amd.agents import MAPPO
+
+    got = []
+    for graph in (False, True):
+        learner, net = _learner(MAPPO, 8, graph)
+        torch.manual_seed(11)
+        for k in range(3):  # the first update runs eagerly, the others replay
+            learner.update(_obs(16, 202, 9 + k))
+            torch.cuda.synchronize()
+        got.append([p.detach().clone() for p in net.parameters()])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("algorithm,extra", [("mappo", []), ("mappo", ["--graph-rollout", "on", "--graph-update", "on"]),
+                                             ("mappo", ["--env-shards", "2", "--fused-loss", "off"]), ("cmappo", [])])
+def test_training_and_playing_in_low_bits(tmp_path, algorithm, extra):
+    from marl_amd import evaluate, train
+
+    E, A, T = 16, 2, 32
+    returns, freq = train.main(["--num-agents", str(A), "--num-envs", str(E), "--layout", "overcooked_cramped_room_v0", "--num-steps", str(T),
+                                "--total-steps", str(E * A * T * 4), "--ppo-epoch", "2", "--algorithm", algorithm, "--max-steps", "50",
+                                "--data-path", str(tmp_path / "d"), "--seed", "3", "--save", "--save-path", str(tmp_path / "m"),
+                                "--rollout-precision", "mxfp4", "--activation-bits", "8"] + extra)
+    assert len(returns) == 2 and np.isfinite(returns).all()
+    path = next((tmp_path / "m").iterdir())
+    sd = torch.load(path, map_location="cpu", weights_only=True)
+    assert all(torch.isfinite(v).all() for v in sd.values())
+    out = evaluate.main(["--model-path", str(path), "--num-agents", str(A), "--layout", "overcooked_cramped_room_v0", "--num-envs", "32",
+                         "--episodes", "1", "--max-steps", "60", "--precision", "mxfp4"])
+    assert np.isfinite(list(out[0].values())).all()
