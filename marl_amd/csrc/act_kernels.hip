@@ -496,12 +496,12 @@ static ActCut act_cut(int64_t rows, int out, int cols) {
     const int64_t steps = (rows + WG_STEP - 1) / WG_STEP;
     const auto tiles = [&](int bo, int bi) { return (int64_t)((out + bo - 1) / bo) * ((cols + bi - 1) / bi); };
     if (out <= 16 || cols < 4) { c.bo = 16; c.bi = 256; }
-    else if (tiles(128, 256) * (steps / 8) >= 256) { c.bo = 128; c.bi = 256; }
+    else if (tiles(128, 256) * (steps / 4) >= 256) { c.bo = 128; c.bi = 256; }
     else { c.bo = 64; c.bi = 64; }
     const int64_t t = tiles(c.bo, c.bi);
     int64_t s = (c.bo == 128 ? 256 : 512) / t;
     s = s < 1 ? 1 : s;
-    const int64_t least = c.bo == 16 ? 8 : 4, most = (steps + least - 1) / least;  // steps a split
+    const int64_t least = c.bo == 16 ? (steps > 512 ? 8 : 2) : 4, most = (steps + least - 1) / least;  // steps a split
     s = s > most ? most : s;
     const int64_t each = (steps + s - 1) / s;
     c.splits = (int)((steps + each - 1) / each);

@@ -172,15 +172,6 @@ __device__ __forceinline__ void mx_store(const MxLinear& P, int64_t m, bool live
     }
 }
 
-// one 16-byte block of codes, zeros (with any scale) behind the last row or block
-__device__ __forceinline__ u32x4 mx_block(const uint8_t* codes, int64_t row, int64_t rows, int b, int blocks) {
-    if (row < rows && b < blocks) return *reinterpret_cast<const u32x4*>(codes + (row * blocks + b) * 16);
-    return u32x4{0, 0, 0, 0};
-}
-__device__ __forceinline__ uint32_t mx_scale(const uint8_t* scales, int64_t row, int64_t rows, int b, int blocks) {
-    return row < rows && b < blocks ? scales[row * blocks + b] : 127u;
-}
-
 // Rows of 8 to 512 values.  A workgroup has eight waves, WN of them side by side (64 features each) and 8 / WN below one
 // another, and walks row tiles; a wave keeps its 64 features' whole weight in registers (at most 64 of them).  The threads
 // quantise a tile's rows into LDS (four lanes per block, as above); the next tile's values are on their way from memory
@@ -226,24 +217,27 @@ mx_rows_kernel(MxLinear P) {
     __shared__ __align__(16) uint8_t scales[2][T::ROWS][16];  // [block % 4][block / 4]: a lane's scales are one word
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
     const int n0 = (blockIdx.y * WN + wave % WN) * 64, wm = wave / WN * 16 * T::GROUPS;
+    // Features behind the last are the last again (their results are not stored), blocks behind a row's end its last one again
+    // (x is zero there): no load hangs on a condition, so that all of them are under way together.
     u32x4 w[4][KS];
-    int ws[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        const int n = n0 + mx_feature<OUT>(t, r >> 2) + (r & 3);
-        uint32_t s = 0;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            w[t][ks] = mx_block(P.w, n, P.out, ks * 4 + g, P.blocks);
-            s |= mx_scale(P.w_scales, n, P.out, ks * 4 + g, P.blocks) << (8 * ks);
-        }
-        ws[t] = (int)s;
-    }
+    uint32_t wsb[4][KS];
     float bias[16];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
-        const int n = n0 + mx_feature<OUT>(k >> 2, g) + (k & 3);
-        bias[k] = P.bias && n < P.out ? P.bias[n] : 0.0f;
+    for (int t = 0; t < 4; ++t) {
+        const int64_t row = (int64_t)min(n0 + mx_feature<OUT>(t, r >> 2) + (r & 3), P.out - 1) * P.blocks;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const int64_t at = row + min(ks * 4 + g, P.blocks - 1);
+            w[t][ks] = *reinterpret_cast<const u32x4*>(P.w + at * 16);
+            wsb[t][ks] = P.w_scales[at];
+        }
+    }
+    if (P.bias) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) bias[k] = P.bias[min(n0 + mx_feature<OUT>(k >> 2, g) + (k & 3), P.out - 1)];
+    } else {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) bias[k] = 0.0f;
     }
 
     // An item: 8 values of a block (float rows) or a whole block (codes).  Rows behind the last are the last again, their
@@ -296,6 +290,14 @@ mx_rows_kernel(MxLinear P) {
     if constexpr (AHEAD) {
 #pragma unroll
         for (int q = 0; q < ITEMS; ++q) load(blockIdx.x, q, q);
+    }
+    int ws[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        uint32_t word = 0;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) word |= wsb[t][ks] << (8 * ks);
+        ws[t] = (int)word;
     }
     int buf = 0;
     for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, buf ^= 1) {
@@ -558,9 +560,8 @@ static void launch_rows(const MxLinear& P, int in, int out, hipStream_t stream) 
 }
 template <int KS>
 static void launch_rows_wide(const MxLinear& P, int in, int out, hipStream_t stream) {
-    // Side by side as many waves as there are features for, so that a row is quantised once; with few rows, where that
-    // would leave most of the chip without work, two.
-    if (P.out <= 128 || P.rows <= 1024) launch_rows<KS, 2>(P, in, out, stream);
+    // Side by side as many waves as there are features for, so that a row is quantised once.
+    if (P.out <= 128) launch_rows<KS, 2>(P, in, out, stream);
     else if (P.out <= 256) launch_rows<KS, 4>(P, in, out, stream);
     else launch_rows<KS, 8>(P, in, out, stream);
 }
