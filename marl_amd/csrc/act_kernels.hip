@@ -25,7 +25,7 @@ __device__ __forceinline__ uint32_t act_scale_byte(uint32_t top) {
 }
 
 // Four lanes per block, eight values each.  Bound by memory.
-template <int TYPE, bool POSITIVE>
+template <int TYPE, bool POSITIVE, bool NT>
 __global__ void __launch_bounds__(256)
 act_compress_kernel(const void* __restrict__ x, int64_t rows, int cols, int64_t pitch, int blocks,
                     uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
@@ -35,7 +35,7 @@ act_compress_kernel(const void* __restrict__ x, int64_t rows, int cols, int64_t 
     if (row >= rows) return;  // whole quads leave together
     float v[8];
     const int64_t at = (int64_t)b * LB_BLOCK + quarter * 8;
-    load_eight<TYPE>(x, row * pitch + at, row * pitch + cols, v);
+    load_eight<TYPE, NT>(x, row * pitch + at, row * pitch + cols, v);
     if (POSITIVE) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = v[k] < 0.0f ? 0.0f : v[k];  // a NaN stays
@@ -545,12 +545,15 @@ extern "C" int marl_act_compress(const void* d_x, int x_type, int64_t num_rows, 
     if (((uintptr_t)d_x & (lb_type_bytes(x_type) - 1)) != 0) return set_error(MARL_ERR_INVALID, "d_x must be aligned to its elements");
     if (too_many_blocks(num_rows, num_cols)) return set_error(MARL_ERR_INVALID, "2^30 or more blocks of 32 values in one call");
     const int blocks = (int)lb_blocks(num_cols);
-    auto pick = [&](auto positive) {
-        constexpr bool pos = decltype(positive)::value;
-        return x_type == MARL_F32 ? act_compress_kernel<MARL_F32, pos> : x_type == MARL_BF16 ? act_compress_kernel<MARL_BF16, pos>
-                                                                                             : act_compress_kernel<MARL_F16, pos>;
+    const auto pick = [&](auto positive, auto nt) {
+        constexpr bool pos = decltype(positive)::value, hint = decltype(nt)::value;
+        return x_type == MARL_F32 ? act_compress_kernel<MARL_F32, pos, hint> : x_type == MARL_BF16 ? act_compress_kernel<MARL_BF16, pos, hint>
+                                                                                                   : act_compress_kernel<MARL_F16, pos, hint>;
     };
-    auto kernel = nonnegative ? pick(std::true_type{}) : pick(std::false_type{});
+    const auto yes = std::true_type{};
+    const auto no = std::false_type{};
+    const bool nt = (uint64_t)num_rows * num_cols * lb_type_bytes(x_type) > LB_NT_BYTES;
+    auto kernel = nonnegative ? (nt ? pick(yes, yes) : pick(yes, no)) : (nt ? pick(no, yes) : pick(no, no));
     hipLaunchKernelGGL(kernel, dim3(block_grid(num_rows, num_cols)), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), d_x, num_rows,
                        num_cols, row_stride, blocks, d_codes, d_scales);
     return act_hip(hipGetLastError(), "activation compression launch");

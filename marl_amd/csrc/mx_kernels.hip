@@ -36,7 +36,7 @@ __device__ __forceinline__ uint32_t mx_codes(const float (&v)[8], uint32_t byte)
 
 // Four lanes per block, eight values each: the block's maximum is two DPP moves away and a wave reads 2 KiB of a row in
 // consecutive pieces.  Bound by memory.
-template <int TYPE>
+template <int TYPE, bool NT>
 __global__ void __launch_bounds__(256)
 mx_quantize_kernel(const void* __restrict__ x, int64_t rows, int cols, int64_t pitch, int blocks,
                    uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
@@ -45,7 +45,7 @@ mx_quantize_kernel(const void* __restrict__ x, int64_t rows, int cols, int64_t p
     split_block(blockIdx.x * 256 + threadIdx.x, (uint32_t)blocks, row, b, quarter);
     if (row >= rows) return;  // whole quads leave together
     float v[8];
-    load_eight<TYPE>(x, row * pitch + (int64_t)b * LB_BLOCK + quarter * 8, row * pitch + cols, v);
+    load_eight<TYPE, NT>(x, row * pitch + (int64_t)b * LB_BLOCK + quarter * 8, row * pitch + cols, v);
     const uint32_t byte = mx_scale_byte(quad_max(abs_top(v)));
     reinterpret_cast<uint32_t*>(codes)[(row * blocks + b) * 4 + quarter] = mx_codes(v, byte);
     if (quarter == 0) scales[row * blocks + b] = (uint8_t)byte;
@@ -533,7 +533,10 @@ static bool mx_short_rows(int64_t cols) { return cols >= 8 && cols <= 512; }
 static hipError_t launch_quantize(const void* x, int type, int64_t rows, int cols, int64_t pitch, uint8_t* codes,
                                   uint8_t* scales, hipStream_t stream) {
     const int blocks = (int)lb_blocks(cols);
-    auto kernel = type == MARL_F32 ? mx_quantize_kernel<MARL_F32> : type == MARL_BF16 ? mx_quantize_kernel<MARL_BF16> : mx_quantize_kernel<MARL_F16>;
+    const bool nt = (uint64_t)rows * cols * lb_type_bytes(type) > LB_NT_BYTES;
+    auto kernel = type == MARL_F32 ? (nt ? mx_quantize_kernel<MARL_F32, true> : mx_quantize_kernel<MARL_F32, false>)
+                : type == MARL_BF16 ? (nt ? mx_quantize_kernel<MARL_BF16, true> : mx_quantize_kernel<MARL_BF16, false>)
+                                    : (nt ? mx_quantize_kernel<MARL_F16, true> : mx_quantize_kernel<MARL_F16, false>);
     hipLaunchKernelGGL(kernel, dim3(block_grid(rows, cols)), dim3(256), 0, stream, x, rows, cols, pitch, blocks, codes, scales);
     return hipGetLastError();
 }
