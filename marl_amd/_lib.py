@@ -123,7 +123,7 @@ def call(fn, what: str, device, *args) -> None:
     import torch
 
     index = device.index
-    if index == torch.cuda.current_device():
+    if index == torch._C._cuda_getDevice():
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
