@@ -281,7 +281,7 @@ enum {
  *                   byte first.
  *   d_codes   uint8 [num_rows][B][16], 16-byte aligned;   d_scales   uint8 [num_rows][B]
  * d_x: num_rows rows of x_type (MARL_F32, MARL_BF16, MARL_F16), row_stride elements from one row to
- * the next (0 = num_cols).  Fewer than 2^30 blocks a call; no rows is a call that does nothing.
+ * the next (0 = num_cols).  At most 2^30 - 64 blocks a call; no rows is a call that does nothing.
  */
 int marl_mx_quantize(const void *d_x, int x_type, int64_t num_rows, int num_cols, int64_t row_stride,
                      uint8_t *d_codes, uint8_t *d_scales, void *stream);

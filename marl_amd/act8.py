@@ -23,7 +23,7 @@ class Act8:
 
     def __init__(self, codes, scales, nonnegative):
         rows, cols = _bytes_on_gpu(codes, "codes")
-        if cols == 0 or _bytes_on_gpu(scales, "scales") != (rows, -(-cols // BLOCK)) or scales.device != codes.device:
+        if not 0 < cols < 1 << 31 or _bytes_on_gpu(scales, "scales") != (rows, -(-cols // BLOCK)) or scales.device != codes.device:
             raise ValueError("scales must be [rows, ceil(cols / 32)] beside the codes' [rows, cols], on the same device")
         self.codes, self.scales, self.nonnegative = codes, scales, bool(nonnegative)
         self.shape, self.device = codes.shape, codes.device

@@ -94,8 +94,9 @@ act_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restri
 //   gw[o][i] = sum_m g[m][o] x[m][i],   gb[o] = sum_m g[m][o]
 //
 // The sum runs over the rows, 32 of them a step of v_mfma_f32_16x16x32_bf16.  x is a bfloat16 exactly.  A float32 g is
-// the sum of three bfloat16 numbers exactly (its 24 bits cut into eights), so three products with float32 sums give
-// float32's accuracy; a float16 g needs two and a bfloat16 g one.
+// the sum of three bfloat16 numbers exactly (its 24 bits cut into eights; of a g below 2^-109 what lies under bfloat16's
+// smallest, 2^-133, is lost), so three products with float32 sums give float32's accuracy; a float16 g needs two and a
+// bfloat16 g one.
 // Both operands are wanted with the rows innermost: a thread takes 4 (g) or 8 rows (x) of four columns and writes 8 or 16
 // bytes per column and part to LDS, which is the transposition.
 
@@ -238,7 +239,7 @@ struct WeightGrad {
     }
 
     __device__ __forceinline__ void convert_x(const RawX& raw, int buf) const {
-        float s[8], z[8];
+        float s[8];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const int v = (int)f_bits(scale_value(raw.s[k]));
@@ -248,15 +249,12 @@ struct WeightGrad {
             s[4 * k + 3] = bits_f(__builtin_amdgcn_update_dpp(0, v, 0xFF, 0xF, 0xF, true));
         }
 #pragma unroll
-        for (int k = 0; k < 8; ++k) z[k] = -P.zero * s[k];
-#pragma unroll
         for (int c = 0; c < 4; ++c) {
             u32x4 u;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {  // (code - zero) * scale: every step of it is exact
+            for (int k = 0; k < 4; ++k) {  // every step of it is exact (128 times the largest scale, taken off afterwards, would not be)
                 const uint32_t xa = raw.x[2 * k] >> (8 * xback), xb = raw.x[2 * k + 1] >> (8 * xback);
-                u[k] = high_halves(fmaf((float)(xa >> (8 * c) & 255u), s[2 * k], z[2 * k]),
-                                   fmaf((float)(xb >> (8 * c) & 255u), s[2 * k + 1], z[2 * k + 1]));
+                u[k] = high_halves(((float)(xa >> (8 * c) & 255u) - P.zero) * s[2 * k], ((float)(xb >> (8 * c) & 255u) - P.zero) * s[2 * k + 1]);
             }
             *reinterpret_cast<u32x4*>(&S.B[buf][c * (BI / 4) + xc][piece(c * (BI / 4) + xc, xr >> 3)]) = u;
         }
@@ -557,7 +555,7 @@ extern "C" int marl_act_compress(const void* d_x, int x_type, int64_t num_rows, 
     if (row_stride == 0) row_stride = num_cols;
     if (row_stride < num_cols) return set_error(MARL_ERR_INVALID, "row_stride is smaller than num_cols");
     if (((uintptr_t)d_x & (lb_type_bytes(x_type) - 1)) != 0) return set_error(MARL_ERR_INVALID, "d_x must be aligned to its elements");
-    if (too_many_blocks(num_rows, num_cols)) return set_error(MARL_ERR_INVALID, "2^30 or more blocks of 32 values in one call");
+    if (too_many_blocks(num_rows, num_cols)) return set_error(MARL_ERR_INVALID, "more than 2^30 - 64 blocks of 32 values in one call");
     const int blocks = (int)lb_blocks(num_cols);
     const auto pick = [&](auto positive, auto nt) {
         constexpr bool pos = decltype(positive)::value, hint = decltype(nt)::value;
@@ -581,7 +579,7 @@ extern "C" int marl_act_dequantize(const uint8_t* d_codes, const uint8_t* d_scal
     if (num_rows == 0) return MARL_OK;
     if (!d_codes || !d_scales || !d_out) return set_error(MARL_ERR_INVALID, "NULL argument to marl_act_dequantize");
     if (((uintptr_t)d_out & (lb_type_bytes(out_type) - 1)) != 0) return set_error(MARL_ERR_INVALID, "d_out must be aligned to its elements");
-    if (too_many_blocks(num_rows, num_cols)) return set_error(MARL_ERR_INVALID, "2^30 or more blocks of 32 values in one call");
+    if (too_many_blocks(num_rows, num_cols)) return set_error(MARL_ERR_INVALID, "more than 2^30 - 64 blocks of 32 values in one call");
     auto kernel = out_type == MARL_F32 ? act_dequantize_kernel<MARL_F32> : out_type == MARL_BF16 ? act_dequantize_kernel<MARL_BF16>
                                                                                                  : act_dequantize_kernel<MARL_F16>;
     hipLaunchKernelGGL(kernel, dim3(block_grid(num_rows, num_cols)), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), d_codes, d_scales,

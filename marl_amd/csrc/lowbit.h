@@ -127,8 +127,8 @@ __device__ __forceinline__ void store_eight(void* p, int64_t at, int64_t end, co
     }
 }
 
-// Passes over [rows][blocks of 32] have four lanes per block and one thread number for them all, so a call holds fewer
-// than 2^30 blocks (a launch holds fewer than 2^32 threads).  `thread` to row, block of the row, and quarter of the block:
+// Passes over [rows][blocks of 32] have four lanes per block and one thread number for them all, so a call holds at most
+// 2^30 - 64 blocks (a launch, whole workgroups of 256, holds fewer than 2^32 threads).  `thread` to row, block of the row, and quarter of the block:
 __device__ __forceinline__ void split_block(uint32_t thread, uint32_t per_row, int64_t& row, int& b, int& quarter) {
     const uint32_t block = thread >> 2, r = block / per_row;
     row = r;
@@ -136,7 +136,7 @@ __device__ __forceinline__ void split_block(uint32_t thread, uint32_t per_row, i
     quarter = (int)(thread & 3);
 }
 static inline bool too_many_blocks(int64_t rows, int64_t cols) {
-    return rows >= ((int64_t)1 << 30) || (uint64_t)rows * lb_blocks(cols) >= ((uint64_t)1 << 30);
+    return rows >= ((int64_t)1 << 30) || (uint64_t)rows * lb_blocks(cols) > ((uint64_t)1 << 30) - 64;
 }
 static inline uint32_t block_grid(int64_t rows, int64_t cols) {  // workgroups of 256 threads
     return (uint32_t)(((uint64_t)rows * lb_blocks(cols) * 4 + 255) / 256);

@@ -652,7 +652,7 @@ extern "C" int marl_mx_quantize(const void* d_x, int x_type, int64_t num_rows, i
     if (row_stride < num_cols) return set_error(MARL_ERR_INVALID, "row_stride is smaller than num_cols");
     if (((uintptr_t)d_x & (lb_type_bytes(x_type) - 1)) != 0 || ((uintptr_t)d_codes & 15u) != 0)
         return set_error(MARL_ERR_INVALID, "d_x must be aligned to its elements, d_codes to 16 bytes");
-    if (too_many_blocks(num_rows, num_cols)) return set_error(MARL_ERR_INVALID, "2^30 or more blocks of 32 values in one call");
+    if (too_many_blocks(num_rows, num_cols)) return set_error(MARL_ERR_INVALID, "more than 2^30 - 64 blocks of 32 values in one call");
     return hip_result(launch_quantize(d_x, x_type, num_rows, num_cols, row_stride, d_codes, d_scales, reinterpret_cast<hipStream_t>(stream)),
                       "MXFP4 quantisation launch");
 }
@@ -666,7 +666,7 @@ extern "C" int marl_mx_dequantize(const uint8_t* d_codes, const uint8_t* d_scale
     if (!d_codes || !d_scales || !d_out) return set_error(MARL_ERR_INVALID, "NULL argument to marl_mx_dequantize");
     if (((uintptr_t)d_codes & 15u) != 0 || ((uintptr_t)d_out & (lb_type_bytes(out_type) - 1)) != 0)
         return set_error(MARL_ERR_INVALID, "d_codes must be 16-byte aligned, d_out aligned to its elements");
-    if (too_many_blocks(num_rows, num_cols)) return set_error(MARL_ERR_INVALID, "2^30 or more blocks of 32 values in one call");
+    if (too_many_blocks(num_rows, num_cols)) return set_error(MARL_ERR_INVALID, "more than 2^30 - 64 blocks of 32 values in one call");
     const int blocks = (int)lb_blocks(num_cols);
     auto kernel = out_type == MARL_F32 ? mx_dequantize_kernel<MARL_F32> : out_type == MARL_BF16 ? mx_dequantize_kernel<MARL_BF16> : mx_dequantize_kernel<MARL_F16>;
     hipLaunchKernelGGL(kernel, dim3(block_grid(num_rows, num_cols)), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), d_codes, d_scales, num_rows, num_cols, blocks, d_out);
@@ -700,7 +700,7 @@ extern "C" int marl_mx_linear(const void* d_x, const uint8_t* d_x_scales, int x_
         ((uintptr_t)d_bias & 3u) != 0 || ((uintptr_t)d_workspace & 15u) != 0)
         return set_error(MARL_ERR_INVALID, "codes and the workspace must be 16-byte aligned, the others aligned to their elements");
     if (too_many_blocks(num_rows, num_cols) || too_many_blocks(num_rows, num_out) || num_out > (1 << 22))
-        return set_error(MARL_ERR_INVALID, "fewer than 2^30 blocks of 32 values on either side and at most 2^22 output features in one call");
+        return set_error(MARL_ERR_INVALID, "at most 2^30 - 64 blocks of 32 values on either side and at most 2^22 output features in one call");
     if (!mx_short_rows(num_cols) && num_rows > (int64_t)65535 * 64)
         return set_error(MARL_ERR_INVALID, "of rows of fewer than 8 or more than 512 values at most 4,194,240 in one call");
     if (marl_mx_linear_workspace_bytes(x_type, num_rows, num_cols, num_out) != 0 && !d_workspace)

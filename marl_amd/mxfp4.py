@@ -25,6 +25,8 @@ def _rows(x, name):
     if not isinstance(x, torch.Tensor) or x.dtype not in _TYPES or x.dim() != 2 or not x.is_cuda:
         raise ValueError(f"{name} must be a float32, bfloat16 or float16 [rows, cols] tensor on the GPU")
     rows, cols = x.shape
+    if cols >= 1 << 31:  # a C int
+        raise ValueError(f"{name} has 2^31 or more columns")
     if x.is_contiguous():
         if cols == 0:
             raise ValueError(f"{name} has no columns")
@@ -49,7 +51,7 @@ class MXFP4:
     def __init__(self, codes, scales, cols):
         rows, width = _bytes_on_gpu(codes, "codes")
         blocks = -(-cols // BLOCK)
-        if cols <= 0 or width != 16 * blocks or _bytes_on_gpu(scales, "scales") != (rows, blocks) or scales.device != codes.device:
+        if not 0 < cols < 1 << 31 or width != 16 * blocks or _bytes_on_gpu(scales, "scales") != (rows, blocks) or scales.device != codes.device:
             raise ValueError(f"codes and scales of {cols} columns must be [rows, {16 * blocks}] and [rows, {blocks}] on one device")
         self.codes, self.scales, self.shape, self.device = codes, scales, torch.Size((rows, cols)), codes.device
 
@@ -96,19 +98,19 @@ def linear(x, weight, bias=None, relu=False, out_dtype=torch.float32):
     if not isinstance(weight, MXFP4):
         raise ValueError("weight must be an MXFP4 (mxfp4.quantize)")
     n, cols = weight.shape
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (x, bias)):
+        raise ValueError("mxfp4.linear has no gradient: call it under torch.no_grad()")
     if isinstance(x, MXFP4):
         rows, xcols = x.shape
         x_data, x_scales, x_type, stride = x.codes, x.scales, _MXFP4, 0
     else:
-        if isinstance(x, torch.Tensor) and x.requires_grad and torch.is_grad_enabled():
-            raise ValueError("mxfp4.linear has no gradient: call it under torch.no_grad()")
         x, rows, xcols, stride = _rows(x, "x")
         x_data, x_scales, x_type = x, None, _TYPES[x.dtype]
     device = x.device
     if xcols != cols or device != weight.device:
         raise ValueError(f"x has {xcols} columns on {device}, the weight {cols} on {weight.device}")
-    if n == 0:
-        raise ValueError("weight has no rows")
+    if n == 0 or n > 1 << 22:
+        raise ValueError("weight has no rows, or more than 2^22")
     if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or not bias.is_contiguous() or bias.device != device):
         raise ValueError(f"bias must be a contiguous float32 tensor of {n} entries on the device of x")
     if out_dtype == "mxfp4":

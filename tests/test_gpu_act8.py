@@ -171,6 +171,55 @@ def test_largest_gradients_do_not_overflow_in_their_parts():
     assert gw[2].count_nonzero() == 1 and torch.isfinite(gw).all()
 
 
+def test_kept_values_up_to_the_largest():
+    """128 steps of the largest scale are no float32, but no value is 128 steps: what the gradient reads is what is read back"""
+    from marl_amd import act8
+
+    x = torch.zeros(64, 96, device="cuda")
+    x[:, 0], x[:, 1], x[:, 33], x[5, 70] = 3.4028234663852886e38, 1e37, 3.0, -1.7014118346046923e38
+    for rows, out in ((64, 1), (64, 20), (3, 20)):
+        act = act8.compress(x[:rows])
+        g = torch.zeros(rows, out, device="cuda")
+        g[min(5, rows - 1)] = 2.0 ** -100
+        gw, _, _ = act8.weight_grad(g, act)
+        want = act.dequantize()[min(5, rows - 1)] * 2.0 ** -100  # one term: exact
+        assert torch.equal(gw, want.expand(out, 96))
+    # scales that compressing never writes read as the formula says
+    for byte in (0, 1, 249, 254):
+        codes = torch.full((8, 32), 128, dtype=torch.uint8, device="cuda")
+        codes[2, 3] = 129
+        act = act8.Act8(codes, torch.full((8, 1), byte, dtype=torch.uint8, device="cuda"), False)
+        value = 2.0 ** (byte - 127)
+        assert act.dequantize()[2, 3].item() == value and act.dequantize().count_nonzero() == 1
+        gw, _, _ = act8.weight_grad(torch.full((8, 5), 2.0 ** -20 if byte > 200 else 2.0 ** 20, device="cuda"), act)
+        if byte:  # a matrix unit may take bfloat16's denormals for zeros
+            assert (gw[:, 3] == value * (2.0 ** -20 if byte > 200 else 2.0 ** 20)).all()
+        assert gw.count_nonzero() == (5 if byte else gw[:, 3].count_nonzero())
+
+
+def test_offsets_beyond_32_bits():
+    from marl_amd import act8
+
+    rows, cols, last = 4_300_000, 512, 70
+    x = torch.empty(rows, cols, dtype=torch.float16, device="cuda")
+    x.zero_()
+    x[-last:] = _x(last, cols, torch.float16, 1)
+    act, small = act8.compress(x), act8.compress(x[-last:].clone())
+    assert torch.equal(act.codes[-last:], small.codes) and torch.equal(act.scales[-last:], small.scales)
+    back = act.dequantize(torch.bfloat16)
+    assert torch.equal(back[-last:], small.dequantize(torch.bfloat16)) and not back[:-last].any()
+    del back
+    mask = act8.Act8(torch.ones(rows, cols, dtype=torch.uint8, device="cuda"), act.scales, True)
+    mask.codes[-1, ::2] = 0
+    x.zero_()
+    x[-last:] = _x(last, cols, torch.float16, 2)  # now the gradient
+    gw, gb, masked = act8.weight_grad(x, act, mask)
+    assert torch.equal(masked[:-1], x[:-1]) and not masked[-1, ::2].any() and torch.equal(masked[-1, 1::2], x[-1, 1::2])
+    g, xv = masked[-last:].double(), small.dequantize().double()
+    for got, want, size in ((gw.double(), g.t() @ xv, g.abs().t() @ xv.abs()), (gb.double(), g.sum(0), g.abs().sum(0))):
+        assert ((got - want).abs() <= last * 2.0 ** -23 * size).all()
+
+
 def test_every_output_is_written_and_nothing_else():
     from marl_amd import _lib, act8
     from marl_amd.mxfp4 import _p
@@ -248,3 +297,5 @@ def test_refusals():
         act8.Act8(act.codes.int(), act.scales, True)
     with pytest.raises(ValueError):
         act.dequantize(torch.float64)
+    with pytest.raises(ValueError):  # a C int counts the columns
+        act8.compress(torch.empty(1, (1 << 32) + 32, dtype=torch.float16, device="cuda"))

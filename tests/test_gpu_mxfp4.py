@@ -232,6 +232,46 @@ def test_two_calls_at_once_do_not_share_anything():
         assert all(torch.equal(y, want[k]) for y in got[k])
 
 
+def test_offsets_beyond_32_bits():
+    from marl_amd import mxfp4
+
+    rows, cols, last = 4_300_000, 512, 40  # many rows: values, codes, results behind 2^32 bytes, values behind 2^31 elements
+    x = torch.empty(rows, cols, dtype=torch.float16, device="cuda")
+    x.zero_()
+    x[-last:] = torch.from_numpy(np.random.default_rng(1).standard_normal((last, cols))).half()
+    w = mxfp4.quantize(torch.from_numpy(np.random.default_rng(2).standard_normal((512, cols))).float().cuda())
+    q, small = mxfp4.quantize(x), mxfp4.quantize(x[-last:].clone())
+    assert torch.equal(q.codes[-last:], small.codes) and torch.equal(q.scales[-last:], small.scales) and not q.codes[:-last].any()
+    back = q.dequantize(torch.float16)
+    assert torch.equal(back[-last:], small.dequantize(torch.float16)) and not back[:-last].any()
+    del back
+    y, want = mxfp4.linear(x, w, out_dtype=torch.float16), mxfp4.linear(small, w, out_dtype=torch.float16)
+    assert torch.equal(y[-last:], want) and not y[:-last].any()
+    del y
+    y = mxfp4.linear(q, w, out_dtype="mxfp4")
+    want = mxfp4.linear(small, w, out_dtype="mxfp4")
+    assert torch.equal(y.codes[-last:], want.codes) and torch.equal(y.scales[-last:], want.scales)
+
+
+@pytest.mark.parametrize("rows", [1, 20])
+def test_a_weight_beyond_32_bits(rows):
+    """rows of 2^26 values, the last of them in the row's last stretch: 4.7 GB of codes"""
+    from marl_amd import mxfp4
+
+    out, cols = 140, (1 << 26) - 7
+    w = torch.zeros(out, cols, dtype=torch.float16, device="cuda")
+    x = torch.zeros(rows, cols, dtype=torch.float16, device="cuda")
+    w[:, 3], w[:, -5:], x[:, 3] = 1.0, torch.arange(1, 6, device="cuda").half() / 2, 2.0
+    w[-1, -1] = 6.0
+    x[:, -5:] = torch.tensor([1.0, 2.0, 0.5, 4.0, 3.0], device="cuda").half()
+    # The rows of 0.5 .. 2.5 have a scale of 1/2, of which they are 1, 2, 3, 4 and 5, halfway between 4 and 6: the even code is
+    # 4's, so 2.5 reads as 2.  The last row (a scale of 1) and x are MXFP4 numbers as they stand.
+    read = w[:, -5:].float()
+    read[:-1, 4] = 2.0
+    want = read @ x[:, -5:].float().t() + 2.0
+    assert torch.equal(mxfp4.linear(x, mxfp4.quantize(w)), want.t())
+
+
 def test_refusals():
     from marl_amd import mxfp4
 
@@ -258,3 +298,10 @@ def test_refusals():
         mxfp4.MXFP4(w.codes[:, :16], w.scales, 40)
     with pytest.raises(ValueError):
         mxfp4.quantize(x, out=w)
+    with pytest.raises(ValueError):  # a C int counts the columns
+        mxfp4.quantize(torch.empty(1, (1 << 32) + 32, dtype=torch.float16, device="cuda"))
+    learned = torch.zeros(w.shape[0], device="cuda", requires_grad=True)
+    with pytest.raises(ValueError):
+        mxfp4.linear(x, w, learned)
+    with torch.no_grad():
+        mxfp4.linear(x, w, learned)
