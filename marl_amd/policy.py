@@ -16,6 +16,7 @@ import warnings
 
 import torch
 from torch import nn
+from torch.autograd.function import once_differentiable
 from torch.distributions import Categorical
 
 from . import act8, mxfp4
@@ -209,6 +210,7 @@ class _KeptLinear(torch.autograd.Function):
         return out, kept.codes, kept.scales
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, gy, *_kept):
         codes, scales, weight, out_codes, out_scales = ctx.saved_tensors
         mask = None if out_codes is None else act8.Act8(out_codes, out_scales, True)
@@ -267,7 +269,8 @@ class Agent(nn.Module):
         value stay in float32.  The log-probabilities that a rollout stores are those of the policy that acted, so the PPO
         ratio starts from it.  `rollout_step` reads the weights as `refresh_rollout_heads` last quantised them; every other call
         quantises them anew."""
-        self._acting = {}
+        if self._acting is None:  # captured launches read the weights where they are
+            self._acting = {}
         return self
 
     def use_activation_checkpoints(self):
@@ -291,16 +294,21 @@ class Agent(nn.Module):
         """network(x) for acting: in 4 bits if `use_mxfp4_rollouts` asked for it, as `_trunk` otherwise"""
         if self._acting is None or not x.is_cuda or torch.is_grad_enabled():
             return self._trunk(x)
-        l0, l1 = self.network[0], self.network[2]
-        h = mxfp4.linear(x, self._acting_weight("network.0", l0, fresh), l0.bias.detach(), relu=True, out_dtype="mxfp4")
-        return mxfp4.linear(h, self._acting_weight("network.2", l1, fresh), l1.bias.detach(), relu=True)
+        rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+        h = self._acting_layer("network.2", self.network[2], self._acting_layer("network.0", self.network[0], rows, fresh, "mxfp4"), fresh)
+        return h if x.dim() == 2 else h.view(*x.shape[:-1], -1)
+
+    def _acting_layer(self, name, layer, x, fresh, out_dtype=None):
+        """relu(x W^T + b) in 4 bits, of the rows of x or of the layer before's result"""
+        return mxfp4.linear(x, self._acting_weight(name, layer, fresh), layer.bias.detach().float(), relu=True,
+                            out_dtype=out_dtype or layer.weight.dtype)
 
     def _acting_central(self, joint_obs, fresh=False):
         if self._acting is None or not joint_obs.is_cuda or torch.is_grad_enabled() or self.centralised_critics is None:
             return self._central(joint_obs)
         c = self.centralised_critics
-        h = mxfp4.linear(joint_obs, self._acting_weight("centralised_critics.0", c[0], fresh), c[0].bias.detach(), relu=True)
-        return _linear(c[4], _linear(c[2], h, True), False)
+        h = self._acting_layer("centralised_critics.0", c[0], joint_obs.reshape(-1, joint_obs.shape[-1]), fresh)
+        return _linear(c[4], _linear(c[2], h, True), False).view(*joint_obs.shape[:-1], 1)
 
     def _kept_heads(self, x):
         """logits and value with every activation kept in 8 bits: both heads as one layer, so that the hidden layer is read once"""
@@ -350,16 +358,20 @@ class Agent(nn.Module):
             value = self._acting_central(joint_obs) if joint_obs is not None else _linear(self.critic, hidden, False)
             action, logprob, entropy = self.sampler.sample(logits)
             return action, logprob, entropy, value
+        given = action is not None
         if joint_obs is None and self._keeps(x):
             logits, value = self._kept_heads(x)
         else:
-            hidden = self._acting_trunk(x) if action is None else self._trunk(x)
+            hidden = self._trunk(x) if given else self._acting_trunk(x)
             logits, value = _linear(self.actor, hidden, False), None
         dist = Categorical(logits=logits, validate_args=False)
         if action is None:
             action = dist.sample()
         if value is None:
-            value = self._central(joint_obs) if joint_obs is not None else _linear(self.critic, hidden, False)
+            if joint_obs is None:
+                value = _linear(self.critic, hidden, False)
+            else:
+                value = self._central(joint_obs) if given else self._acting_central(joint_obs)
         return action, dist.log_prob(action), dist.entropy(), value
 
     def refresh_rollout_heads(self):

@@ -110,6 +110,57 @@ def test_a_rollout_step_replayed_from_a_graph_follows_the_refreshed_weights():
         torch.testing.assert_close(got, want, rtol=1e-5, atol=1e-5)
 
 
+def test_asking_twice_leaves_the_weights_where_captured_launches_read_them():
+    net, _ = _agent()
+    net.use_fused_sampling(3).use_mxfp4_rollouts()
+    net.refresh_rollout_heads()
+    held = {k: w.codes.data_ptr() for k, w in net._acting.items()}
+    net.use_mxfp4_rollouts()
+    net.refresh_rollout_heads()
+    assert held and {k: w.codes.data_ptr() for k, w in net._acting.items()} == held
+
+
+def test_acting_without_the_fused_sampler_and_on_any_shape():
+    net, _ = _agent(num_envs=16)
+    x = _obs(32, 202)
+    net.use_mxfp4_rollouts()
+    with torch.no_grad():
+        own = net.get_action_and_value(x, joint_obs=x.view(1, -1))[3]
+        rows = net.get_prob(x).logits
+        # the head's library call differs with the shape
+        torch.testing.assert_close(net.get_prob(x.view(4, 8, 202)).logits, rows.view(4, 8, 7), rtol=1e-5, atol=1e-5)
+        torch.testing.assert_close(net.get_prob(x[5]).logits, rows[5], rtol=1e-5, atol=1e-5)
+        exact = net.get_value(x, joint_obs=x.view(1, -1))
+        net.use_fused_sampling(3)
+        fused = net.get_action_and_value(x, joint_obs=x.view(1, -1))[3]
+    assert torch.equal(own, fused) and not torch.equal(own, exact)
+
+
+def test_acting_of_a_policy_in_bfloat16():
+    net, _ = _agent()
+    x = _obs(600, 202)
+    net = net.bfloat16().use_mxfp4_rollouts()
+    with torch.no_grad():
+        hidden = net._acting_trunk(x.bfloat16())
+    l0, l1 = net.network[0], net.network[2]
+    h = x.double().cpu().numpy()
+    for layer in (l0, l1):
+        w = ref.mxfp4(layer.weight.detach().double().cpu().numpy())[2]
+        h = np.maximum(ref.mxfp4(h)[2] @ w.T + layer.bias.detach().double().cpu().numpy(), 0.0).astype(np.float32).astype(np.float64)
+    assert hidden.dtype == torch.bfloat16
+    # one rounding to bfloat16 of sums that are off by a few float32 steps of their terms
+    np.testing.assert_allclose(hidden.double().cpu().numpy(), h, rtol=2.0 ** -8, atol=2e-5)
+
+
+def test_kept_activations_have_no_second_derivative():
+    net, _ = _agent(central=False)
+    net.use_activation_checkpoints()
+    logits, value = net.logits_and_value(_obs(20, 202))
+    g = torch.autograd.grad(logits.square().sum() + value.sum(), net.network[0].weight, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+
+
 def test_the_centralised_critic_acts_in_4_bits():
     net, _ = _agent(num_envs=16)
     x = _obs(32, 202)
