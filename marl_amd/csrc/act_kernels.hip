@@ -472,12 +472,13 @@ act_weight_grad_kernel(ActGrad P) {
     pass.run(split, turn % tiles);
 }
 
-// Sums of the splits in double: the weight's entries, then the bias's.  A workgroup has 64 entries, its four waves every
-// fourth split each, and their four sums are added in order.
-__global__ void __launch_bounds__(256)
+// Sums of the splits in double: the weight's entries, then the bias's.  A workgroup has 64 entries, its WAVES waves every
+// WAVES-th split each, and their sums are added in order.
+template <int WAVES>
+__global__ void __launch_bounds__(64 * WAVES)
 act_join_kernel(const float* __restrict__ part_w, const float* __restrict__ part_b, int64_t nw, int nb, int splits,
                 float* __restrict__ gw, float* __restrict__ gb) {
-    __shared__ double sums[4][64];
+    __shared__ double sums[WAVES][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t at = (int64_t)blockIdx.x * 64 + lane;
     const bool bias = at >= nw, live = at < nw + nb;
@@ -486,20 +487,22 @@ act_join_kernel(const float* __restrict__ part_w, const float* __restrict__ part
     double s = 0.0;
     if (live)
 #pragma unroll 8
-        for (int k = wave; k < splits; k += 4) s += (double)p[k * step];
+        for (int k = wave; k < splits; k += WAVES) s += (double)p[k * step];
     sums[wave][lane] = s;
     __syncthreads();
     if (wave || !live) return;
-    const float v = (float)((sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]));
-    if (bias) gb[at - nw] = v;
-    else gw[at] = v;
+    double all = 0.0;
+#pragma unroll
+    for (int k = 0; k < WAVES; ++k) all += sums[k][lane];
+    if (bias) gb[at - nw] = (float)all;
+    else gw[at] = (float)all;
 }
 
 // ------------------------------------------------------------------------------------------------------------ host
 
 // How a weight gradient is cut: the tile, and into how many splits of the rows.  Measured in us (float32, with a mask):
-//   out <= 16: tiles of 16 x 256; a split has 8 steps, where there are few rows 2 (2048 x 8 x 256: 8.3, with 8 steps 17.6),
-//     since the sums of few entries over many splits are slow to join (65000 x 8 x 256: 17.8, with 512 splits 19.4)
+//   out <= 16: tiles of 16 x 256 on two workgroups a compute unit; a split has at least 4 steps, where there are few rows 2
+//     (65000 x 8 x 256: 15.6, with 8 steps 17.9, 2 steps 19.7; 2048 x 8 x 256: 7.6, with 8 steps 17.6)
 //   otherwise tiles of 128 x 256 on one workgroup a compute unit where there is work for them with 4 steps a split (8192 x 512 x
 //     202: 24.5, with small tiles 28.5), else 64 x 64 on two with 4 steps (2048 x 512 x 202: 14.5; 2 steps 18.5, 8 steps 15.8)
 struct ActCut { int bo, bi, splits; int64_t grid; };
@@ -513,7 +516,7 @@ static ActCut act_cut(int64_t rows, int out, int cols) {
     const int64_t t = tiles(c.bo, c.bi);
     int64_t s = (c.bo == 128 ? 256 : 512) / t;
     s = s < 1 ? 1 : s;
-    const int64_t least = c.bo == 16 ? (steps > 512 ? 8 : 2) : 4, most = (steps + least - 1) / least;
+    const int64_t least = c.bo == 16 ? (steps > 512 ? 4 : 2) : 4, most = (steps + least - 1) / least;
     s = s > most ? most : s;
     const int64_t each = (steps + s - 1) / s;
     c.splits = (int)((steps + each - 1) / each);
@@ -628,8 +631,10 @@ extern "C" int marl_act_weight_grad(const void* d_grad, int grad_type, int64_t n
     else launch_weight_grad_type<MARL_F16>(P, c, s);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || c.splits == 1) return act_hip(e, "weight gradient launch");
-    const int64_t threads = nw + num_out;
-    hipLaunchKernelGGL(act_join_kernel, dim3((uint32_t)((threads + 63) / 64)), dim3(256), 0, s, P.gw, P.gb, nw, num_out, c.splits,
-                       d_grad_weight, d_grad_bias);
+    const int64_t groups = (nw + num_out + 63) / 64;
+    // where the entries leave half of the compute units empty, four times the waves to each (65000 x 8 x 256: 17.9 against 20.0)
+    const bool few = groups < 128;
+    hipLaunchKernelGGL(few ? act_join_kernel<16> : act_join_kernel<4>, dim3((uint32_t)groups), dim3(few ? 1024 : 256), 0, s, P.gw, P.gb, nw,
+                       num_out, c.splits, d_grad_weight, d_grad_bias);
     return act_hip(hipGetLastError(), "weight gradient join launch");
 }
