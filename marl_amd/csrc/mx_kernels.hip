@@ -177,7 +177,7 @@ __device__ __forceinline__ void mx_store(const MxLinear& P, int64_t m, bool live
 // another, and walks row tiles; a wave keeps its 64 features' whole weight in registers (at most 64 of them).  The threads
 // quantise a tile's rows into LDS (four lanes per block, as above); the next tile's values are on their way from memory
 // meanwhile.  Bound by memory: rows in, results out, the weight once per workgroup.  float32 rows and results: 131072 x 202 ->
-// 512 in 79 us (4.7 TB/s), 131072 x 512 -> 256 in 82 us (4.9 TB/s; with MXFP4 rows 38 us); what is missing to a copy's rate
+// 512 in 79 us (4.7 TB/s), 131072 x 512 -> 256 in 80 us (5.0 TB/s; with MXFP4 rows 33 us); what is missing to a copy's rate
 // is the stores', 64 bytes of 16 rows at a time.  Few rows take 5 to 10 us, most of it the weight's way into the registers.
 template <int WN>
 struct MxTile {
@@ -208,14 +208,25 @@ __device__ __forceinline__ void raw_use(const MxRaw<TYPE>& raw, float (&v)[8]) {
     }
 }
 
+// Workgroups on a compute unit.  MXFP4 results of float rows are small and leave the quantising, which two overlap (131072 x 202
+// -> 512 in float32: 48 against 41 us) where the registers suffice (not with 16 blocks a row, 59 and 65 us, nor with the 64 rows
+// that two waves side by side have, 24 and 28).  Elsewhere two read the weight twice and are slower (131072 x 512 -> 256: in
+// float32 87 against 90 us, from MXFP4 to MXFP4 27 and 35; 21847 x 420 -> 250 in bfloat16 15 and 18).
+constexpr int mx_workgroups(int ks, int in, int out, int wn) { return out == MARL_MXFP4 && in != MARL_MXFP4 && ks == 2 && wn > 2 ? 2 : 1; }
+
 template <int KS, int IN, int OUT, int WN>
-__global__ void __launch_bounds__(512)
+__global__ void __launch_bounds__(512, 2 * mx_workgroups(KS, IN, OUT, WN))
 mx_rows_kernel(MxLinear P) {
     typedef MxTile<WN> T;
     constexpr int NB = KS * 4;             // blocks of a row, padded to whole matrix instructions
     constexpr int PITCH = NB * 16 + 16;    // LDS bytes per row of codes; the 16 keep a wave's rows apart in the banks
     constexpr int ITEMS = T::ROWS * NB * (IN == MARL_MXFP4 ? 1 : 4) / 512 > 0 ? T::ROWS * NB * (IN == MARL_MXFP4 ? 1 : 4) / 512 : 1;
     constexpr bool AHEAD = ITEMS <= 4;     // whether the next tile's values fit in registers meanwhile
+    // Whether the next tile is filled in before this one is multiplied, and loads go out two tiles earlier: a store does not
+    // hold up the loads behind it then.  131072 rows: MXFP4 512 -> 256 in 32.5 us, otherwise 37; float32 202 -> 512 80 and 82.
+    // It takes registers: MXFP4 results of float rows, which live on two workgroups a compute unit, 45 and 42.
+    constexpr bool PIPED = IN == MARL_MXFP4 || (IN == MARL_F32 && OUT != MARL_MXFP4 && WN > 2);
+    static_assert(!PIPED || AHEAD, "two tiles' values in registers");
     __shared__ __align__(16) uint8_t codes[2][T::ROWS][PITCH];
     __shared__ __align__(16) uint8_t scales[2][T::ROWS][16];  // [block % 4][block / 4]: a lane's scales are one word
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
@@ -246,31 +257,31 @@ mx_rows_kernel(MxLinear P) {
     // An item: 8 values of a block (float rows) or a whole block (codes).  Rows behind the last are the last again, their
     // results are not stored; every path makes the same loads.
     const int64_t all = (P.rows - 1) * P.pitch + P.cols;  // elements from the first row's start to the last one's end
-    MxRaw<IN == MARL_MXFP4 ? MARL_BF16 : IN> raw[AHEAD ? ITEMS : 1];
-    uint32_t raw_s[AHEAD ? ITEMS : 1];
-    const auto load = [&](int64_t tile, int q, int slot) {
+    MxRaw<IN == MARL_MXFP4 ? MARL_BF16 : IN> raw[PIPED ? 2 : 1][AHEAD ? ITEMS : 1];
+    uint32_t raw_s[PIPED ? 2 : 1][AHEAD ? ITEMS : 1];
+    const auto load = [&](int64_t tile, int q, int set, int slot) {
         const int it = tid + q * 512;
         if constexpr (IN == MARL_MXFP4) {
             const int64_t m = min(tile * T::ROWS + it / NB, P.rows - 1) * P.blocks + min(it % NB, P.blocks - 1);
-            raw[slot].u[0] = reinterpret_cast<const u32x4*>(P.x)[m];
-            raw_s[slot] = P.x_scales[m];
+            raw[set][slot].u[0] = reinterpret_cast<const u32x4*>(P.x)[m];
+            raw_s[set][slot] = P.x_scales[m];
         } else {
             const int64_t m = min(tile * T::ROWS + (it >> 2) / NB, P.rows - 1);
-            raw_load<IN>(raw[slot], P.x, min(m * P.pitch + (it >> 2) % NB * LB_BLOCK + (it & 3) * 8, all - 8));
+            raw_load<IN>(raw[set][slot], P.x, min(m * P.pitch + (it >> 2) % NB * LB_BLOCK + (it & 3) * 8, all - 8));
         }
     };
-    const auto quantise = [&](int64_t tile, int q, int slot, int buf) {
+    const auto quantise = [&](int64_t tile, int q, int set, int slot, int buf) {
         const int it = tid + q * 512;
         if (T::ROWS * NB * (IN == MARL_MXFP4 ? 1 : 4) < 512 && it >= T::ROWS * NB * (IN == MARL_MXFP4 ? 1 : 4)) return;
         if constexpr (IN == MARL_MXFP4) {
             const int row = it / NB, b = it % NB;
             const bool there = b < P.blocks;
-            *reinterpret_cast<u32x4*>(&codes[buf][row][b * 16]) = there ? raw[slot].u[0] : u32x4{0, 0, 0, 0};
-            scales[buf][row][(b & 3) * 4 + (b >> 2)] = (uint8_t)(there ? raw_s[slot] : 127u);
+            *reinterpret_cast<u32x4*>(&codes[buf][row][b * 16]) = there ? raw[set][slot].u[0] : u32x4{0, 0, 0, 0};
+            scales[buf][row][(b & 3) * 4 + (b >> 2)] = (uint8_t)(there ? raw_s[set][slot] : 127u);
         } else {
             const int quarter = it & 3, b = (it >> 2) % NB, row = (it >> 2) / NB;
             float v[8];
-            raw_use<IN>(raw[slot], v);
+            raw_use<IN>(raw[set][slot], v);
             // What lies behind a row's end is the next row, and counts as 0; only behind the last row there is nothing, and
             // its last values were read as the tensor's last eight: move them down.
             const int64_t back = min(tile * T::ROWS + row, P.rows - 1) * P.pitch + b * LB_BLOCK + quarter * 8 - (all - 8);
@@ -289,10 +300,12 @@ mx_rows_kernel(MxLinear P) {
         }
     };
 
-    const int64_t tiles = (P.rows + T::ROWS - 1) / T::ROWS;
+    const int64_t tiles = (P.rows + T::ROWS - 1) / T::ROWS, step = gridDim.x;
     if constexpr (AHEAD) {
 #pragma unroll
-        for (int q = 0; q < ITEMS; ++q) load(blockIdx.x, q, q);
+        for (int set = 0; set < (PIPED ? 2 : 1); ++set)
+#pragma unroll
+            for (int q = 0; q < ITEMS; ++q) load(blockIdx.x + set * step, q, set, q);
     }
     int ws[4];
 #pragma unroll
@@ -302,15 +315,7 @@ mx_rows_kernel(MxLinear P) {
         for (int ks = 0; ks < KS; ++ks) word |= wsb[t][ks] << (8 * ks);
         ws[t] = (int)word;
     }
-    int buf = 0;
-    for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, buf ^= 1) {
-#pragma unroll
-        for (int q = 0; q < ITEMS; ++q) {
-            if constexpr (!AHEAD) load(tile, q, 0);
-            quantise(tile, q, AHEAD ? q : 0, buf);
-            if constexpr (AHEAD) load(tile + gridDim.x, q, q);
-        }
-        __syncthreads();  // one barrier a tile: the other buffer is free once every wave has come here
+    const auto multiply = [&](int64_t tile, int buf) {
 #pragma unroll
         for (int rt = 0; rt < T::GROUPS; ++rt) {
             f32x4 acc[4];
@@ -329,6 +334,39 @@ mx_rows_kernel(MxLinear P) {
             for (int k = 0; k < 16; ++k) v[k] = acc[k >> 2][k & 3] + bias[k];
             const int64_t m = tile * T::ROWS + row;
             mx_store<OUT>(P, m, m < P.rows, n0, g, v);
+        }
+    };
+    // One barrier a tile: the other buffer is free once every wave has come there.
+    if constexpr (PIPED) {
+        // a tile's values, loaded into raw[set], into LDS buffer `buf`, and the loads of the next tile for that set
+        const auto fill = [&](int64_t tile, int buf, int set) {
+#pragma unroll
+            for (int q = 0; q < ITEMS; ++q) quantise(tile, q, set, q, buf);
+#pragma unroll
+            for (int q = 0; q < ITEMS; ++q) load(tile + 2 * step, q, set, q);
+        };
+        fill(blockIdx.x, 0, 0);
+        __syncthreads();
+        for (int64_t tile = blockIdx.x; tile < tiles; tile += 2 * step) {
+            if (tile + step < tiles) fill(tile + step, 1, 1);
+            multiply(tile, 0);
+            __syncthreads();
+            if (tile + step >= tiles) break;
+            if (tile + 2 * step < tiles) fill(tile + 2 * step, 0, 0);
+            multiply(tile + step, 1);
+            __syncthreads();
+        }
+    } else {
+        int buf = 0;
+        for (int64_t tile = blockIdx.x; tile < tiles; tile += step, buf ^= 1) {
+#pragma unroll
+            for (int q = 0; q < ITEMS; ++q) {
+                if constexpr (!AHEAD) load(tile, q, 0, 0);
+                quantise(tile, q, 0, AHEAD ? q : 0, buf);
+                if constexpr (AHEAD) load(tile + step, q, 0, q);
+            }
+            __syncthreads();
+            multiply(tile, buf);
         }
     }
 }
@@ -560,10 +598,7 @@ static void launch_rows(const MxLinear& P, int in, int out, hipStream_t stream) 
     auto kernel = in == MARL_F32 ? rows_kernel_out<KS, WN, MARL_F32>(out) : in == MARL_BF16 ? rows_kernel_out<KS, WN, MARL_BF16>(out)
                 : in == MARL_F16 ? rows_kernel_out<KS, WN, MARL_F16>(out) : rows_kernel_out<KS, WN, MARL_MXFP4>(out);
     const int64_t tiles = (P.rows + MxTile<WN>::ROWS - 1) / MxTile<WN>::ROWS;
-    // One workgroup a compute unit: two read the weight twice and are slower where results are written out in full (131072
-    // x 512 -> 256 in float32: 87 against 90 us; 21847 x 420 -> 250 in bfloat16: 15 against 18); MXFP4 results are small
-    // and leave the conversions, which two overlap (131072 x 202 -> 512: 48 against 41 us).
-    const int64_t resident = out == MARL_MXFP4 ? 512 : 256;
+    const int64_t resident = 256 * mx_workgroups(KS, in, out, WN);
     hipLaunchKernelGGL(kernel, dim3((uint32_t)(tiles < resident ? tiles : resident), (P.out + 64 * WN - 1) / (64 * WN)), dim3(512), 0, stream, P);
 }
 template <int KS>
