@@ -44,8 +44,8 @@ def compress(x, nonnegative=False):
     its largest value, so a value is off by at most half that; a positive one that would round to 0 becomes one step."""
     x, rows, cols, stride = _rows(x, "x")
     out = Act8.__new__(Act8)
-    out.codes = torch.empty((rows, cols), dtype=torch.uint8, device=x.device)
-    out.scales = torch.empty((rows, -(-cols // BLOCK)), dtype=torch.uint8, device=x.device)
+    out.codes = torch.empty(rows, cols, dtype=torch.uint8, device=x.device)
+    out.scales = torch.empty(rows, -(-cols // BLOCK), dtype=torch.uint8, device=x.device)
     out.nonnegative, out.shape, out.device = bool(nonnegative), x.shape, x.device
     _lib.call(_lib.lib().marl_act_compress, "marl_act_compress", x.device, x.data_ptr(), _TYPES[x.dtype], rows, cols, stride,
               1 if nonnegative else 0, out.codes.data_ptr(), out.scales.data_ptr())
@@ -66,10 +66,10 @@ def weight_grad(grad, act, mask=None):
     if mask is not None and (not isinstance(mask, Act8) or not mask.nonnegative or mask.shape != grad.shape or mask.device != device):
         raise ValueError("mask must be a nonnegative Act8 of grad's shape, on its device")
     cols = act.shape[1]
-    masked = torch.empty((rows, out), dtype=grad.dtype, device=device) if mask is not None else None
+    masked = torch.empty_like(grad) if mask is not None else None
     if rows == 0:
         return torch.zeros((out, cols), device=device), torch.zeros(out, device=device), masked
-    gw = torch.empty((out, cols), dtype=torch.float32, device=device)
+    gw = torch.empty(out, cols, dtype=torch.float32, device=device)
     gb = torch.empty(out, dtype=torch.float32, device=device)
     L = _lib.lib()
     need = L.marl_act_weight_grad_workspace_bytes(rows, out, cols)

@@ -72,8 +72,8 @@ class MXFP4:
 def _empty(rows, cols, device):
     blocks = -(-cols // BLOCK)
     new = MXFP4.__new__(MXFP4)
-    new.codes = torch.empty((rows, 16 * blocks), dtype=torch.uint8, device=device)
-    new.scales = torch.empty((rows, blocks), dtype=torch.uint8, device=device)
+    new.codes = torch.empty(rows, 16 * blocks, dtype=torch.uint8, device=device)
+    new.scales = torch.empty(rows, blocks, dtype=torch.uint8, device=device)
     new.shape, new.device = torch.Size((rows, cols)), device
     return new
 
@@ -117,7 +117,7 @@ def linear(x, weight, bias=None, relu=False, out_dtype=torch.float32):
         y = _empty(rows, n, device)
         y_data, y_scales, y_type = y.codes, y.scales, _MXFP4
     elif out_dtype in _TYPES:
-        y = y_data = torch.empty((rows, n), dtype=out_dtype, device=device)
+        y = y_data = torch.empty(rows, n, dtype=out_dtype, device=device)
         y_scales, y_type = None, _TYPES[out_dtype]
     else:
         raise ValueError('out_dtype must be torch.float32, torch.bfloat16, torch.float16 or "mxfp4"')
