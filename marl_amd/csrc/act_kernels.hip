@@ -182,12 +182,13 @@ __device__ __forceinline__ uint32_t load_four_bytes(const uint8_t* p, uint32_t a
 // A column of the tile lies in LDS at (column % 4) * (columns / 4) + column / 4, so that the lanes of a wave, which take
 // four neighbouring columns each, write to neighbouring places, and a lane's results are four neighbouring inputs.
 //
-// 131072 rows x 256 outputs x 512 inputs, float32 gradient with a mask: 116 us and 6 us for the joining kernel.  237 MB
-// come from HBM once (46 us at 5.17 TB/s) and three bf16 products take 85 us at the rate of a large one (1.2 PFLOP/s);
-// both tile columns read g, both tile rows x, 470 MB through the compute units at 4.1 TB/s, and that holds it now.
-// Measured and no faster, 118 to 137 us: 1024 threads; waves that only load and convert before waves that only multiply,
-// over three buffers; loads three and four steps ahead.  Larger tiles read less but double the partial sums of each
-// workgroup, whose joining costs as much again.
+// 131072 rows x 256 outputs x 512 inputs, float32 gradient with a mask: 119 us and 6 us for the joining kernel (bfloat16, one
+// product: 91 and 6).  237 MB come from HBM once and 168 MB go there, 78 us at a copy's rate; three bf16 products take 85 us at
+// the rate of a large library product, 41 us at the matrix units' own.  Those are busy 35 % of the time and the vector units as
+// long, and a wave waits 38 % of it, for loads and at the barrier: 254 registers leave two waves to a SIMD, which overlap only
+// partly.  Measured and no faster, 118 to 137 us: 1024 threads; waves that only load and convert before waves that only multiply,
+// over three buffers; loads three and four steps ahead; a quarter fewer vector instructions.  Two workgroups a compute unit
+// double the partial sums (16 MB): 10 us more.
 template <int TYPE, int BO, int BI, int WO, int WI, bool MASK, bool NARROW>
 struct WeightGrad {
     static constexpr int PARTS = grad_parts<TYPE>(), BYTES = TYPE == MARL_F32 ? 4 : 2;
