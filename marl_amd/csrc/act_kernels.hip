@@ -185,10 +185,10 @@ __device__ __forceinline__ uint32_t load_four_bytes(const uint8_t* p, uint32_t a
 // 131072 rows x 256 outputs x 512 inputs, float32 gradient with a mask: 119 us and 6 us for the joining kernel (bfloat16, one
 // product: 91 and 6).  237 MB come from HBM once and 168 MB go there, 78 us at a copy's rate; three bf16 products take 85 us at
 // the rate of a large library product, 41 us at the matrix units' own.  Those are busy 35 % of the time and the vector units as
-// long, and a wave waits 38 % of it, for loads and at the barrier: 254 registers leave two waves to a SIMD, which overlap only
-// partly.  Measured and no faster, 118 to 137 us: 1024 threads; waves that only load and convert before waves that only multiply,
-// over three buffers; loads three and four steps ahead; a quarter fewer vector instructions.  Two workgroups a compute unit
-// double the partial sums (16 MB): 10 us more.
+// long, and a wave waits 38 % of it, for loads and at the barrier.  Measured and no faster, 118 to 137 us: 1024 threads; waves that
+// only load and convert before waves that only multiply, over three buffers; loads two, three and four steps ahead without any that
+// depends on a condition (bfloat16 with a mask 10 % faster); a quarter fewer vector instructions; fewer output features to the
+// waves that convert g.  Two workgroups a compute unit double the partial sums (16 MB): 10 us more.
 template <int TYPE, int BO, int BI, int WO, int WI, bool MASK, bool NARROW>
 struct WeightGrad {
     static constexpr int PARTS = grad_parts<TYPE>(), BYTES = TYPE == MARL_F32 ? 4 : 2;
@@ -422,11 +422,19 @@ struct WeightGrad {
 #pragma unroll
             for (int b = 0; b < 4; ++b) acc[a][b] = f32x4{0, 0, 0, 0};
 
-        const bool wave_x = wave * 64 < XITEMS, wave_g = wave * 64 + 63 >= THREADS - GITEMS;  // every wave passes the same barriers
-        if (wave_x && wave_g) walk<true, true>();
-        else if (wave_x) walk<true, false>();
-        else if (wave_g) walk<false, true>();
-        else walk<false, false>();
+        // what a wave converts; each form passes the same barriers, and only those that the tile has are there
+        const bool wave_x = wave * 64 < XITEMS, wave_g = wave * 64 + 63 >= THREADS - GITEMS;
+        if constexpr (XITEMS + GITEMS > THREADS) {
+            static_assert(XITEMS == THREADS, "where some have both, all have x");
+            if (wave_g) walk<true, true>();
+            else walk<true, false>();
+        } else if (wave_x) {
+            walk<true, false>();
+        } else if (wave_g) {
+            walk<false, true>();
+        } else if constexpr (XITEMS + GITEMS < THREADS) {
+            walk<false, false>();
+        }
 
         const int r = lane & 15, g = lane >> 4, ic = i0 + 4 * (wi + r);
         float* gw = P.gw + (size_t)split * P.out * P.cols;
