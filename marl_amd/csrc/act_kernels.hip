@@ -140,10 +140,10 @@ __device__ __forceinline__ u32x4 load_four(const void* p, uint32_t at, int have)
     }
     if constexpr (TYPE == MARL_F32) {
         typedef u32x4 u32x4_a4 __attribute__((aligned(4)));
-        return *reinterpret_cast<const u32x4_a4*>(static_cast<const uint32_t*>(p) + at);
+        return *reinterpret_cast<const u32x4_a4*>(static_cast<const uint8_t*>(p) + at * 4u);
     } else {
         typedef u32x2 u32x2_a2 __attribute__((aligned(2)));
-        const u32x2 q = *reinterpret_cast<const u32x2_a2*>(static_cast<const uint16_t*>(p) + at);
+        const u32x2 q = *reinterpret_cast<const u32x2_a2*>(static_cast<const uint8_t*>(p) + at * 2u);
         return u32x4{q.x, q.y, 0, 0};
     }
 }
@@ -182,18 +182,20 @@ __device__ __forceinline__ uint32_t load_four_bytes(const uint8_t* p, uint32_t a
 // A column of the tile lies in LDS at (column % 4) * (columns / 4) + column / 4, so that the lanes of a wave, which take
 // four neighbouring columns each, write to neighbouring places, and a lane's results are four neighbouring inputs.
 //
-// 131072 rows x 256 outputs x 512 inputs, float32 gradient with a mask: 119 us and 6 us for the joining kernel (bfloat16, one
-// product: 91 and 6).  237 MB come from HBM once and 168 MB go there, 78 us at a copy's rate; three bf16 products take 85 us at
+// 131072 rows x 256 outputs x 512 inputs, float32 gradient with a mask: 116 us and 6 us for the joining kernel (bfloat16, one
+// product, 75 and 6).  237 MB come from HBM once and 168 MB go there, 78 us at a copy's rate; three bf16 products take 85 us at
 // the rate of a large library product, 41 us at the matrix units' own.  Those are busy 35 % of the time and the vector units as
-// long, and a wave waits 38 % of it, for loads and at the barrier.  Measured and no faster, 118 to 137 us: 1024 threads; waves that
-// only load and convert before waves that only multiply, over three buffers; loads two, three and four steps ahead without any that
-// depends on a condition (bfloat16 with a mask 10 % faster); a quarter fewer vector instructions; fewer output features to the
-// waves that convert g.  Two workgroups a compute unit double the partial sums (16 MB): 10 us more.
+// long; g and x reach the compute units twice, 470 MB at 4.1 TB/s, which is what loads alone in this order reach (4.5).
+// Measured and no faster, 118 to 137 us: 1024 threads; waves that only load and convert before waves that only multiply, over
+// three buffers; loads three and four steps ahead; a quarter fewer vector instructions; fewer output features to the waves that
+// convert g.  Two workgroups a compute unit double the partial sums (16 MB): 10 us more.
 template <int TYPE, int BO, int BI, int WO, int WI, bool MASK, bool NARROW>
 struct WeightGrad {
     static constexpr int PARTS = grad_parts<TYPE>(), BYTES = TYPE == MARL_F32 ? 4 : 2;
     static constexpr int THREADS = 64 * WO * WI, TO = BO / WO / 16, GITEMS = 2 * BO, XITEMS = BI;
     static_assert(BI == 64 * WI && GITEMS <= THREADS && XITEMS <= THREADS, "a wave has 64 input features, a thread one item of each kind");
+
+    static constexpr bool STEADY = BO == 128;  // every step makes the same loads
 
     struct Lds {
         uint8_t A[2][PARTS][BO][WG_PITCH];
@@ -212,11 +214,15 @@ struct WeightGrad {
     float bsum[4] = {0, 0, 0, 0};
     f32x4 acc[TO][4];
 
-    // Rows behind the last are the last one again (their g counts as 0).  A step's place is the same for the whole
-    // workgroup, what differs from thread to thread is a 32-bit offset (at most 32 rows of 2^20 values).
+    // Rows behind the last are the last one again (their g counts as 0), and in the largest tile, which has many steps, so are
+    // steps behind the last: were the loads left out on some path, the compiler would no longer know how many are under way, and
+    // wait for all (131072 x 512 x 202 with a mask: 100 us in bfloat16, 143 in float32; so 130 and 148).  In the others the steps
+    // there are to spare cost more than that (65000 x 8 x 256 in bfloat16: 14.4 us, with them 15.5).  A step's place is the same
+    // for the whole workgroup, what differs from thread to thread is a 32-bit offset (at most 32 rows of 2^20 values).
     template <bool X, bool G>
     __device__ __forceinline__ void fetch(RawX& x, RawG& g, int64_t m0) const {
-        if (m0 >= last) return;
+        if (!STEADY && m0 >= last) return;
+        m0 = min(m0, last - 1);
         const int lim = (int)min(last - 1 - m0, (int64_t)WG_STEP - 1);
         if constexpr (X) {
             const uint8_t* codes = P.codes + m0 * P.cols;
@@ -315,10 +321,10 @@ struct WeightGrad {
             const uint32_t at = (uint32_t)((gr + k) * P.out + c0);
             if (c0 + 4 <= P.out) {
                 if constexpr (TYPE == MARL_F32) {
-                    *reinterpret_cast<f32x4_a4*>(reinterpret_cast<float*>(masked) + at) = f32x4{v[k][0], v[k][1], v[k][2], v[k][3]};
+                    *reinterpret_cast<f32x4_a4*>(masked + at * 4u) = f32x4{v[k][0], v[k][1], v[k][2], v[k][3]};
                 } else {
                     typedef u32x2 u32x2_a2 __attribute__((aligned(2)));
-                    *reinterpret_cast<u32x2_a2*>(reinterpret_cast<uint16_t*>(masked) + at) =
+                    *reinterpret_cast<u32x2_a2*>(masked + at * 2u) =
                         u32x2{(uint32_t)to_half_type<TYPE>(v[k][0]) | (uint32_t)to_half_type<TYPE>(v[k][1]) << 16,
                               (uint32_t)to_half_type<TYPE>(v[k][2]) | (uint32_t)to_half_type<TYPE>(v[k][3]) << 16};
                 }
@@ -326,8 +332,8 @@ struct WeightGrad {
 #pragma unroll
                 for (int c = 0; c < 3; ++c) {
                     if (c0 + c >= P.out) continue;
-                    if constexpr (TYPE == MARL_F32) reinterpret_cast<float*>(masked)[at + c] = v[k][c];
-                    else reinterpret_cast<uint16_t*>(masked)[at + c] = to_half_type<TYPE>(v[k][c]);
+                    if constexpr (TYPE == MARL_F32) *reinterpret_cast<float*>(masked + (at + c) * 4u) = v[k][c];
+                    else *reinterpret_cast<uint16_t*>(masked + (at + c) * 2u) = to_half_type<TYPE>(v[k][c]);
                 }
             }
         }
@@ -360,7 +366,7 @@ struct WeightGrad {
 
     template <bool X, bool G>
     __device__ __forceinline__ void convert(const RawX& x, const RawG& g, int64_t m0, int buf) {
-        if (m0 >= last) return;
+        if (!STEADY && m0 >= last) return;
         if constexpr (X) convert_x(x, buf);
         if constexpr (G)
             if (has_g) convert_g(g, m0, buf);
@@ -386,7 +392,8 @@ struct WeightGrad {
         __syncthreads();
         for (int64_t m0 = first; m0 < last; m0 += 2 * stride) {
             step<X, G>(x1, g1, m0, 0);
-            if (m0 + stride < last) step<X, G>(x0, g0, m0 + stride, 1);
+            if (m0 + stride >= last) break;
+            step<X, G>(x0, g0, m0 + stride, 1);
         }
     }
 
