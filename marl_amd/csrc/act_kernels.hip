@@ -184,7 +184,7 @@ __device__ __forceinline__ uint32_t load_four_bytes(const uint8_t* p, uint32_t a
 //
 // 131072 rows x 256 outputs x 512 inputs, float32 gradient with a mask: 116 us and 6 us for the joining kernel (bfloat16, one
 // product, 75 and 6).  237 MB come from HBM once and 168 MB go there, 78 us at a copy's rate; three bf16 products take 85 us at
-// the rate of a large library product, 41 us at the matrix units' own.  Those are busy 35 % of the time and the vector units as
+// the rate of a large library product, 41 us at the matrix units' own.  Those are busy 37 % of the time and the vector units as
 // long; g and x reach the compute units twice, 470 MB at 4.1 TB/s, which is what loads alone in this order reach (4.5).
 // Measured and no faster, 118 to 137 us: 1024 threads; waves that only load and convert before waves that only multiply, over
 // three buffers; loads three and four steps ahead; a quarter fewer vector instructions; fewer output features to the waves that
