@@ -268,6 +268,26 @@ def test_same_bits_every_time_on_any_stream_and_from_a_graph():
         assert all(torch.equal(a, b) for a, b in zip(out3, want))
 
 
+def test_two_calls_at_once_do_not_share_anything():
+    from marl_amd import act8
+
+    cases = []
+    for k, (rows, out, cols) in enumerate(((30000, 256, 512), (30000, 8, 256), (2048, 70, 202))):
+        x, y = _x(rows, cols, torch.float32, k), _x(rows, out, torch.float32, 10 + k, "relu")
+        cases.append((_x(rows, out, torch.float32, 20 + k), act8.compress(x), act8.compress(y, nonnegative=True)))
+    want = [act8.weight_grad(*c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for case, stream in zip(cases, streams):
+            with torch.cuda.stream(stream):
+                got.append(act8.weight_grad(*case))
+    torch.cuda.synchronize()
+    for k, r in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(r, want[k % len(cases)]))
+
+
 def test_no_rows():
     from marl_amd import act8
 

@@ -120,6 +120,23 @@ def test_asking_twice_leaves_the_weights_where_captured_launches_read_them():
     assert held and {k: w.codes.data_ptr() for k, w in net._acting.items()} == held
 
 
+def test_a_copied_policy_acts_with_weights_of_its_own(tmp_path):
+    net, _ = _agent()
+    x = _obs(64, 202)
+    net.use_mxfp4_rollouts()
+    with torch.no_grad():
+        before = net.get_prob(x).logits.clone()
+        twin = copy.deepcopy(net)
+        torch.save(net.state_dict(), tmp_path / "net.pth")  # the 4-bit weights are no part of it
+        for p in net.network.parameters():
+            p.mul_(2.0)
+        assert not torch.equal(net.get_prob(x).logits, before)
+        assert torch.equal(twin.get_prob(x).logits, before)
+        assert twin._acting["network.0"].codes.data_ptr() != net._acting["network.0"].codes.data_ptr()
+        net.load_state_dict(torch.load(tmp_path / "net.pth", weights_only=True))
+        assert torch.equal(net.get_prob(x).logits, before)
+
+
 def test_acting_without_the_fused_sampler_and_on_any_shape():
     net, _ = _agent(num_envs=16)
     x = _obs(32, 202)

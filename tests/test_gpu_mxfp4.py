@@ -232,6 +232,18 @@ def test_two_calls_at_once_do_not_share_anything():
         assert all(torch.equal(y, want[k]) for y in got[k])
 
 
+@pytest.mark.parametrize("cols", [5, 202, 700])
+def test_no_rows(cols):
+    from marl_amd import mxfp4
+
+    w = mxfp4.quantize(torch.ones(9, cols, device="cuda"))
+    x = torch.zeros(0, cols, device="cuda")
+    q = mxfp4.quantize(x)
+    assert q.shape == (0, cols) and q.dequantize().shape == (0, cols)
+    for rows in (x, q):
+        assert mxfp4.linear(rows, w).shape == (0, 9) and mxfp4.linear(rows, w, out_dtype="mxfp4").shape == (0, 9)
+
+
 def test_offsets_beyond_32_bits():
     from marl_amd import mxfp4
 
