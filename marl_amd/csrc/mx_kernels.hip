@@ -101,10 +101,14 @@ struct MxLinear {
     int splits;
 };
 
-template <int OUT> constexpr int mx_span() { return OUT == MARL_F32 ? 4 : OUT == MARL_MXFP4 ? 16 : 8; }
+// NT tiles of 16 features to a wave, 4 or 2
+template <int OUT, int NT> constexpr int mx_span() {
+    constexpr int most = OUT == MARL_F32 ? 4 : OUT == MARL_MXFP4 ? 16 : 8;
+    return most < 4 * NT ? most : 4 * NT;
+}
 // first of the four neighbouring features that lane group g has from tile t
-template <int OUT> __device__ __forceinline__ int mx_feature(int t, int g) {
-    constexpr int SPAN = mx_span<OUT>(), TILES = SPAN / 4;
+template <int OUT, int NT> __device__ __forceinline__ int mx_feature(int t, int g) {
+    constexpr int SPAN = mx_span<OUT, NT>(), TILES = SPAN / 4;
     return t / TILES * (4 * SPAN) + g * SPAN + t % TILES * 4;
 }
 
@@ -121,36 +125,45 @@ __device__ __forceinline__ f32x4 mx_mfma(u32x4 a, u32x4 b, f32x4 c, int ks, int 
 
 // Results of one lane: row m, v[4 t + i] is feature n0 + mx_feature(t, g) + i.  All lanes of the wave come here together
 // (the MXFP4 form exchanges maxima between lanes); `live` says whether row m exists.
-template <int OUT>
-__device__ __forceinline__ void mx_store(const MxLinear& P, int64_t m, bool live, int n0, int g, float (&v)[16]) {
+template <int OUT, int NT>
+__device__ __forceinline__ void mx_store(const MxLinear& P, int64_t m, bool live, int n0, int g, float (&v)[4 * NT]) {
+    constexpr int SPAN = mx_span<OUT, NT>();
     if (P.relu) {
 #pragma unroll
-        for (int k = 0; k < 16; ++k) v[k] = v[k] < 0.0f ? 0.0f : v[k];  // a NaN stays
+        for (int k = 0; k < 4 * NT; ++k) v[k] = v[k] < 0.0f ? 0.0f : v[k];  // a NaN stays
     }
     if constexpr (OUT == MARL_MXFP4) {
-        const int n = n0 + 16 * g;
+        const int n = n0 + SPAN * g;
         uint32_t top = 0;
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
+        for (int k = 0; k < SPAN; ++k) {
             if (n + k >= P.out) v[k] = 0.0f;
             top = max(top, f_bits(v[k]) & 0x7FFFFFFFu);
         }
-        top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));  // the lane with the block's other half
+        top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));  // the lanes with the rest of the block
+        if constexpr (NT == 2) top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
         const int yb = (P.out + LB_BLOCK - 1) / LB_BLOCK, b = n / LB_BLOCK;
         if (!live || b >= yb) return;
         const uint32_t byte = mx_scale_byte(top);
-        float lo[8], hi[8];
+        uint32_t* to = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(P.y) + (m * yb + b) * 16 + (n & (LB_BLOCK - 1)) / 2);
+        float part[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) { lo[k] = v[k]; hi[k] = v[8 + k]; }
-        *reinterpret_cast<u32x2*>(static_cast<uint8_t*>(P.y) + (m * yb + b) * 16 + (n & 16) / 2) = u32x2{mx_codes(lo, byte), mx_codes(hi, byte)};
-        if ((n & 16) == 0) P.y_scales[m * yb + b] = (uint8_t)byte;
+        for (int k = 0; k < 8; ++k) part[k] = v[k];
+        if constexpr (SPAN == 16) {
+            float rest[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) rest[k] = v[8 + k];
+            *reinterpret_cast<u32x2*>(to) = u32x2{mx_codes(part, byte), mx_codes(rest, byte)};
+        } else {
+            *to = mx_codes(part, byte);
+        }
+        if ((n & (LB_BLOCK - 1)) == 0) P.y_scales[m * yb + b] = (uint8_t)byte;
     } else {
         if (!live) return;
         const int64_t row = m * P.out;
-        constexpr int SPAN = mx_span<OUT>();
 #pragma unroll
-        for (int s = 0; s < 16 / SPAN; ++s) {
-            const int n = n0 + mx_feature<OUT>(s * SPAN / 4, g);
+        for (int s = 0; s < 4 * NT / SPAN; ++s) {
+            const int n = n0 + mx_feature<OUT, NT>(s * SPAN / 4, g);
             if (n + SPAN <= P.out) {
                 if constexpr (OUT == MARL_F32) {
                     *reinterpret_cast<f32x4_a4*>(static_cast<float*>(P.y) + row + n) = f32x4{v[4 * s], v[4 * s + 1], v[4 * s + 2], v[4 * s + 3]};
@@ -173,15 +186,16 @@ __device__ __forceinline__ void mx_store(const MxLinear& P, int64_t m, bool live
     }
 }
 
-// Rows of 8 to 512 values.  A workgroup has eight waves, WN of them side by side (64 features each) and 8 / WN below one
-// another, and walks row tiles; a wave keeps its 64 features' whole weight in registers (at most 64 of them).  The threads
+// Rows of 8 to 512 values.  A workgroup has eight waves, WN of them side by side (16 NT = 64 features each) and 8 / WN below one
+// another, and walks row tiles; a wave keeps its features' whole weight in registers (at most 64 of them).  The threads
 // quantise a tile's rows into LDS (four lanes per block, as above); the next tile's values are on their way from memory
 // meanwhile.  Bound by memory: rows in, results out, the weight once per workgroup.  float32 rows and results: 131072 x 202 ->
 // 512 in 79 us (4.7 TB/s), 131072 x 512 -> 256 in 80 us (5.0 TB/s; with MXFP4 rows 33 us); what is missing to a copy's rate
-// is the stores', 64 bytes of 16 rows at a time.  Few rows take 5 to 10 us, most of it the weight's way into the registers.
-template <int WN>
+// is the stores', 64 bytes of 16 rows at a time.  Few rows, with 32 features to a wave and one
+// tile to a workgroup, take 3 to 5 us, of which a launch is 2.
+template <int WN, int NT>
 struct MxTile {
-    static constexpr int WM = 8 / WN, GROUPS = WN == 8 ? 2 : 1;  // waves along the rows; groups of 16 rows each of them has
+    static constexpr int WM = 8 / WN, GROUPS = WN == 8 && NT == 4 ? 2 : 1;  // waves along the rows; groups of 16 rows each of them has
     static constexpr int ROWS = 16 * WM * GROUPS;
 };
 
@@ -214,10 +228,10 @@ __device__ __forceinline__ void raw_use(const MxRaw<TYPE>& raw, float (&v)[8]) {
 // float32 87 against 90 us, from MXFP4 to MXFP4 27 and 35; 21847 x 420 -> 250 in bfloat16 15 and 18).
 constexpr int mx_workgroups(int ks, int in, int out, int wn) { return out == MARL_MXFP4 && in != MARL_MXFP4 && ks == 2 && wn > 2 ? 2 : 1; }
 
-template <int KS, int IN, int OUT, int WN>
+template <int KS, int IN, int OUT, int WN, int NT>
 __global__ void __launch_bounds__(512, 2 * mx_workgroups(KS, IN, OUT, WN))
 mx_rows_kernel(MxLinear P) {
-    typedef MxTile<WN> T;
+    typedef MxTile<WN, NT> T;
     constexpr int NB = KS * 4;             // blocks of a row, padded to whole matrix instructions
     constexpr int PITCH = NB * 16 + 16;    // LDS bytes per row of codes; the 16 keep a wave's rows apart in the banks
     constexpr int ITEMS = T::ROWS * NB * (IN == MARL_MXFP4 ? 1 : 4) / 512 > 0 ? T::ROWS * NB * (IN == MARL_MXFP4 ? 1 : 4) / 512 : 1;
@@ -225,20 +239,20 @@ mx_rows_kernel(MxLinear P) {
     // Whether the next tile is filled in before this one is multiplied, and loads go out two tiles earlier: a store does not
     // hold up the loads behind it then.  131072 rows: MXFP4 512 -> 256 in 32.5 us, otherwise 37; float32 202 -> 512 80 and 82.
     // It takes registers: MXFP4 results of float rows, which live on two workgroups a compute unit, 45 and 42.
-    constexpr bool PIPED = IN == MARL_MXFP4 || (IN == MARL_F32 && OUT != MARL_MXFP4 && WN > 2);
+    constexpr bool PIPED = NT == 4 && (IN == MARL_MXFP4 || (IN == MARL_F32 && OUT != MARL_MXFP4 && WN > 2));
     static_assert(!PIPED || AHEAD, "two tiles' values in registers");
     __shared__ __align__(16) uint8_t codes[2][T::ROWS][PITCH];
     __shared__ __align__(16) uint8_t scales[2][T::ROWS][16];  // [block % 4][block / 4]: a lane's scales are one word
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
-    const int n0 = (blockIdx.y * WN + wave % WN) * 64, wm = wave / WN * 16 * T::GROUPS;
+    const int n0 = (blockIdx.y * WN + wave % WN) * (16 * NT), wm = wave / WN * 16 * T::GROUPS;
     // Features behind the last are the last again (their results are not stored), blocks behind a row's end its last one again
     // (x is zero there): no load hangs on a condition, so that all of them are under way together.
-    u32x4 w[4][KS];
-    uint32_t wsb[4][KS];
-    float bias[16];
+    u32x4 w[NT][KS];
+    uint32_t wsb[NT][KS];
+    float bias[4 * NT];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        const int64_t row = (int64_t)min(n0 + mx_feature<OUT>(t, r >> 2) + (r & 3), P.out - 1) * P.blocks;
+    for (int t = 0; t < NT; ++t) {
+        const int64_t row = (int64_t)min(n0 + mx_feature<OUT, NT>(t, r >> 2) + (r & 3), P.out - 1) * P.blocks;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             const int64_t at = row + min(ks * 4 + g, P.blocks - 1);
@@ -248,10 +262,10 @@ mx_rows_kernel(MxLinear P) {
     }
     if (P.bias) {
 #pragma unroll
-        for (int k = 0; k < 16; ++k) bias[k] = P.bias[min(n0 + mx_feature<OUT>(k >> 2, g) + (k & 3), P.out - 1)];
+        for (int k = 0; k < 4 * NT; ++k) bias[k] = P.bias[min(n0 + mx_feature<OUT, NT>(k >> 2, g) + (k & 3), P.out - 1)];
     } else {
 #pragma unroll
-        for (int k = 0; k < 16; ++k) bias[k] = 0.0f;
+        for (int k = 0; k < 4 * NT; ++k) bias[k] = 0.0f;
     }
 
     // An item: 8 values of a block (float rows) or a whole block (codes).  Rows behind the last are the last again, their
@@ -307,9 +321,9 @@ mx_rows_kernel(MxLinear P) {
 #pragma unroll
             for (int q = 0; q < ITEMS; ++q) load(blockIdx.x + set * step, q, set, q);
     }
-    int ws[4];
+    int ws[NT];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < NT; ++t) {
         uint32_t word = 0;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) word |= wsb[t][ks] << (8 * ks);
@@ -318,22 +332,22 @@ mx_rows_kernel(MxLinear P) {
     const auto multiply = [&](int64_t tile, int buf) {
 #pragma unroll
         for (int rt = 0; rt < T::GROUPS; ++rt) {
-            f32x4 acc[4];
+            f32x4 acc[NT];
 #pragma unroll
-            for (int t = 0; t < 4; ++t) acc[t] = f32x4{0, 0, 0, 0};
+            for (int t = 0; t < NT; ++t) acc[t] = f32x4{0, 0, 0, 0};
             const int row = wm + rt * 16 + r;
             const int xs = *reinterpret_cast<const int*>(&scales[buf][row][g * 4]);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 const u32x4 x = *reinterpret_cast<const u32x4*>(&codes[buf][row][(ks * 4 + g) * 16]);
 #pragma unroll
-                for (int t = 0; t < 4; ++t) acc[t] = mx_mfma(w[t][ks], x, acc[t], ks, ws[t], xs);
+                for (int t = 0; t < NT; ++t) acc[t] = mx_mfma(w[t][ks], x, acc[t], ks, ws[t], xs);
             }
-            float v[16];
+            float v[4 * NT];
 #pragma unroll
-            for (int k = 0; k < 16; ++k) v[k] = acc[k >> 2][k & 3] + bias[k];
+            for (int k = 0; k < 4 * NT; ++k) v[k] = acc[k >> 2][k & 3] + bias[k];
             const int64_t m = tile * T::ROWS + row;
-            mx_store<OUT>(P, m, m < P.rows, n0, g, v);
+            mx_store<OUT, NT>(P, m, m < P.rows, n0, g, v);
         }
     };
     // One barrier a tile: the other buffer is free once every wave has come there.
@@ -356,6 +370,11 @@ mx_rows_kernel(MxLinear P) {
             multiply(tile + step, 1);
             __syncthreads();
         }
+    } else if constexpr (NT == 2) {  // a workgroup has one tile
+#pragma unroll
+        for (int q = 0; q < ITEMS; ++q) quantise(blockIdx.x, q, 0, q, 0);
+        __syncthreads();
+        multiply(blockIdx.x, 0);
     } else {
         int buf = 0;
         for (int64_t tile = blockIdx.x; tile < tiles; tile += step, buf ^= 1) {
@@ -463,7 +482,7 @@ mx_stream_kernel(MxLinear P) {
     // rows and features behind the last are the last again, their results are not stored
     int64_t wrow[4], xrow[RM];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) wrow[t] = (int64_t)min(n0 + mx_feature<OUT>(t, r >> 2) + (r & 3), P.out - 1) * P.blocks;
+    for (int t = 0; t < 4; ++t) wrow[t] = (int64_t)min(n0 + mx_feature<OUT, 4>(t, r >> 2) + (r & 3), P.out - 1) * P.blocks;
 #pragma unroll
     for (int q = 0; q < RM; ++q) xrow[q] = min(m0 + q * 16 + r, P.rows - 1) * P.blocks;
     const uint8_t* xc = static_cast<const uint8_t*>(P.x);
@@ -507,16 +526,16 @@ mx_stream_kernel(MxLinear P) {
             float* part = P.part + ((int64_t)blockIdx.z * P.rows + m) * P.out;
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
-                const int n = n0 + mx_feature<OUT>(k >> 2, g) + (k & 3);
+                const int n = n0 + mx_feature<OUT, 4>(k >> 2, g) + (k & 3);
                 if (n < P.out) part[n] = v[k];
             }
         } else {
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
-                const int n = n0 + mx_feature<OUT>(k >> 2, g) + (k & 3);
+                const int n = n0 + mx_feature<OUT, 4>(k >> 2, g) + (k & 3);
                 v[k] += P.bias && n < P.out ? P.bias[n] : 0.0f;
             }
-            mx_store<OUT>(P, m, m < P.rows, n0, g, v);
+            mx_store<OUT, 4>(P, m, m < P.rows, n0, g, v);
         }
     }
 }
@@ -584,29 +603,37 @@ static hipError_t launch_quantize(const void* x, int type, int64_t rows, int col
     return hipGetLastError();
 }
 
-template <int KS, int WN, int IN>
+template <int KS, int WN, int NT, int IN>
 static void (*rows_kernel_out(int out))(MxLinear) {
     switch (out) {
-        case MARL_F32: return mx_rows_kernel<KS, IN, MARL_F32, WN>;
-        case MARL_BF16: return mx_rows_kernel<KS, IN, MARL_BF16, WN>;
-        case MARL_F16: return mx_rows_kernel<KS, IN, MARL_F16, WN>;
-        default: return mx_rows_kernel<KS, IN, MARL_MXFP4, WN>;
+        case MARL_F32: return mx_rows_kernel<KS, IN, MARL_F32, WN, NT>;
+        case MARL_BF16: return mx_rows_kernel<KS, IN, MARL_BF16, WN, NT>;
+        case MARL_F16: return mx_rows_kernel<KS, IN, MARL_F16, WN, NT>;
+        default: return mx_rows_kernel<KS, IN, MARL_MXFP4, WN, NT>;
     }
 }
-template <int KS, int WN>
+template <int KS, int WN, int NT>
 static void launch_rows(const MxLinear& P, int in, int out, hipStream_t stream) {
-    auto kernel = in == MARL_F32 ? rows_kernel_out<KS, WN, MARL_F32>(out) : in == MARL_BF16 ? rows_kernel_out<KS, WN, MARL_BF16>(out)
-                : in == MARL_F16 ? rows_kernel_out<KS, WN, MARL_F16>(out) : rows_kernel_out<KS, WN, MARL_MXFP4>(out);
-    const int64_t tiles = (P.rows + MxTile<WN>::ROWS - 1) / MxTile<WN>::ROWS;
-    const int64_t resident = 256 * mx_workgroups(KS, in, out, WN);
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)(tiles < resident ? tiles : resident), (P.out + 64 * WN - 1) / (64 * WN)), dim3(512), 0, stream, P);
+    auto kernel = in == MARL_F32 ? rows_kernel_out<KS, WN, NT, MARL_F32>(out) : in == MARL_BF16 ? rows_kernel_out<KS, WN, NT, MARL_BF16>(out)
+                : in == MARL_F16 ? rows_kernel_out<KS, WN, NT, MARL_F16>(out) : rows_kernel_out<KS, WN, NT, MARL_MXFP4>(out);
+    const int64_t tiles = (P.rows + MxTile<WN, NT>::ROWS - 1) / MxTile<WN, NT>::ROWS;
+    const int64_t resident = NT == 2 ? tiles : 256 * mx_workgroups(KS, in, out, WN);
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)(tiles < resident ? tiles : resident), (P.out + 16 * NT * WN - 1) / (16 * NT * WN)), dim3(512), 0, stream, P);
 }
 template <int KS>
 static void launch_rows_wide(const MxLinear& P, int in, int out, hipStream_t stream) {
-    // Side by side as many waves as there are features for, so that a row is quantised once.
-    if (P.out <= 128) launch_rows<KS, 2>(P, in, out, stream);
-    else if (P.out <= 256) launch_rows<KS, 4>(P, in, out, stream);
-    else launch_rows<KS, 8>(P, in, out, stream);
+    // Where tiles of 16 rows and 256 features are at most two to a compute unit, those: a wave has half the weight to fetch before it can
+    // multiply, and that is what few rows take.  In us, with them and without: 202 -> 512 in float32 32 rows 3.2 and 5.8, 2048 rows
+    // 3.9 and 6.5, 4096 (512 tiles) 5.8 and 7.1, 8192 9.0 and 7.9; 512 -> 256 from MXFP4 32 rows 4.5 and 8.4, 4096 5.3 and 9.1.
+    const int64_t small = (P.rows + 15) / 16 * ((P.out + 255) / 256);
+    if (small <= 512) {
+        launch_rows<KS, 8, 2>(P, in, out, stream);
+        return;
+    }
+    // Otherwise side by side as many waves as there are features for, so that a row is quantised once.
+    if (P.out <= 128) launch_rows<KS, 2, 4>(P, in, out, stream);
+    else if (P.out <= 256) launch_rows<KS, 4, 4>(P, in, out, stream);
+    else launch_rows<KS, 8, 4>(P, in, out, stream);
 }
 static void (*stream_kernel(int out))(MxLinear) {
     switch (out) {
