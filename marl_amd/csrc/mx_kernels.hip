@@ -190,8 +190,7 @@ __device__ __forceinline__ void mx_store(const MxLinear& P, int64_t m, bool live
 // another, and walks row tiles; a wave keeps its features' whole weight in registers (at most 64 of them).  The threads
 // quantise a tile's rows into LDS (four lanes per block, as above); the next tile's values are on their way from memory
 // meanwhile.  Bound by memory: rows in, results out, the weight once per workgroup.  float32 rows and results: 131072 x 202 ->
-// 512 in 79 us (4.7 TB/s), 131072 x 512 -> 256 in 80 us (5.0 TB/s; with MXFP4 rows 33 us); what is missing to a copy's rate
-// is the stores', 64 bytes of 16 rows at a time.  Few rows, with 32 features to a wave and one
+// 512 in 79 us (4.7 TB/s), 131072 x 512 -> 256 in 75 us (5.4 TB/s; with MXFP4 rows 33 us).  Few rows, with 32 features to a wave and one
 // tile to a workgroup, take 3 to 5 us, of which a launch is 2.
 template <int WN, int NT>
 struct MxTile {
@@ -222,25 +221,27 @@ __device__ __forceinline__ void raw_use(const MxRaw<TYPE>& raw, float (&v)[8]) {
     }
 }
 
-// Workgroups on a compute unit.  MXFP4 results of float rows are small and leave the quantising, which two overlap (131072 x 202
-// -> 512 in float32: 48 against 41 us) where the registers suffice (not with 16 blocks a row, 59 and 65 us, nor with the 64 rows
-// that two waves side by side have, 24 and 28).  Elsewhere two read the weight twice and are slower (131072 x 512 -> 256: in
-// float32 87 against 90 us, from MXFP4 to MXFP4 27 and 35; 21847 x 420 -> 250 in bfloat16 15 and 18).
-constexpr int mx_workgroups(int ks, int in, int out, int wn) { return out == MARL_MXFP4 && in != MARL_MXFP4 && ks == 2 && wn > 2 ? 2 : 1; }
+// Workgroups on a compute unit.  Two where a wave has two tiles of features, and for MXFP4 results of float rows, which are small and
+// leave the quantising, if the registers suffice (131072 x 202 -> 512 in float32: 48 against 41 us; not with 16 blocks a row, 59
+// and 65 us, nor with the 64 rows that two waves side by side have, 24 and 28).  Elsewhere two read the weight twice and are slower
+// (131072 x 512 -> 256 from MXFP4 to MXFP4 27 and 35 us).
+constexpr int mx_workgroups(int ks, int in, int out, int wn, int nt) {
+    return nt == 2 || (out == MARL_MXFP4 && in != MARL_MXFP4 && ks == 2 && wn > 2) ? 2 : 1;
+}
 
-template <int KS, int IN, int OUT, int WN, int NT>
-__global__ void __launch_bounds__(512, 2 * mx_workgroups(KS, IN, OUT, WN))
+// ONE: a workgroup has one tile
+template <int KS, int IN, int OUT, int WN, int NT, bool ONE>
+__global__ void __launch_bounds__(512, 2 * mx_workgroups(KS, IN, OUT, WN, NT))
 mx_rows_kernel(MxLinear P) {
     typedef MxTile<WN, NT> T;
     constexpr int NB = KS * 4;             // blocks of a row, padded to whole matrix instructions
     constexpr int PITCH = NB * 16 + 16;    // LDS bytes per row of codes; the 16 keep a wave's rows apart in the banks
     constexpr int ITEMS = T::ROWS * NB * (IN == MARL_MXFP4 ? 1 : 4) / 512 > 0 ? T::ROWS * NB * (IN == MARL_MXFP4 ? 1 : 4) / 512 : 1;
-    constexpr bool AHEAD = ITEMS <= 4;     // whether the next tile's values fit in registers meanwhile
+    static_assert(ITEMS <= 4, "the next tile's values are in registers meanwhile");
     // Whether the next tile is filled in before this one is multiplied, and loads go out two tiles earlier: a store does not
     // hold up the loads behind it then.  131072 rows: MXFP4 512 -> 256 in 32.5 us, otherwise 37; float32 202 -> 512 80 and 82.
     // It takes registers: MXFP4 results of float rows, which live on two workgroups a compute unit, 45 and 42.
     constexpr bool PIPED = NT == 4 && (IN == MARL_MXFP4 || (IN == MARL_F32 && OUT != MARL_MXFP4 && WN > 2));
-    static_assert(!PIPED || AHEAD, "two tiles' values in registers");
     __shared__ __align__(16) uint8_t codes[2][T::ROWS][PITCH];
     __shared__ __align__(16) uint8_t scales[2][T::ROWS][16];  // [block % 4][block / 4]: a lane's scales are one word
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
@@ -271,8 +272,8 @@ mx_rows_kernel(MxLinear P) {
     // An item: 8 values of a block (float rows) or a whole block (codes).  Rows behind the last are the last again, their
     // results are not stored; every path makes the same loads.
     const int64_t all = (P.rows - 1) * P.pitch + P.cols;  // elements from the first row's start to the last one's end
-    MxRaw<IN == MARL_MXFP4 ? MARL_BF16 : IN> raw[PIPED ? 2 : 1][AHEAD ? ITEMS : 1];
-    uint32_t raw_s[PIPED ? 2 : 1][AHEAD ? ITEMS : 1];
+    MxRaw<IN == MARL_MXFP4 ? MARL_BF16 : IN> raw[PIPED ? 2 : 1][ITEMS];
+    uint32_t raw_s[PIPED ? 2 : 1][ITEMS];
     const auto load = [&](int64_t tile, int q, int set, int slot) {
         const int it = tid + q * 512;
         if constexpr (IN == MARL_MXFP4) {
@@ -315,12 +316,10 @@ mx_rows_kernel(MxLinear P) {
     };
 
     const int64_t tiles = (P.rows + T::ROWS - 1) / T::ROWS, step = gridDim.x;
-    if constexpr (AHEAD) {
 #pragma unroll
-        for (int set = 0; set < (PIPED ? 2 : 1); ++set)
+    for (int set = 0; set < (PIPED ? 2 : 1); ++set)
 #pragma unroll
-            for (int q = 0; q < ITEMS; ++q) load(blockIdx.x + set * step, q, set, q);
-    }
+        for (int q = 0; q < ITEMS; ++q) load(blockIdx.x + set * step, q, set, q);
     int ws[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -370,7 +369,7 @@ mx_rows_kernel(MxLinear P) {
             multiply(tile + step, 1);
             __syncthreads();
         }
-    } else if constexpr (NT == 2) {  // a workgroup has one tile
+    } else if constexpr (ONE) {
 #pragma unroll
         for (int q = 0; q < ITEMS; ++q) quantise(blockIdx.x, q, 0, q, 0);
         __syncthreads();
@@ -380,9 +379,8 @@ mx_rows_kernel(MxLinear P) {
         for (int64_t tile = blockIdx.x; tile < tiles; tile += step, buf ^= 1) {
 #pragma unroll
             for (int q = 0; q < ITEMS; ++q) {
-                if constexpr (!AHEAD) load(tile, q, 0, 0);
-                quantise(tile, q, 0, AHEAD ? q : 0, buf);
-                if constexpr (AHEAD) load(tile + step, q, 0, q);
+                quantise(tile, q, 0, q, buf);
+                load(tile + step, q, 0, q);
             }
             __syncthreads();
             multiply(tile, buf);
@@ -603,21 +601,26 @@ static hipError_t launch_quantize(const void* x, int type, int64_t rows, int col
     return hipGetLastError();
 }
 
-template <int KS, int WN, int NT, int IN>
+template <int KS, int IN, int WN, int NT, bool ONE>
 static void (*rows_kernel_out(int out))(MxLinear) {
     switch (out) {
-        case MARL_F32: return mx_rows_kernel<KS, IN, MARL_F32, WN, NT>;
-        case MARL_BF16: return mx_rows_kernel<KS, IN, MARL_BF16, WN, NT>;
-        case MARL_F16: return mx_rows_kernel<KS, IN, MARL_F16, WN, NT>;
-        default: return mx_rows_kernel<KS, IN, MARL_MXFP4, WN, NT>;
+        case MARL_F32: return mx_rows_kernel<KS, IN, MARL_F32, WN, NT, ONE>;
+        case MARL_BF16: return mx_rows_kernel<KS, IN, MARL_BF16, WN, NT, ONE>;
+        case MARL_F16: return mx_rows_kernel<KS, IN, MARL_F16, WN, NT, ONE>;
+        default: return mx_rows_kernel<KS, IN, MARL_MXFP4, WN, NT, ONE>;
     }
 }
-template <int KS, int WN, int NT>
+// FLOATS, CODES: which rows come here
+template <int KS, int WN, int NT, bool ONE, bool FLOATS, bool CODES>
 static void launch_rows(const MxLinear& P, int in, int out, hipStream_t stream) {
-    auto kernel = in == MARL_F32 ? rows_kernel_out<KS, WN, NT, MARL_F32>(out) : in == MARL_BF16 ? rows_kernel_out<KS, WN, NT, MARL_BF16>(out)
-                : in == MARL_F16 ? rows_kernel_out<KS, WN, NT, MARL_F16>(out) : rows_kernel_out<KS, WN, NT, MARL_MXFP4>(out);
+    void (*kernel)(MxLinear) = nullptr;
+    if constexpr (FLOATS)
+        kernel = in == MARL_F32 ? rows_kernel_out<KS, MARL_F32, WN, NT, ONE>(out) : in == MARL_BF16 ? rows_kernel_out<KS, MARL_BF16, WN, NT, ONE>(out)
+                                                                                                    : rows_kernel_out<KS, MARL_F16, WN, NT, ONE>(out);
+    if constexpr (CODES)
+        if (in == MARL_MXFP4) kernel = rows_kernel_out<KS, MARL_MXFP4, WN, NT, ONE>(out);
     const int64_t tiles = (P.rows + MxTile<WN, NT>::ROWS - 1) / MxTile<WN, NT>::ROWS;
-    const int64_t resident = NT == 2 ? tiles : 256 * mx_workgroups(KS, in, out, WN);
+    const int64_t resident = ONE ? tiles : 256 * mx_workgroups(KS, in, out, WN, NT);
     hipLaunchKernelGGL(kernel, dim3((uint32_t)(tiles < resident ? tiles : resident), (P.out + 16 * NT * WN - 1) / (16 * NT * WN)), dim3(512), 0, stream, P);
 }
 template <int KS>
@@ -626,14 +629,16 @@ static void launch_rows_wide(const MxLinear& P, int in, int out, hipStream_t str
     // multiply, and that is what few rows take.  In us, with them and without: 202 -> 512 in float32 32 rows 3.2 and 5.8, 2048 rows
     // 3.9 and 6.5, 4096 (512 tiles) 5.8 and 7.1, 8192 9.0 and 7.9; 512 -> 256 from MXFP4 32 rows 4.5 and 8.4, 4096 5.3 and 9.1.
     const int64_t small = (P.rows + 15) / 16 * ((P.out + 255) / 256);
-    if (small <= 512) {
-        launch_rows<KS, 8, 2>(P, in, out, stream);
-        return;
-    }
+    if (small <= 512) return launch_rows<KS, 8, 2, true, true, true>(P, in, out, stream);
+    // The same tiles, walked by two workgroups a compute unit, for long float rows whose features they cover: 131072 x 512 -> 256 in
+    // float32 75 us, with four tiles of features to a wave 81; 21847 x 420 -> 250 in bfloat16 11.7 and 13.0; 131072 x 400 -> 100 48
+    // and 65.  Not for short rows (131072 x 202 -> 256 45 and 45, to MXFP4 32 and 25) nor for codes (512 -> 256 37 and 33).
+    if constexpr (KS == 4)
+        if (in != MARL_MXFP4 && P.out <= 256) return launch_rows<KS, 8, 2, false, true, false>(P, in, out, stream);
     // Otherwise side by side as many waves as there are features for, so that a row is quantised once.
-    if (P.out <= 128) launch_rows<KS, 2, 4>(P, in, out, stream);
-    else if (P.out <= 256) launch_rows<KS, 4, 4>(P, in, out, stream);
-    else launch_rows<KS, 8, 4>(P, in, out, stream);
+    if (P.out <= 128) launch_rows<KS, 2, 4, false, KS == 2, true>(P, in, out, stream);
+    else if (P.out <= 256) launch_rows<KS, 4, 4, false, KS == 2, true>(P, in, out, stream);
+    else launch_rows<KS, 8, 4, false, true, true>(P, in, out, stream);
 }
 static void (*stream_kernel(int out))(MxLinear) {
     switch (out) {
