@@ -1,6 +1,6 @@
 #!/usr/bin/env python3
-"""A rollout step (policy, sampling, env) at 65,536 two-agent kitchens with the trunk in float32 and in 4 bits, and forward and
-backward of an update's minibatch with float32 and with 8-bit activations (time, and the peak of allocated memory)."""
+"""A rollout step (policy, sampling, env) at 65,536 two-agent kitchens with the trunk in float32 and in 4 bits, the policy's part of
+it for few kitchens, and forward and backward of an update's minibatch with float32 and with 8-bit activations (time, and the peak of allocated memory)."""
 import os
 import sys
 import time
@@ -59,6 +59,19 @@ def main():
             torch.cuda.reset_peak_memory_stats()
             t = us(update, 10)
             print(f"forward and backward of {M} samples, {bits}-bit activations: {t:.0f} us, peak {torch.cuda.max_memory_allocated() / 1e9:.2f} GB", flush=True)
+    for rows in (32, 512, 4096):  # the policy's part of a step, replayed from a graph of 32 as small rollouts are
+        for precision in ("float32", "mxfp4"):
+            net._acting = None
+            if precision == "mxfp4":
+                net.use_mxfp4_rollouts()
+            net.refresh_rollout_heads()
+            policy = lambda: net.rollout_step(obs[:rows], logp[:rows], value[:rows], actions[:rows])  # noqa: E731
+            us(policy, 3)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                for _ in range(32):
+                    policy()
+            print(f"policy of {rows} rows in a graph, {precision}: {us(graph.replay, 20) / 32:.1f} us", flush=True)
 
 
 if __name__ == "__main__":
