@@ -135,6 +135,15 @@ def test_weight_gradient(rows, out, cols):
             _grad_case(rows, out, cols, dtype, kind, with_mask, rows + out + cols + k, wild=with_mask and k % 2 == 0)
 
 
+@pytest.mark.parametrize("rows,out,cols", [(9001, 300, 520), (33000, 130, 33), (16390, 512, 202), (131, 2000, 1500)])
+def test_weight_gradient_in_the_largest_tiles(rows, out, cols):
+    k = 0
+    for dtype in DTYPES:
+        for kind, with_mask in (("relu", True), ("normal", False)):
+            k += 1
+            _grad_case(rows, out, cols, dtype, kind, with_mask, rows + out + cols + k, wild=with_mask and dtype != torch.float16)
+
+
 def test_rows_that_the_mask_leaves_empty():
     from marl_amd import act8
 

@@ -134,6 +134,34 @@ def test_product_of_float_rows(rows, cols, out):
             _linear_case(x, w, bias, relu, torch.float32)
 
 
+@pytest.mark.parametrize("cols", [8, 202, 256, 257, 512])
+@pytest.mark.parametrize("out", [8, 200, 512])
+def test_many_rows_equal_their_pieces(cols, out):
+    """the forms that many rows take add in the order of those that few take, which are held to 64 bits above"""
+    from marl_amd import mxfp4
+
+    rows, piece = 20011, 4000
+    w, b = mxfp4.quantize(_x(out, cols, torch.float32, 1)), torch.randn(out, device="cuda")
+    for dtype in DTYPES:
+        x = _x(rows, cols, dtype, 2)
+        x[777], x[778, 0], x[-1, -1] = 0.0, float("nan"), float("inf")
+        q = mxfp4.quantize(x)
+        parts = [mxfp4.MXFP4(c.contiguous(), s.contiguous(), cols) for c, s in zip(q.codes.split(piece), q.scales.split(piece))]
+        for out_dtype in (torch.float32, torch.bfloat16, torch.float16):
+            want = torch.cat([mxfp4.linear(v, w, b, relu=True, out_dtype=out_dtype) for v in x.split(piece)])
+            for rows_in in (x, q):
+                torch.testing.assert_close(mxfp4.linear(rows_in, w, b, relu=True, out_dtype=out_dtype), want, rtol=0, atol=0, equal_nan=True)
+            small = torch.cat([mxfp4.linear(v, w, b, relu=True, out_dtype=out_dtype) for v in parts])
+            torch.testing.assert_close(small, want, rtol=0, atol=0, equal_nan=True)
+        want = mxfp4.quantize(mxfp4.linear(x, w, b))
+        for rows_in in (x, q):
+            got = mxfp4.linear(rows_in, w, b, out_dtype="mxfp4")
+            assert torch.equal(got.codes, want.codes) and torch.equal(got.scales, want.scales)
+        for v, c, s in zip(parts, want.codes.split(piece), want.scales.split(piece)):
+            got = mxfp4.linear(v, w, b, out_dtype="mxfp4")
+            assert torch.equal(got.codes, c) and torch.equal(got.scales, s)
+
+
 @pytest.mark.parametrize("rows,cols,out", [(1, 202, 512), (40, 202, 512), (130, 512, 33), (9, 700, 96), (70, 1500, 40)])
 def test_layers_in_a_row_quantised_between(rows, cols, out):
     """out_dtype="mxfp4" holds what quantising the float32 result would give, and is the next layer's x; an x that is
