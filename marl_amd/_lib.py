@@ -25,6 +25,7 @@ EXPORTS = (
 )
 
 _lib = None
+_torch = None
 
 
 class MarlAmdError(RuntimeError):
@@ -120,14 +121,15 @@ def lib() -> ctypes.CDLL:
 def call(fn, what: str, device, *args) -> None:
     """fn(*args, stream) with `device` current and its current stream: an entry point's call for tensors on `device`.
     Small passes are bound by the host, so nothing is switched that is right already."""
-    import torch
-
+    global _torch
+    if _torch is None:
+        import torch as _torch
     index = device.index
-    if index == torch._C._cuda_getDevice():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if index == _torch._C._cuda_getDevice():
+        rc = fn(*args, _torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(index):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        with _torch.cuda.device(index):
+            rc = fn(*args, _torch._C._cuda_getCurrentRawStream(index))
     if rc != 0:
         check(rc, what)
 

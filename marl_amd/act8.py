@@ -32,9 +32,10 @@ class Act8:
         """the values, as a [rows, cols] tensor (exact also in bfloat16)"""
         if dtype not in _TYPES:
             raise ValueError("dtype must be torch.float32, torch.bfloat16 or torch.float16")
-        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        rows, cols = self.shape
+        out = torch.empty(rows, cols, dtype=dtype, device=self.device)
         _lib.call(_lib.lib().marl_act_dequantize, "marl_act_dequantize", self.device, self.codes.data_ptr(), self.scales.data_ptr(),
-                  self.shape[0], self.shape[1], 1 if self.nonnegative else 0, _TYPES[dtype], out.data_ptr())
+                  rows, cols, 1 if self.nonnegative else 0, _TYPES[dtype], out.data_ptr())
         return out
 
 

@@ -188,7 +188,7 @@ __device__ __forceinline__ uint32_t load_four_bytes(const uint8_t* p, uint32_t a
 // long; g and x reach the compute units twice, 470 MB at 4.1 TB/s, which is what loads alone in this order reach (4.5).
 // Measured and no faster, 118 to 137 us: 1024 threads; waves that only load and convert before waves that only multiply, over
 // three buffers; loads three and four steps ahead; a quarter fewer vector instructions; fewer output features to the waves that
-// convert g.  Two workgroups a compute unit double the partial sums (16 MB): 10 us more.
+// convert g.  Two workgroups a compute unit double the partial sums (34 MB): 10 us more.
 template <int TYPE, int BO, int BI, int WO, int WI, bool MASK, bool NARROW>
 struct WeightGrad {
     static constexpr int PARTS = grad_parts<TYPE>(), BYTES = TYPE == MARL_F32 ? 4 : 2;

@@ -63,18 +63,20 @@ class MXFP4:
         """the values, as a [rows, cols] tensor (rounded once more for the 16-bit types)"""
         if dtype not in _TYPES:
             raise ValueError("dtype must be torch.float32, torch.bfloat16 or torch.float16")
-        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        rows, cols = self.shape
+        out = torch.empty(rows, cols, dtype=dtype, device=self.device)
         _lib.call(_lib.lib().marl_mx_dequantize, "marl_mx_dequantize", self.device, self.codes.data_ptr(), self.scales.data_ptr(),
-                  self.shape[0], self.shape[1], _TYPES[dtype], out.data_ptr())
+                  rows, cols, _TYPES[dtype], out.data_ptr())
         return out
 
 
-def _empty(rows, cols, device):
+def _empty(shape, device):
+    rows, cols = shape
     blocks = -(-cols // BLOCK)
     new = MXFP4.__new__(MXFP4)
     new.codes = torch.empty(rows, 16 * blocks, dtype=torch.uint8, device=device)
     new.scales = torch.empty(rows, blocks, dtype=torch.uint8, device=device)
-    new.shape, new.device = torch.Size((rows, cols)), device
+    new.shape, new.device = shape, device
     return new
 
 
@@ -83,7 +85,7 @@ def quantize(x, out=None):
     to write into (a weight that captured launches read) instead of a new one."""
     x, rows, cols, stride = _rows(x, "x")
     if out is None:
-        out = _empty(rows, cols, x.device)
+        out = _empty(x.shape, x.device)
     elif not isinstance(out, MXFP4) or out.shape != x.shape or out.device != x.device:
         raise ValueError(f"out must be an MXFP4 of shape {tuple(x.shape)} on the device of x")
     _lib.call(_lib.lib().marl_mx_quantize, "marl_mx_quantize", x.device, x.data_ptr(), _TYPES[x.dtype], rows, cols, stride,
@@ -114,7 +116,7 @@ def linear(x, weight, bias=None, relu=False, out_dtype=torch.float32):
     if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or not bias.is_contiguous() or bias.device != device):
         raise ValueError(f"bias must be a contiguous float32 tensor of {n} entries on the device of x")
     if out_dtype == "mxfp4":
-        y = _empty(rows, n, device)
+        y = _empty(torch.Size((rows, n)), device)
         y_data, y_scales, y_type = y.codes, y.scales, _MXFP4
     elif out_dtype in _TYPES:
         y = y_data = torch.empty(rows, n, dtype=out_dtype, device=device)
