@@ -70,7 +70,7 @@ def main(argv=None):
     vec = make_vector_env(args.num_envs, env, seed=args.seed, device=device)
     net = load_policy(args.model_path, vec.single_observation_space, vec.single_action_space, args.num_agents, device)
     if args.precision == "mxfp4":
-        net.use_mxfp4_rollouts()
+        net.use_mxfp4_trunk()
     result = run_inference(net, vec, episodes=args.episodes, greedy=args.greedy)
     for k, r in enumerate(result):
         print(json.dumps({"episode": k, "envs": args.num_envs, **r}))

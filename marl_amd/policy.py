@@ -4,7 +4,7 @@ ReLU), ``actor`` (256 -> n_actions), ``critic`` (256 -> 1) and ``centralised_cri
 (obs_dim * num_agents * num_envs -> 512 -> 256 -> 1).  All layers start orthogonal with gain
 sqrt(2) and zero bias (model.py:6-9).  The matrix products run on PyTorch-ROCm (rocBLAS /
 hipBLASLt); which library call computes a layer of a small batch is a fixed function of its
-shape (`_table_form`).  On request the trunk acts in 4-bit floating point (`use_mxfp4_rollouts`, the
+shape (`_table_form`).  On request the trunk is computed in 4-bit floating point (`use_mxfp4_trunk`, the
 HIP passes of `mxfp4`) and keeps its activations for the backward pass in 8 bits
 (`use_activation_checkpoints`, those of `act8`)."""
 from __future__ import annotations
@@ -170,14 +170,21 @@ def _small_gemm_form(x, weight, bias, relu):
     return form
 
 
+def _forward(x, weight, bias, relu, coarse):
+    if coarse is not None:
+        return mxfp4.linear(x, coarse, bias.float(), relu=relu, out_dtype=weight.dtype)
+    return _FORMS[_small_gemm_form(x, weight, bias, relu)](x, weight, bias, relu)
+
+
 class _LinearReLU(torch.autograd.Function):
     """relu(x @ W^T + b) (or without the ReLU): one GEMM with a fused epilogue, or for the small
     batches where that call is slow a plain product plus in-place bias and ReLU; the backward
-    pass forms the weight gradient with `_weight_grad`."""
+    pass forms the weight gradient with `_weight_grad`.  With `coarse`, the weight in 4 bits, the forward pass is
+    `mxfp4.linear`'s and the gradients go straight through its roundings."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, relu):
-        out = _FORMS[_small_gemm_form(x, weight, bias, relu)](x, weight, bias, relu)
+    def forward(ctx, x, weight, bias, relu, coarse=None):
+        out = _forward(x, weight, bias, relu, coarse)
         ctx.relu = relu
         ctx.save_for_backward(x, weight, out if relu else None)
         return out
@@ -189,7 +196,7 @@ class _LinearReLU(torch.autograd.Function):
             gy = torch.ops.aten.threshold_backward(gy, out, 0)
         gy = gy.contiguous()
         gx = gy @ weight if ctx.needs_input_grad[0] else None
-        return gx, _weight_grad(gy, x), gy.sum(0), None
+        return gx, _weight_grad(gy, x), gy.sum(0), None, None
 
 
 class _KeptLinear(torch.autograd.Function):
@@ -199,8 +206,8 @@ class _KeptLinear(torch.autograd.Function):
     kept output's and exact; the forward pass and the gradient of the input are those of `_LinearReLU`."""
 
     @staticmethod
-    def forward(ctx, x, codes, scales, nonnegative, weight, bias, relu):
-        out = _FORMS[_small_gemm_form(x, weight, bias, relu)](x, weight, bias, relu)
+    def forward(ctx, x, codes, scales, nonnegative, weight, bias, relu, coarse=None):
+        out = _forward(x, weight, bias, relu, coarse)
         kept = act8.compress(out, nonnegative=True) if relu else None
         ctx.nonnegative = nonnegative
         ctx.save_for_backward(codes, scales, weight, kept.codes if relu else None, kept.scales if relu else None)
@@ -216,14 +223,14 @@ class _KeptLinear(torch.autograd.Function):
         mask = None if out_codes is None else act8.Act8(out_codes, out_scales, True)
         gw, gb, masked = act8.weight_grad(gy, act8.Act8(codes, scales, ctx.nonnegative), mask)
         gx = (gy if mask is None else masked) @ weight if ctx.needs_input_grad[0] else None
-        return gx, None, None, None, gw, gb, None
+        return gx, None, None, None, gw, gb, None, None
 
 
-def _linear(layer: nn.Linear, x, relu):
+def _linear(layer: nn.Linear, x, relu, coarse=None):
     if x.is_cuda and x.dim() == 2:
-        if x.shape[0] < _SMALL_ROWS:
+        if x.shape[0] < _SMALL_ROWS and coarse is None:
             _announce_blas_switch_quietly(x)
-        return _LinearReLU.apply(x.contiguous(), layer.weight, layer.bias, relu)
+        return _LinearReLU.apply(x.contiguous(), layer.weight, layer.bias, relu, coarse)
     out = layer(x)
     return torch.relu(out) if relu else out
 
@@ -252,25 +259,36 @@ class Agent(nn.Module):
         # decentralised learner never evaluates it and may leave it out.
         self.sampler = None  # set by use_fused_sampling(); plain torch.distributions otherwise
         self._head_w = self._head_b = None  # stacked heads of rollout_step
-        self._acting = None  # 4-bit weights of the layers that act in 4 bits, set by use_mxfp4_rollouts()
+        self._coarse = None  # 4-bit weights of the trunk, set by use_mxfp4_trunk()
         self._keep_in_8_bits = False  # set by use_activation_checkpoints()
         self.centralised_critics = (_mlp([d * self.num_agents * self.num_envs, 512, 256, 1], final_activation=False)
                                     if build_centralised else None)
 
-    def _trunk(self, x):
+    def _trunk(self, x, fresh=False):
         """network(x): each Linear + ReLU pair runs as one hipBLASLt GEMM with the bias and the
         ReLU in its epilogue: the same float32 result bit for bit, one pass less over the
         activations (250 us instead of 365 us for 131,072 x 202 -> 512)."""
-        return _linear(self.network[2], _linear(self.network[0], x, True), True)
+        l0, l1 = self.network[0], self.network[2]
+        if self._coarse is None or not x.is_cuda:
+            return _linear(l1, _linear(l0, x, True), True)
+        rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+        w0, w1 = self._coarse_weight("network.0", l0, fresh), self._coarse_weight("network.2", l1, fresh)
+        if torch.is_grad_enabled():
+            h = _linear(l1, _linear(l0, rows, True, w0), True, w1)
+        else:  # the same numbers, with what lies between the layers in 4 bits
+            h = mxfp4.linear(rows, w0, l0.bias.float(), relu=True, out_dtype="mxfp4")
+            h = mxfp4.linear(h, w1, l1.bias.float(), relu=True, out_dtype=l1.weight.dtype)
+        return h if x.dim() == 2 else h.view(*x.shape[:-1], -1)
 
-    def use_mxfp4_rollouts(self):
-        """Acting (rollouts, evaluation: no autograd) computes the trunk in 4-bit floating point (`mxfp4.linear`), and of the
-        centralised critic its first layer, whose weight is most of what a rollout step reads.  Heads, updates and the bootstrap
-        value stay in float32.  The log-probabilities that a rollout stores are those of the policy that acted, so the PPO
-        ratio starts from it.  `rollout_step` reads the weights as `refresh_rollout_heads` last quantised them; every other call
-        quantises them anew."""
-        if self._acting is None:  # captured launches read the weights where they are
-            self._acting = {}
+    def use_mxfp4_trunk(self):
+        """The trunk is computed in 4-bit floating point (`mxfp4.linear`: weights, observations and the hidden layer), and so is the
+        first layer of the centralised critic, whose weight is most of what a rollout step reads.  Updates train this policy:
+        their forward pass is the same numbers, and the gradients go straight through the roundings to the float32 weights,
+        which the optimizer steps and a checkpoint holds.  (Acting in 4 bits and updating in float32 does not train: the
+        two policies differ by more than the PPO clip.)  Heads stay in float32.  `rollout_step` reads the weights as
+        `refresh_rollout_heads` last quantised them; every other call quantises them anew."""
+        if self._coarse is None:  # captured launches read the weights where they are
+            self._coarse = {}
         return self
 
     def use_activation_checkpoints(self):
@@ -281,34 +299,14 @@ class Agent(nn.Module):
         self._keep_in_8_bits = True
         return self
 
-    def _acting_weight(self, name, layer, fresh):
+    def _coarse_weight(self, name, layer, fresh):
         """`layer`'s weight in 4 bits, in the same storage every time; quantised anew unless `fresh` says that it is current"""
-        held = self._acting.get(name)
+        held = self._coarse.get(name)
         if held is None or held.device != layer.weight.device:
-            held = self._acting[name] = mxfp4.quantize(layer.weight.detach())
+            held = self._coarse[name] = mxfp4.quantize(layer.weight.detach())
         elif not fresh:
             mxfp4.quantize(layer.weight.detach(), out=held)
         return held
-
-    def _acting_trunk(self, x, fresh=False):
-        """network(x) for acting: in 4 bits if `use_mxfp4_rollouts` asked for it, as `_trunk` otherwise"""
-        if self._acting is None or not x.is_cuda or torch.is_grad_enabled():
-            return self._trunk(x)
-        rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-        h = self._acting_layer("network.2", self.network[2], self._acting_layer("network.0", self.network[0], rows, fresh, "mxfp4"), fresh)
-        return h if x.dim() == 2 else h.view(*x.shape[:-1], -1)
-
-    def _acting_layer(self, name, layer, x, fresh, out_dtype=None):
-        """relu(x W^T + b) in 4 bits, of the rows of x or of the layer before's result"""
-        return mxfp4.linear(x, self._acting_weight(name, layer, fresh), layer.bias.detach().float(), relu=True,
-                            out_dtype=out_dtype or layer.weight.dtype)
-
-    def _acting_central(self, joint_obs, fresh=False):
-        if self._acting is None or not joint_obs.is_cuda or torch.is_grad_enabled() or self.centralised_critics is None:
-            return self._central(joint_obs)
-        c = self.centralised_critics
-        h = self._acting_layer("centralised_critics.0", c[0], joint_obs.reshape(-1, joint_obs.shape[-1]), fresh)
-        return _linear(c[4], _linear(c[2], h, True), False).view(*joint_obs.shape[:-1], 1)
 
     def _kept_heads(self, x):
         """logits and value with every activation kept in 8 bits: both heads as one layer, so that the hidden layer is read once"""
@@ -316,8 +314,10 @@ class Agent(nn.Module):
         codes, scales, nonnegative, h = kept.codes, kept.scales, False, x.contiguous()
         if x.shape[0] < _SMALL_ROWS:
             _announce_blas_switch_quietly(x)
-        for layer in (self.network[0], self.network[2]):
-            h, codes, scales = _KeptLinear.apply(h, codes, scales, nonnegative, layer.weight, layer.bias, True)
+        for name in ("network.0", "network.2"):
+            layer = self.get_submodule(name)
+            coarse = None if self._coarse is None else self._coarse_weight(name, layer, False)
+            h, codes, scales = _KeptLinear.apply(h, codes, scales, nonnegative, layer.weight, layer.bias, True, coarse)
             nonnegative = True
         heads = _KeptLinear.apply(h, codes, scales, True, torch.cat([self.actor.weight, self.critic.weight]),
                                   torch.cat([self.actor.bias, self.critic.bias]), False)
@@ -334,11 +334,12 @@ class Agent(nn.Module):
         self.sampler = CategoricalSampler(seed, row_index_base, next(self.parameters()).device)
         return self
 
-    def _central(self, joint_obs):
+    def _central(self, joint_obs, fresh=False):
         if self.centralised_critics is None:
             raise RuntimeError("this Agent was built without its centralised critic (build_centralised=False)")
         c = self.centralised_critics
-        return _linear(c[4], _linear(c[2], _linear(c[0], joint_obs, True), True), False)
+        coarse = None if self._coarse is None or not joint_obs.is_cuda else self._coarse_weight("centralised_critics.0", c[0], fresh)
+        return _linear(c[4], _linear(c[2], _linear(c[0], joint_obs, True, coarse), True), False)
 
     def get_value(self, x, joint_obs=None):
         if joint_obs is not None:
@@ -353,16 +354,15 @@ class Agent(nn.Module):
         # synchronisation per call, and cannot run under hipGraph capture; it changes no result
         if action is None and self.sampler is not None and x.is_cuda and not torch.is_grad_enabled():
             # rollout: sample, log-probability and entropy in one launch
-            hidden = self._acting_trunk(x)
+            hidden = self._trunk(x)
             logits = _linear(self.actor, hidden, False)
-            value = self._acting_central(joint_obs) if joint_obs is not None else _linear(self.critic, hidden, False)
+            value = self._central(joint_obs) if joint_obs is not None else _linear(self.critic, hidden, False)
             action, logprob, entropy = self.sampler.sample(logits)
             return action, logprob, entropy, value
-        given = action is not None
         if joint_obs is None and self._keeps(x):
             logits, value = self._kept_heads(x)
         else:
-            hidden = self._trunk(x) if given else self._acting_trunk(x)
+            hidden = self._trunk(x)
             logits, value = _linear(self.actor, hidden, False), None
         dist = Categorical(logits=logits, validate_args=False)
         if action is None:
@@ -371,7 +371,7 @@ class Agent(nn.Module):
             if joint_obs is None:
                 value = _linear(self.critic, hidden, False)
             else:
-                value = self._central(joint_obs) if given else self._acting_central(joint_obs)
+                value = self._central(joint_obs)
         return action, dist.log_prob(action), dist.entropy(), value
 
     def refresh_rollout_heads(self):
@@ -385,11 +385,11 @@ class Agent(nn.Module):
         with torch.no_grad():
             torch.cat([self.actor.weight, self.critic.weight], out=self._head_w)
             torch.cat([self.actor.bias, self.critic.bias], out=self._head_b)
-        if self._acting is not None:  # the 4-bit weights that rollout_step reads
-            self._acting_weight("network.0", self.network[0], False)
-            self._acting_weight("network.2", self.network[2], False)
-            if self.centralised_critics is not None and "centralised_critics.0" in self._acting:
-                self._acting_weight("centralised_critics.0", self.centralised_critics[0], False)
+        if self._coarse is not None:  # the 4-bit weights that rollout_step reads
+            self._coarse_weight("network.0", self.network[0], False)
+            self._coarse_weight("network.2", self.network[2], False)
+            if self.centralised_critics is not None and "centralised_critics.0" in self._coarse:
+                self._coarse_weight("centralised_critics.0", self.centralised_critics[0], False)
 
     def rollout_step(self, x, logprob_out, value_out, actions_out=None, slot=None, joint=False, row_offset=0):
         """The rollout half of `get_action_and_value` for the decentralised critic, writing the
@@ -409,15 +409,15 @@ class Agent(nn.Module):
             raise RuntimeError("rollout_step needs use_fused_sampling()")
         if joint:
             with torch.no_grad():
-                logits = _linear(self.actor, self._acting_trunk(x, fresh=True), False)
+                logits = _linear(self.actor, self._trunk(x, fresh=True), False)
                 actions, _, _ = self.sampler.sample(logits, want_entropy=False, actions_out=actions_out,
                                                     logprob_out=logprob_out, slot=slot)
-                value_out.copy_(self._acting_central(x.view(1, -1), fresh=True).view(1).expand_as(value_out))
+                value_out.copy_(self._central(x.view(1, -1), fresh=True).view(1).expand_as(value_out))
             return actions
         if getattr(self, "_head_w", None) is None:
             self.refresh_rollout_heads()
         with torch.no_grad():
-            heads = torch.addmm(self._head_b, self._acting_trunk(x, fresh=True), self._head_w.t())
+            heads = torch.addmm(self._head_b, self._trunk(x, fresh=True), self._head_w.t())
             actions, _, _ = self.sampler.sample(heads, want_entropy=False, actions_out=actions_out, logprob_out=logprob_out,
                                                 slot=slot, num_actions=self.actor.out_features, next_column_out=value_out,
                                                 row_offset=row_offset)
@@ -431,4 +431,4 @@ class Agent(nn.Module):
         return _linear(self.actor, hidden, False), _linear(self.critic, hidden, False)
 
     def get_prob(self, x):
-        return Categorical(logits=_linear(self.actor, self._acting_trunk(x), False), validate_args=False)
+        return Categorical(logits=_linear(self.actor, self._trunk(x), False), validate_args=False)

@@ -65,9 +65,9 @@ def build_parser():
                    help="Adam step as one multi-tensor launch (GPU only) or PyTorch's default per-operation launches")
     p.add_argument("--fused-loss", choices=["on", "off"], default="on",
                    help="decentralised MAPPO on the GPU: loss and head gradients from one HIP pass instead of autograd's small ops")
-    p.add_argument("--rollout-precision", choices=["float32", "mxfp4"], default="float32",
-                   help="the trunk of the acting policy in float32, or in 4-bit floating point (marl_amd.mxfp4; needs --sampler "
-                        "fused); updates stay in float32")
+    p.add_argument("--trunk-precision", choices=["float32", "mxfp4"], default="float32",
+                   help="the policy's trunk in float32, or in 4-bit floating point (marl_amd.mxfp4): acting and updates, whose "
+                        "gradients go straight through the roundings to the float32 weights")
     p.add_argument("--activation-bits", type=int, choices=[32, 8], default=32,
                    help="what an update keeps of the trunk's activations for its backward pass: float32, or 8 bits a value "
                         "(marl_amd.act8), a quarter of the memory")
@@ -95,8 +95,6 @@ def main(argv=None):
         raise SystemExit(f"--algorithm {args.algorithm} is outside this build (MAPPO / CMAPPO rollout path only)")
     if args.render:
         raise SystemExit("--render is not available: there is no renderer in this build")
-    if args.rollout_precision == "mxfp4" and args.sampler != "fused":
-        raise SystemExit("--rollout-precision mxfp4 needs --sampler fused")
     rank, local_rank, world = dist_utils.init_from_env()
     local_rank %= max(torch.cuda.device_count(), 1)
     torch.cuda.set_device(local_rank)
@@ -128,8 +126,8 @@ def main(argv=None):
     dist_utils.broadcast_parameters(net)
     if args.sampler == "fused":
         net.use_fused_sampling(args.seed, row_index_base=rank * args.num_envs * args.num_agents)
-    if args.rollout_precision == "mxfp4":
-        net.use_mxfp4_rollouts()
+    if args.trunk_precision == "mxfp4":
+        net.use_mxfp4_trunk()
     if args.activation_bits == 8:
         net.use_activation_checkpoints()
     # main.py:294.  fused: the whole Adam step is one multi-tensor launch instead of seventeen

@@ -40,7 +40,7 @@ def main():
 
     for precision in ("float32", "mxfp4"):
         if precision == "mxfp4":
-            net.use_mxfp4_rollouts()
+            net.use_mxfp4_trunk()
         net.refresh_rollout_heads()
         t = us(step, 50)
         print(f"rollout step, {precision}: {t:.1f} us, {N / t * 1e6:.3g} agent-steps/s", flush=True)
@@ -61,9 +61,9 @@ def main():
             print(f"forward and backward of {M} samples, {bits}-bit activations: {t:.0f} us, peak {torch.cuda.max_memory_allocated() / 1e9:.2f} GB", flush=True)
     for rows in (32, 512, 4096):  # the policy's part of a step, replayed from a graph of 32 as small rollouts are
         for precision in ("float32", "mxfp4"):
-            net._acting = None
+            net._coarse = None
             if precision == "mxfp4":
-                net.use_mxfp4_rollouts()
+                net.use_mxfp4_trunk()
             net.refresh_rollout_heads()
             policy = lambda: net.rollout_step(obs[:rows], logp[:rows], value[:rows], actions[:rows])  # noqa: E731
             us(policy, 3)

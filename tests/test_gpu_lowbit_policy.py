@@ -45,7 +45,7 @@ def test_every_acting_call_computes_the_trunk_in_4_bits(rows):
     net.use_fused_sampling(3)
     with torch.no_grad():
         plain = net.get_prob(x).logits
-    net.use_mxfp4_rollouts()
+    net.use_mxfp4_trunk()
     want = _acting_logits(net, x)
     want = want - np.log(np.exp(want).sum(1, keepdims=True))
     with torch.no_grad():
@@ -58,19 +58,24 @@ def test_every_acting_call_computes_the_trunk_in_4_bits(rows):
         a2 = net.rollout_step(x, lp, v)
         np.testing.assert_allclose(lp.cpu().numpy(), want[np.arange(rows), a2.cpu().numpy()], rtol=0, atol=2e-5)
         torch.testing.assert_close(v, value.squeeze(1), rtol=1e-5, atol=1e-5)
+        assert torch.equal(net.get_value(x), net.get_action_and_value(x)[3])
     assert not torch.equal(got, plain)  # it is another policy
-    # with autograd on, and for the bootstrap value, nothing changes
-    assert torch.equal(net.get_prob(x).logits.detach(), plain)
+    # an update computes the same numbers (the heads in other library calls)
+    logits = net.logits_and_value(x)[0].detach()
+    torch.testing.assert_close(torch.log_softmax(logits, 1), got, rtol=1e-5, atol=1e-5)
+    net.use_activation_checkpoints()
+    logits = net.logits_and_value(x)[0].detach()
+    torch.testing.assert_close(torch.log_softmax(logits, 1), got, rtol=1e-5, atol=1e-5)
 
 
 def test_changed_weights_reach_the_acting_policy():
     net, _ = _agent()
     x = _obs(64, 202)
-    net.use_fused_sampling(3).use_mxfp4_rollouts()
+    net.use_fused_sampling(3).use_mxfp4_trunk()
     lp, v = torch.empty(64, device="cuda"), torch.empty(64, device="cuda")
     net.refresh_rollout_heads()
     net.rollout_step(x, lp, v)
-    held = {k: w.codes.data_ptr() for k, w in net._acting.items()}
+    held = {k: w.codes.data_ptr() for k, w in net._coarse.items()}
     before = v.clone()
     with torch.no_grad():
         for p in net.network.parameters():
@@ -79,7 +84,7 @@ def test_changed_weights_reach_the_acting_policy():
     net.refresh_rollout_heads()
     net.rollout_step(x, lp, v)
     assert not torch.equal(v, before)
-    assert {k: w.codes.data_ptr() for k, w in net._acting.items()} == held  # captured launches read the same places
+    assert {k: w.codes.data_ptr() for k, w in net._coarse.items()} == held  # captured launches read the same places
     np.testing.assert_allclose(expected.double().cpu().numpy(),
                                (lambda l: l - np.log(np.exp(l).sum(1, keepdims=True)))(_acting_logits(net, x)), rtol=0, atol=2e-5)
 
@@ -87,7 +92,7 @@ def test_changed_weights_reach_the_acting_policy():
 def test_a_rollout_step_replayed_from_a_graph_follows_the_refreshed_weights():
     net, _ = _agent()
     x = _obs(32, 202)
-    net.use_fused_sampling(3).use_mxfp4_rollouts()
+    net.use_fused_sampling(3).use_mxfp4_trunk()
     lp, v = torch.empty(32, device="cuda"), torch.empty(32, device="cuda")
     net.refresh_rollout_heads()
     net.rollout_step(x, lp, v)
@@ -112,18 +117,18 @@ def test_a_rollout_step_replayed_from_a_graph_follows_the_refreshed_weights():
 
 def test_asking_twice_leaves_the_weights_where_captured_launches_read_them():
     net, _ = _agent()
-    net.use_fused_sampling(3).use_mxfp4_rollouts()
+    net.use_fused_sampling(3).use_mxfp4_trunk()
     net.refresh_rollout_heads()
-    held = {k: w.codes.data_ptr() for k, w in net._acting.items()}
-    net.use_mxfp4_rollouts()
+    held = {k: w.codes.data_ptr() for k, w in net._coarse.items()}
+    net.use_mxfp4_trunk()
     net.refresh_rollout_heads()
-    assert held and {k: w.codes.data_ptr() for k, w in net._acting.items()} == held
+    assert held and {k: w.codes.data_ptr() for k, w in net._coarse.items()} == held
 
 
 def test_a_copied_policy_acts_with_weights_of_its_own(tmp_path):
     net, _ = _agent()
     x = _obs(64, 202)
-    net.use_mxfp4_rollouts()
+    net.use_mxfp4_trunk()
     with torch.no_grad():
         before = net.get_prob(x).logits.clone()
         twin = copy.deepcopy(net)
@@ -132,7 +137,7 @@ def test_a_copied_policy_acts_with_weights_of_its_own(tmp_path):
             p.mul_(2.0)
         assert not torch.equal(net.get_prob(x).logits, before)
         assert torch.equal(twin.get_prob(x).logits, before)
-        assert twin._acting["network.0"].codes.data_ptr() != net._acting["network.0"].codes.data_ptr()
+        assert twin._coarse["network.0"].codes.data_ptr() != net._coarse["network.0"].codes.data_ptr()
         net.load_state_dict(torch.load(tmp_path / "net.pth", weights_only=True))
         assert torch.equal(net.get_prob(x).logits, before)
 
@@ -140,25 +145,28 @@ def test_a_copied_policy_acts_with_weights_of_its_own(tmp_path):
 def test_acting_without_the_fused_sampler_and_on_any_shape():
     net, _ = _agent(num_envs=16)
     x = _obs(32, 202)
-    net.use_mxfp4_rollouts()
+    net.use_mxfp4_trunk()
     with torch.no_grad():
         own = net.get_action_and_value(x, joint_obs=x.view(1, -1))[3]
         rows = net.get_prob(x).logits
         # the head's library call differs with the shape
         torch.testing.assert_close(net.get_prob(x.view(4, 8, 202)).logits, rows.view(4, 8, 7), rtol=1e-5, atol=1e-5)
         torch.testing.assert_close(net.get_prob(x[5]).logits, rows[5], rtol=1e-5, atol=1e-5)
-        exact = net.get_value(x, joint_obs=x.view(1, -1))
+        assert torch.equal(net.get_value(x, joint_obs=x.view(1, -1)), own)
         net.use_fused_sampling(3)
         fused = net.get_action_and_value(x, joint_obs=x.view(1, -1))[3]
+    net._coarse = None
+    with torch.no_grad():
+        exact = net.get_value(x, joint_obs=x.view(1, -1))
     assert torch.equal(own, fused) and not torch.equal(own, exact)
 
 
 def test_acting_of_a_policy_in_bfloat16():
     net, _ = _agent()
     x = _obs(600, 202)
-    net = net.bfloat16().use_mxfp4_rollouts()
+    net = net.bfloat16().use_mxfp4_trunk()
     with torch.no_grad():
-        hidden = net._acting_trunk(x.bfloat16())
+        hidden = net._trunk(x.bfloat16())
     l0, l1 = net.network[0], net.network[2]
     h = x.double().cpu().numpy()
     for layer in (l0, l1):
@@ -181,7 +189,7 @@ def test_kept_activations_have_no_second_derivative():
 def test_the_centralised_critic_acts_in_4_bits():
     net, _ = _agent(num_envs=16)
     x = _obs(32, 202)
-    net.use_fused_sampling(3).use_mxfp4_rollouts()
+    net.use_fused_sampling(3).use_mxfp4_trunk()
     lp, v = torch.empty(32, device="cuda"), torch.empty(32, device="cuda")
     net.rollout_step(x, lp, v, joint=True)
     c = net.centralised_critics
@@ -249,6 +257,40 @@ def test_gradients_of_the_kept_activations(rows):
         mine = dict(net.named_parameters())[name].grad.double().cpu().numpy()
         close = 4e-6 if name.endswith("bias") or name == "network.0.weight" else 2.0 ** -6
         assert np.linalg.norm(mine - w) <= close * np.linalg.norm(w) + 1e-12, name
+
+
+@pytest.mark.parametrize("rows", [5, 600, 8192])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_gradients_go_straight_through_the_roundings(rows, bits):
+    """forward in 4 bits; backward as if the roundings were not there: masks of the 4-bit outputs, inputs as they were before
+    rounding (or as kept in 8 bits), the float32 weights"""
+    net, _ = _agent(central=False)
+    net.use_mxfp4_trunk()
+    if bits == 8:
+        net.use_activation_checkpoints()
+    x = _obs(rows, 202, rows)
+    d = lambda t: t.detach().double().cpu().numpy()  # noqa: E731
+    w0, w1 = d(net.network[0].weight), d(net.network[2].weight)
+    h = [d(x)]
+    for w in (w0, w1):  # zero biases
+        h.append(np.maximum(ref.mxfp4(h[-1])[2] @ ref.mxfp4(w)[2].T, 0.0).astype(np.float32).astype(np.float64))
+    kept = [ref.act8(h[0], False)[2], ref.act8(h[1], True)[2], ref.act8(h[2], True)[2]] if bits == 8 else h
+    g = torch.randn(rows, 8, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)) / rows
+    gh = d(g)
+    wh = np.concatenate([d(net.actor.weight), d(net.critic.weight)])
+    g1 = (gh @ wh) * (h[2] > 0)
+    g0 = (g1 @ w1) * (h[1] > 0)
+    want = {"heads.weight": gh.T @ kept[2], "heads.bias": gh.sum(0), "network.2.weight": g1.T @ kept[1], "network.2.bias": g1.sum(0),
+            "network.0.weight": g0.T @ kept[0], "network.0.bias": g0.sum(0)}
+    logits, value = net.logits_and_value(x)
+    np.testing.assert_allclose(np.concatenate([d(logits), d(value)], 1), h[2] @ wh.T, rtol=0, atol=2e-5)
+    torch.autograd.backward([logits, value], [g[:, :7], g[:, 7:]])
+    got = {k: p.grad.double().cpu().numpy() for k, p in net.named_parameters()}
+    got["heads.weight"] = np.concatenate([got.pop("actor.weight"), got.pop("critic.weight")])
+    got["heads.bias"] = np.concatenate([got.pop("actor.bias"), got.pop("critic.bias")])
+    for name, w in want.items():
+        # sums in float32, through at most two float32 products of up to 256 terms
+        assert np.linalg.norm(got[name] - w) <= 4e-6 * np.linalg.norm(w) + 1e-12, name
 
 
 def test_a_weight_gradient_against_differences():
@@ -336,12 +378,15 @@ def test_updates_with_kept_activations_follow_the_float32_ones(name, fused):
         assert (after[8][k] - d).norm() <= 2.0 ** -6 * d.norm() + 1e-9, k
 
 
-def test_captured_updates_equal_eager_ones():
+@pytest.mark.parametrize("bits,trunk", [(8, "float32"), (8, "mxfp4"), (32, "mxfp4")])
+def test_captured_updates_equal_eager_ones(bits, trunk):
     from marl_amd.agents import MAPPO
 
     got = []
     for graph in (False, True):
-        learner, net = _learner(MAPPO, 8, graph)
+        learner, net = _learner(MAPPO, bits, graph)
+        if trunk == "mxfp4":
+            net.use_mxfp4_trunk()
         torch.manual_seed(11)
         for k in range(3):  # the first update runs eagerly, the others replay
             learner.update(_obs(16, 202, 9 + k))
@@ -360,7 +405,7 @@ def test_training_and_playing_in_low_bits(tmp_path, algorithm, extra):
     returns, freq = train.main(["--num-agents", str(A), "--num-envs", str(E), "--layout", "overcooked_cramped_room_v0", "--num-steps", str(T),
                                 "--total-steps", str(E * A * T * 4), "--ppo-epoch", "2", "--algorithm", algorithm, "--max-steps", "50",
                                 "--data-path", str(tmp_path / "d"), "--seed", "3", "--save", "--save-path", str(tmp_path / "m"),
-                                "--rollout-precision", "mxfp4", "--activation-bits", "8"] + extra)
+                                "--trunk-precision", "mxfp4", "--activation-bits", "8"] + extra)
     assert len(returns) == 2 and np.isfinite(returns).all()
     path = next((tmp_path / "m").iterdir())
     sd = torch.load(path, map_location="cpu", weights_only=True)

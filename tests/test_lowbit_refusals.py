@@ -122,8 +122,8 @@ def test_python_calls_refuse_host_tensors():
 def test_the_command_refuses_what_does_not_fit():
     from marl_amd import train
 
-    with pytest.raises(SystemExit, match="--sampler fused"):
-        train.main(["--rollout-precision", "mxfp4", "--sampler", "torch"])
+    with pytest.raises(SystemExit):
+        train.main(["--trunk-precision", "int4"])
     with pytest.raises(SystemExit):
         train.main(["--activation-bits", "16"])
 
@@ -138,7 +138,7 @@ def test_policy_options_leave_the_host_path_alone():
     x = torch.randn(6, 20)
     with torch.no_grad():
         want = net.get_prob(x).logits
-    net.use_mxfp4_rollouts().use_activation_checkpoints()
+    net.use_mxfp4_trunk().use_activation_checkpoints()
     with torch.no_grad():
         assert torch.equal(net.get_prob(x).logits, want)
     logits, value = net.logits_and_value(x)
