@@ -269,7 +269,7 @@ enum {
 };
 
 /*
- * 4-bit microscaled floating point (MXFP4) for the layers of an acting policy (no counterpart in the
+ * 4-bit microscaled floating point (MXFP4) for the layers of the policy (no counterpart in the
  * reference, whose model.py:13-27 computes them in float32).
  *
  * A row of num_cols values is cut into blocks of 32, B = ceil(num_cols / 32) of them, the last one

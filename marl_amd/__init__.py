@@ -9,7 +9,7 @@ Public surface (mirrors the reference's modules for this path):
   marl_amd.mxfp4          quantize, linear (policy layers in 4-bit floating point, HIP kernels)
   marl_amd.act8           compress, weight_grad (activations kept in 8 bits for the backward pass, HIP kernels)
   marl_amd.rollout_buffer Buffer
-  marl_amd.policy         Agent (actor-critic MLP, PyTorch-ROCm; its trunk acts in 4 bits and keeps 8-bit activations on request)
+  marl_amd.policy         Agent (actor-critic MLP, PyTorch-ROCm; its trunk in 4 bits and with 8-bit activations on request)
   marl_amd.agents         MAPPO, CMAPPO
   marl_amd.rollout        agent_environment_loop
   marl_amd.train          command-line entry point

@@ -1,9 +1,9 @@
-"""4-bit microscaled floating point for the layers of an acting policy (libmarl_amd.so `marl_mx_*`).
+"""4-bit microscaled floating point for the layers of the policy (libmarl_amd.so `marl_mx_*`).
 
 Blocks of 32 values along a row share a power-of-two scale; a value is one of 0, .5, 1, 1.5, 2, 3, 4, 6 or their
 negatives times it.  `linear` computes a layer with both operands in that form and sums in float32: the reference's
-layers (model.py:13-27) at an eighth of the weight bytes, and on the matrix cores' 4-bit rate.  Inference only: nothing
-here has a gradient.  (The whole numbers of the two-agent observations, -3 to 4, come through unchanged.)
+layers (model.py:13-27) at an eighth of the weight bytes, and on the matrix cores' 4-bit rate.  Nothing here has a
+gradient of its own; an update of the policy passes them straight through the roundings (policy.py).  (The whole numbers of the two-agent observations, -3 to 4, come through unchanged.)
 """
 from __future__ import annotations
 

@@ -47,8 +47,8 @@ def main():
     for M in (2048, 131072, 1048576):
         x = obs.repeat(-(-M // N), 1)[:M].contiguous()
         g = torch.randn(M, 8, device=dev) / M
-        for bits in (32, 8):
-            net._keep_in_8_bits = bits == 8
+        for trunk, bits in (("float32", 32), ("float32", 8), ("mxfp4", 8)):
+            net._keep_in_8_bits, net._coarse = bits == 8, {} if trunk == "mxfp4" else None
 
             def update():
                 net.zero_grad(set_to_none=True)
@@ -58,7 +58,7 @@ def main():
             torch.cuda.empty_cache()
             torch.cuda.reset_peak_memory_stats()
             t = us(update, 10)
-            print(f"forward and backward of {M} samples, {bits}-bit activations: {t:.0f} us, peak {torch.cuda.max_memory_allocated() / 1e9:.2f} GB", flush=True)
+            print(f"forward and backward of {M} samples, {trunk} trunk, {bits}-bit activations: {t:.0f} us, peak {torch.cuda.max_memory_allocated() / 1e9:.2f} GB", flush=True)
     for rows in (32, 512, 4096):  # the policy's part of a step, replayed from a graph of 32 as small rollouts are
         for precision in ("float32", "mxfp4"):
             net._coarse = None
@@ -75,8 +75,8 @@ def main():
     for M in (512, 2048, 16384, 65536):  # as updates of up to 65,536 samples run
         x = obs[:M].contiguous()
         g = torch.randn(M, 8, device=dev) / M
-        for bits in (32, 8):
-            net._keep_in_8_bits = bits == 8
+        for trunk, bits in (("float32", 32), ("float32", 8), ("mxfp4", 8)):
+            net._keep_in_8_bits, net._coarse = bits == 8, {} if trunk == "mxfp4" else None
 
             def captured():
                 net.zero_grad(set_to_none=False)
@@ -92,7 +92,7 @@ def main():
             graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(graph):
                 captured()
-            print(f"forward and backward of {M} samples in a graph, {bits}-bit activations: {us(graph.replay, 50):.0f} us", flush=True)
+            print(f"forward and backward of {M} samples in a graph, {trunk} trunk, {bits}-bit activations: {us(graph.replay, 50):.0f} us", flush=True)
             del graph
 
 
