@@ -520,14 +520,16 @@ act_join_kernel(const float* __restrict__ part_w, const float* __restrict__ part
 //   out <= 16: tiles of 16 x 256 on two workgroups a compute unit; a split has at least 4 steps, where there are few rows 2
 //     (65000 x 8 x 256: 15.6, with 8 steps 17.9, 2 steps 19.7; 2048 x 8 x 256: 7.6, with 8 steps 17.6)
 //   otherwise tiles of 128 x 256 on one workgroup a compute unit where there is work for them with 4 steps a split (8192 x 512 x
-//     202: 24.5, with small tiles 28.5), else 64 x 64 on two with 4 steps (2048 x 512 x 202: 14.5; 2 steps 18.5, 8 steps 15.8)
+//     202: 24.5, with small tiles 28.5), else 64 x 64 on two with 4 steps (2048 x 512 x 202: 14.5; 2 steps 18.5, 8 steps 15.8),
+//     and for inputs that one of those covers, with which neither operand is read twice (131072 x 512 x 40: 123 and 132, without a
+//     mask x 64: 81 and 107; with two of them it is slower, x 96: 186 and 134)
 struct ActCut { int bo, bi, splits; int64_t grid; };
 static ActCut act_cut(int64_t rows, int out, int cols) {
     ActCut c;
     const int64_t steps = (rows + WG_STEP - 1) / WG_STEP;
     const auto tiles = [&](int bo, int bi) { return (int64_t)((out + bo - 1) / bo) * ((cols + bi - 1) / bi); };
     if (out <= 16 || cols < 4) { c.bo = 16; c.bi = 256; }
-    else if (tiles(128, 256) * (steps / 4) >= 256) { c.bo = 128; c.bi = 256; }
+    else if (cols > 64 && tiles(128, 256) * (steps / 4) >= 256) { c.bo = 128; c.bi = 256; }
     else { c.bo = 64; c.bi = 64; }
     const int64_t t = tiles(c.bo, c.bi);
     int64_t s = (c.bo == 128 ? 256 : 512) / t;
