@@ -170,9 +170,9 @@ def _small_gemm_form(x, weight, bias, relu):
     return form
 
 
-def _forward(x, weight, bias, relu, coarse):
+def _forward(x, weight, bias, relu, coarse, out_dtype):
     if coarse is not None:
-        return mxfp4.linear(x, coarse, bias.float(), relu=relu, out_dtype=weight.dtype)
+        return mxfp4.linear(x, coarse, bias.float(), relu=relu, out_dtype=out_dtype or weight.dtype)
     return _FORMS[_small_gemm_form(x, weight, bias, relu)](x, weight, bias, relu)
 
 
@@ -180,13 +180,13 @@ class _LinearReLU(torch.autograd.Function):
     """relu(x @ W^T + b) (or without the ReLU): one GEMM with a fused epilogue, or for the small
     batches where that call is slow a plain product plus in-place bias and ReLU; the backward
     pass forms the weight gradient with `_weight_grad`.  With `coarse`, the weight in 4 bits, the forward pass is
-    `mxfp4.linear`'s and the gradients go straight through its roundings."""
+    `mxfp4.linear`'s, its result in `out_dtype`, and the gradients go straight through its roundings."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, relu, coarse=None):
-        out = _forward(x, weight, bias, relu, coarse)
+    def forward(ctx, x, weight, bias, relu, coarse=None, out_dtype=None):
+        out = _forward(x, weight, bias, relu, coarse, out_dtype)
         ctx.relu = relu
-        ctx.save_for_backward(x, weight, out if relu else None)
+        ctx.save_for_backward(x.to(weight.dtype), weight, out if relu else None)
         return out
 
     @staticmethod
@@ -194,9 +194,9 @@ class _LinearReLU(torch.autograd.Function):
         x, weight, out = ctx.saved_tensors
         if ctx.relu:
             gy = torch.ops.aten.threshold_backward(gy, out, 0)
-        gy = gy.contiguous()
+        gy = gy.contiguous().to(weight.dtype)
         gx = gy @ weight if ctx.needs_input_grad[0] else None
-        return gx, _weight_grad(gy, x), gy.sum(0), None, None
+        return gx, _weight_grad(gy, x), gy.sum(0), None, None, None
 
 
 class _KeptLinear(torch.autograd.Function):
@@ -206,8 +206,8 @@ class _KeptLinear(torch.autograd.Function):
     kept output's and exact; the forward pass and the gradient of the input are those of `_LinearReLU`."""
 
     @staticmethod
-    def forward(ctx, x, codes, scales, nonnegative, weight, bias, relu, coarse=None):
-        out = _forward(x, weight, bias, relu, coarse)
+    def forward(ctx, x, codes, scales, nonnegative, weight, bias, relu, coarse=None, out_dtype=None):
+        out = _forward(x, weight, bias, relu, coarse, out_dtype)
         kept = act8.compress(out, nonnegative=True) if relu else None
         ctx.nonnegative = nonnegative
         ctx.save_for_backward(codes, scales, weight, kept.codes if relu else None, kept.scales if relu else None)
@@ -222,15 +222,15 @@ class _KeptLinear(torch.autograd.Function):
         codes, scales, weight, out_codes, out_scales = ctx.saved_tensors
         mask = None if out_codes is None else act8.Act8(out_codes, out_scales, True)
         gw, gb, masked = act8.weight_grad(gy, act8.Act8(codes, scales, ctx.nonnegative), mask)
-        gx = (gy if mask is None else masked) @ weight if ctx.needs_input_grad[0] else None
-        return gx, None, None, None, gw, gb, None, None
+        gx = (gy if mask is None else masked).to(weight.dtype) @ weight if ctx.needs_input_grad[0] else None
+        return gx, None, None, None, gw, gb, None, None, None
 
 
-def _linear(layer: nn.Linear, x, relu, coarse=None):
+def _linear(layer: nn.Linear, x, relu, coarse=None, out_dtype=None):
     if x.is_cuda and x.dim() == 2:
         if x.shape[0] < _SMALL_ROWS and coarse is None:
             _announce_blas_switch_quietly(x)
-        return _LinearReLU.apply(x.contiguous(), layer.weight, layer.bias, relu, coarse)
+        return _LinearReLU.apply(x.contiguous(), layer.weight, layer.bias, relu, coarse, out_dtype)
     out = layer(x)
     return torch.relu(out) if relu else out
 
@@ -273,8 +273,8 @@ class Agent(nn.Module):
             return _linear(l1, _linear(l0, x, True), True)
         rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
         w0, w1 = self._coarse_weight("network.0", l0, fresh), self._coarse_weight("network.2", l1, fresh)
-        if torch.is_grad_enabled():
-            h = _linear(l1, _linear(l0, rows, True, w0), True, w1)
+        if torch.is_grad_enabled():  # float32 between the layers also in a 16-bit policy: that is what acting quantises
+            h = _linear(l1, _linear(l0, rows, True, w0, torch.float32), True, w1)
         else:  # the same numbers, with what lies between the layers in 4 bits
             h = mxfp4.linear(rows, w0, l0.bias.float(), relu=True, out_dtype="mxfp4")
             h = mxfp4.linear(h, w1, l1.bias.float(), relu=True, out_dtype=l1.weight.dtype)
@@ -317,7 +317,8 @@ class Agent(nn.Module):
         for name in ("network.0", "network.2"):
             layer = self.get_submodule(name)
             coarse = None if self._coarse is None else self._coarse_weight(name, layer, False)
-            h, codes, scales = _KeptLinear.apply(h, codes, scales, nonnegative, layer.weight, layer.bias, True, coarse)
+            between = torch.float32 if name == "network.0" else None  # with 4-bit weights, as in _trunk
+            h, codes, scales = _KeptLinear.apply(h, codes, scales, nonnegative, layer.weight, layer.bias, True, coarse, between)
             nonnegative = True
         heads = _KeptLinear.apply(h, codes, scales, True, torch.cat([self.actor.weight, self.critic.weight]),
                                   torch.cat([self.actor.bias, self.critic.bias]), False)

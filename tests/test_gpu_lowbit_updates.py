@@ -1,0 +1,83 @@
+"""What an update of the low-bit policy computes, keeps and leaves out."""
+import numpy as np
+import pytest
+import torch
+
+import lowbit_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def _agent(seed=5, central=False, num_envs=1, D=202):
+    from marl_amd.policy import Agent
+    from marl_amd.spaces import Box, Discrete
+
+    torch.manual_seed(seed)
+    return Agent(Box(-1, 1, (D,)), Discrete(7), 2, num_envs, build_centralised=central).cuda()
+
+
+def _obs(rows, d=202, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(rows, d, device="cuda", generator=g)
+    return (x.abs() > 0.9).float() * (x * 1.3).round()
+
+
+def _d(t):
+    return t.detach().double().cpu().numpy()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_an_update_computes_the_numbers_that_acted(dtype, bits, monkeypatch):
+    """also where the parameters have 16 bits: the hidden layer is quantised from its float32 sums in both"""
+    from marl_amd import act8
+
+    net = _agent().to(dtype).use_mxfp4_trunk()
+    with torch.no_grad():
+        for layer in (net.network[0], net.network[2]):
+            layer.bias.normal_(0.0, 0.1)
+    x = _obs(1500).to(dtype)
+    with torch.no_grad():
+        acted = net._trunk(x)
+    assert acted.dtype == dtype
+    if bits == 32:
+        h = net._trunk(x)
+        assert h.requires_grad and torch.equal(h, acted)
+        return
+    seen = []
+    compress = act8.compress
+    monkeypatch.setattr(act8, "compress", lambda t, nonnegative=False: (seen.append(t.detach().clone()), compress(t, nonnegative))[1])
+    net.use_activation_checkpoints()
+    net.logits_and_value(x)
+    assert len(seen) == 3 and torch.equal(seen[2], acted)  # the observations, then what each layer of the trunk gave
+
+
+@pytest.mark.parametrize("dtype,step", [(torch.bfloat16, 2.0 ** -8), (torch.float16, 2.0 ** -11)])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_gradients_of_a_16_bit_policy(dtype, step, bits):
+    net = _agent().to(dtype).use_mxfp4_trunk()
+    if bits == 8:
+        net.use_activation_checkpoints()
+    rows = 600
+    x = _obs(rows).to(dtype)
+    w0, w1 = _d(net.network[0].weight), _d(net.network[2].weight)
+    h = [_d(x)]
+    for w in (w0, w1):
+        h.append(np.maximum(ref.mxfp4(h[-1])[2] @ ref.mxfp4(w)[2].T, 0.0).astype(np.float32).astype(np.float64))
+    kept = [ref.act8(h[0], False)[2], ref.act8(h[1], True)[2], ref.act8(h[2], True)[2]] if bits == 8 else h
+    g = torch.randn(rows, 8, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).to(dtype)
+    gh, wh = _d(g), np.concatenate([_d(net.actor.weight), _d(net.critic.weight)])
+    g1 = (gh @ wh) * (h[2] > 0)
+    g0 = (g1 @ w1) * (h[1] > 0)
+    want = {"heads.weight": gh.T @ kept[2], "network.2.weight": g1.T @ kept[1], "network.2.bias": g1.sum(0),
+            "network.0.weight": g0.T @ kept[0], "network.0.bias": g0.sum(0)}
+    logits, value = net.logits_and_value(x)
+    torch.autograd.backward([logits, value], [g[:, :7], g[:, 7:]])
+    assert all(p.grad.dtype == dtype for p in net.parameters())
+    got = {k: _d(p.grad) for k, p in net.named_parameters()}
+    got["heads.weight"] = np.concatenate([got.pop("actor.weight"), got.pop("critic.weight")])
+    for name, w in want.items():
+        # Roundings to the type: of the layer's input, of the gradient behind each layer (the two heads' are rounded before they
+        # are added: two), and of the result.  Each is off by at most half a step and they are independent, so that their sums grow
+        # as the gradient's own do: at most five of them, five half steps of its norm.
+        assert np.linalg.norm(got[name] - w) <= 5 * step * np.linalg.norm(w) + 1e-12, name
