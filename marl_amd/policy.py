@@ -213,6 +213,7 @@ class _KeptLinear(torch.autograd.Function):
         ctx.save_for_backward(codes, scales, weight, kept.codes if relu else None, kept.scales if relu else None)
         if not relu:
             return out
+        ctx.set_materialize_grads(False)  # no zeros as large as the codes in the place of their gradients
         ctx.mark_non_differentiable(kept.codes, kept.scales)
         return out, kept.codes, kept.scales
 
@@ -220,6 +221,8 @@ class _KeptLinear(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, gy, *_kept):
         codes, scales, weight, out_codes, out_scales = ctx.saved_tensors
+        if gy is None:  # what reads the output has no gradient for it
+            return (None,) * 9
         mask = None if out_codes is None else act8.Act8(out_codes, out_scales, True)
         gw, gb, masked = act8.weight_grad(gy, act8.Act8(codes, scales, ctx.nonnegative), mask)
         gx = (gy if mask is None else masked).to(weight.dtype) @ weight if ctx.needs_input_grad[0] else None

@@ -81,3 +81,36 @@ def test_gradients_of_a_16_bit_policy(dtype, step, bits):
         # are added: two), and of the result.  Each is off by at most half a step and they are independent, so that their sums grow
         # as the gradient's own do: at most five of them, five half steps of its norm.
         assert np.linalg.norm(got[name] - w) <= 5 * step * np.linalg.norm(w) + 1e-12, name
+
+
+def test_no_gradients_are_made_up_for_the_codes(monkeypatch):
+    """codes and scales are results of the layer's Function too; autograd has nothing to hand back for them"""
+    from marl_amd import policy
+
+    seen = []
+    backward = policy._KeptLinear.backward
+    monkeypatch.setattr(policy._KeptLinear, "backward", staticmethod(lambda ctx, gy, *kept: (seen.append(kept), backward(ctx, gy, *kept))[1]))
+    net = _agent().use_activation_checkpoints()
+    logits, value = net.logits_and_value(_obs(40))
+    (logits.sum() + value.sum()).backward()
+    assert sorted(len(k) for k in seen) == [0, 2, 2] and all(g is None for k in seen for g in k)
+
+
+def test_an_output_without_a_gradient_of_its_own():
+    from marl_amd import act8, policy
+
+    class Cut(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, t):
+            return t.clone()
+
+        @staticmethod
+        def backward(ctx, g):
+            return None
+
+    net = _agent().use_activation_checkpoints()
+    x, layer = _obs(40), net.network[0]
+    kept = act8.compress(x)
+    out, _, _ = policy._KeptLinear.apply(x, kept.codes, kept.scales, False, layer.weight, layer.bias, True)
+    Cut.apply(out).sum().backward()
+    assert all(p.grad is None or not p.grad.any() for p in layer.parameters())
