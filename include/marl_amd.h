@@ -346,6 +346,13 @@ int marl_act_weight_grad(const void *d_grad, int grad_type, int64_t num_rows, in
                          float *d_grad_bias, void *d_workspace, void *stream);
 size_t marl_act_weight_grad_workspace_bytes(int64_t num_rows, int num_out, int num_cols);
 
+/* The parameter gradients alone, for a layer whose input needs no gradient: the bits of
+ * marl_act_weight_grad, with the same workspace, and no cut gradient written. */
+int marl_act_param_grad(const void *d_grad, int grad_type, int64_t num_rows, int num_out,
+                        const uint8_t *d_codes, const uint8_t *d_scales, int num_cols, int nonnegative,
+                        const uint8_t *d_mask_codes, float *d_grad_weight, float *d_grad_bias,
+                        void *d_workspace, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -53,11 +53,11 @@ def compress(x, nonnegative=False):
     return out
 
 
-def weight_grad(grad, act, mask=None):
+def weight_grad(grad, act, mask=None, want_masked=True):
     """Gradients of a linear layer y = x W^T + b, or relu of that, from the gradient of y ([rows, out], float32, bfloat16 or
     float16) and the kept x (`act`).  `mask`: y as it was kept (nonnegative) where a ReLU stood behind the layer.
     Returns (grad_weight float32 [out, cols], grad_bias float32 [out], the gradient behind the ReLU in grad's type, or None
-    without a mask)."""
+    without a mask or with `want_masked` False: a layer whose input needs no gradient has no use for it)."""
     grad, rows, out, stride = _rows(grad, "grad")
     if stride != out:
         grad = grad.contiguous()
@@ -67,7 +67,7 @@ def weight_grad(grad, act, mask=None):
     if mask is not None and (not isinstance(mask, Act8) or not mask.nonnegative or mask.shape != grad.shape or mask.device != device):
         raise ValueError("mask must be a nonnegative Act8 of grad's shape, on its device")
     cols = act.shape[1]
-    masked = torch.empty_like(grad) if mask is not None else None
+    masked = torch.empty_like(grad) if mask is not None and want_masked else None
     if rows == 0:
         return torch.zeros((out, cols), device=device), torch.zeros(out, device=device), masked
     gw = torch.empty(out, cols, dtype=torch.float32, device=device)
@@ -75,7 +75,12 @@ def weight_grad(grad, act, mask=None):
     L = _lib.lib()
     need = L.marl_act_weight_grad_workspace_bytes(rows, out, cols)
     work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    mask_codes = None if mask is None else mask.codes.data_ptr()
+    if mask is not None and not want_masked:
+        _lib.call(L.marl_act_param_grad, "marl_act_param_grad", device, grad.data_ptr(), _TYPES[grad.dtype], rows, out,
+                  act.codes.data_ptr(), act.scales.data_ptr(), cols, 1 if act.nonnegative else 0, mask_codes, gw.data_ptr(), gb.data_ptr(), _p(work))
+        return gw, gb, None
     _lib.call(L.marl_act_weight_grad, "marl_act_weight_grad", device, grad.data_ptr(), _TYPES[grad.dtype], rows, out,
               act.codes.data_ptr(), act.scales.data_ptr(), cols, 1 if act.nonnegative else 0,
-              mask.codes.data_ptr() if mask is not None else None, _p(masked), gw.data_ptr(), gb.data_ptr(), _p(work))
+              mask_codes, _p(masked), gw.data_ptr(), gb.data_ptr(), _p(work))
     return gw, gb, masked

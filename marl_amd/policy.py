@@ -224,7 +224,7 @@ class _KeptLinear(torch.autograd.Function):
         if gy is None:  # what reads the output has no gradient for it
             return (None,) * 9
         mask = None if out_codes is None else act8.Act8(out_codes, out_scales, True)
-        gw, gb, masked = act8.weight_grad(gy, act8.Act8(codes, scales, ctx.nonnegative), mask)
+        gw, gb, masked = act8.weight_grad(gy, act8.Act8(codes, scales, ctx.nonnegative), mask, want_masked=ctx.needs_input_grad[0])
         gx = (gy if mask is None else masked).to(weight.dtype) @ weight if ctx.needs_input_grad[0] else None
         return gx, None, None, None, gw, gb, None, None, None
 

@@ -114,3 +114,63 @@ def test_an_output_without_a_gradient_of_its_own():
     out, _, _ = policy._KeptLinear.apply(x, kept.codes, kept.scales, False, layer.weight, layer.bias, True)
     Cut.apply(out).sum().backward()
     assert all(p.grad is None or not p.grad.any() for p in layer.parameters())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,out,cols", [(1, 3, 5), (130, 16, 40), (2048, 512, 202), (9001, 300, 520), (5000, 100, 1)])
+def test_parameter_gradients_without_the_cut_gradient(rows, out, cols, dtype):
+    """the same bits; and nothing but the two results and the workspace is written"""
+    from marl_amd import _lib, act8
+    from marl_amd.mxfp4 import _TYPES, _p
+
+    g = torch.Generator(device="cuda").manual_seed(rows + out)
+    rand = lambda *shape: torch.randn(*shape, device="cuda", generator=g)  # noqa: E731
+    act = act8.compress(rand(rows, cols))
+    mask = act8.compress(torch.relu(rand(rows, out)), nonnegative=True)
+    grad = rand(rows, out).to(dtype)
+    grad[mask.codes == 0] = float("nan")  # what is cut does not count
+    gw, gb, masked = act8.weight_grad(grad, act, mask)
+    gw2, gb2, none = act8.weight_grad(grad, act, mask, want_masked=False)
+    assert none is None and torch.isfinite(gw).all() and torch.equal(gw, gw2) and torch.equal(gb, gb2)
+    assert all(torch.equal(a, b) for a, b in zip(act8.weight_grad(masked, act)[:2], act8.weight_grad(masked, act, want_masked=False)[:2]))
+    L = _lib.lib()
+    need = L.marl_act_weight_grad_workspace_bytes(rows, out, cols)
+    bufs = [torch.full((n + 128,), 7.0, device="cuda") for n in (out * cols, out)]
+    work = torch.full((need + 64,), 9, dtype=torch.uint8, device="cuda")
+    before = [t.clone() for t in (grad.view(torch.int32 if dtype == torch.float32 else torch.int16), mask.codes, act.codes)]
+    _lib.check(L.marl_act_param_grad(_p(grad), _TYPES[dtype], rows, out, _p(act.codes), _p(act.scales), cols, 0, _p(mask.codes),
+                                     _p(bufs[0][64:]), _p(bufs[1][64:]), _p(work), torch.cuda.current_stream().cuda_stream), "marl_act_param_grad")
+    for buf, want in zip(bufs, (gw, gb)):
+        assert torch.equal(buf[64:-64], want.flatten()) and (buf[:64] == 7).all() and (buf[-64:] == 7).all()
+    assert (work[need:] == 9).all()
+    after = (grad.view(torch.int32 if dtype == torch.float32 else torch.int16), mask.codes, act.codes)
+    assert all(torch.equal(a, b) for a, b in zip(before, after))
+
+
+def test_an_update_cuts_no_gradient_that_nothing_reads(monkeypatch):
+    """the first layer's input are the observations: the gradient behind its ReLU, 512 values a sample, goes nowhere"""
+    from marl_amd import act8
+
+    wanted = []
+    weight_grad = act8.weight_grad
+    monkeypatch.setattr(act8, "weight_grad", lambda g, a, m=None, **kw: (wanted.append((a.shape[1], kw.get("want_masked", True))), weight_grad(g, a, m, **kw))[1])
+    net = _agent().use_activation_checkpoints()
+    x = _obs(40)
+    logits, value = net.logits_and_value(x)
+    (logits.sum() + value.sum()).backward()
+    assert wanted == [(256, True), (512, True), (202, False)]
+    first = net.network[0].weight.grad.clone()
+    net.zero_grad()
+    wanted.clear()
+    x.requires_grad_()
+    logits, value = net.logits_and_value(x)
+    (logits.sum() + value.sum()).backward()
+    assert wanted == [(256, True), (512, True), (202, True)]
+    assert torch.equal(net.network[0].weight.grad, first)
+    d = lambda t: t.detach().double()  # noqa: E731
+    h0 = torch.relu(torch.addmm(d(net.network[0].bias), d(x), d(net.network[0].weight).t()))
+    h1 = torch.relu(torch.addmm(d(net.network[2].bias), h0, d(net.network[2].weight).t()))
+    g1 = (d(net.actor.weight).sum(0) + d(net.critic.weight).sum(0)) * (h1 > 0)
+    want = ((g1 @ d(net.network[2].weight)) * (h0 > 0)) @ d(net.network[0].weight)
+    # float32 products of up to 512 terms
+    assert (x.grad.double() - want).norm() <= 4e-6 * want.norm()
