@@ -342,8 +342,12 @@ class Agent(nn.Module):
         if self.centralised_critics is None:
             raise RuntimeError("this Agent was built without its centralised critic (build_centralised=False)")
         c = self.centralised_critics
-        coarse = None if self._coarse is None or not joint_obs.is_cuda else self._coarse_weight("centralised_critics.0", c[0], fresh)
-        return _linear(c[4], _linear(c[2], _linear(c[0], joint_obs, True, coarse), True), False)
+        if self._coarse is None or not joint_obs.is_cuda:
+            return _linear(c[4], _linear(c[2], _linear(c[0], joint_obs, True), True), False)
+        rows = joint_obs if joint_obs.dim() == 2 else joint_obs.reshape(-1, joint_obs.shape[-1])
+        coarse = self._coarse_weight("centralised_critics.0", c[0], fresh)
+        value = _linear(c[4], _linear(c[2], _linear(c[0], rows, True, coarse), True), False)
+        return value if joint_obs.dim() == 2 else value.view(*joint_obs.shape[:-1], -1)
 
     def get_value(self, x, joint_obs=None):
         if joint_obs is not None:
