@@ -302,13 +302,23 @@ class Agent(nn.Module):
         self._keep_in_8_bits = True
         return self
 
-    def _coarse_weight(self, name, layer, fresh):
-        """`layer`'s weight in 4 bits, in the same storage every time; quantised anew unless `fresh` says that it is current"""
-        held = self._coarse.get(name)
-        if held is None or held.device != layer.weight.device:
-            held = self._coarse[name] = mxfp4.quantize(layer.weight.detach())
+    def _coarse_weight(self, name, layer, fresh, keep=False):
+        """`layer`'s weight in 4 bits, in the same storage every time; quantised anew unless `fresh` says that it is current.
+        Calls on other streams read the storage too, so it counts as held once its first codes are there.  A launch that is
+        only being captured puts none there: then the weight is the captured call's own, and what needs the storage
+        (`fresh`, `keep`) is refused."""
+        weight, held = layer.weight.detach(), self._coarse.get(name)
+        if held is None or held.device != weight.device:
+            with torch.cuda.device(weight.device):
+                capturing = torch.cuda.is_current_stream_capturing()
+                if capturing and (fresh or keep):
+                    raise RuntimeError("call refresh_rollout_heads() once before a capture that acts in 4 bits")
+                held = mxfp4.quantize(weight)
+                if not capturing:
+                    torch.cuda.current_stream().synchronize()
+                    self._coarse[name] = held
         elif not fresh:
-            mxfp4.quantize(layer.weight.detach(), out=held)
+            mxfp4.quantize(weight, out=held)
         return held
 
     def _kept_heads(self, x):
@@ -394,10 +404,10 @@ class Agent(nn.Module):
             torch.cat([self.actor.weight, self.critic.weight], out=self._head_w)
             torch.cat([self.actor.bias, self.critic.bias], out=self._head_b)
         if self._coarse is not None:  # the 4-bit weights that rollout_step reads
-            self._coarse_weight("network.0", self.network[0], False)
-            self._coarse_weight("network.2", self.network[2], False)
+            self._coarse_weight("network.0", self.network[0], False, keep=True)
+            self._coarse_weight("network.2", self.network[2], False, keep=True)
             if self.centralised_critics is not None and "centralised_critics.0" in self._coarse:
-                self._coarse_weight("centralised_critics.0", self.centralised_critics[0], False)
+                self._coarse_weight("centralised_critics.0", self.centralised_critics[0], False, keep=True)
 
     def rollout_step(self, x, logprob_out, value_out, actions_out=None, slot=None, joint=False, row_offset=0):
         """The rollout half of `get_action_and_value` for the decentralised critic, writing the
@@ -424,6 +434,8 @@ class Agent(nn.Module):
             return actions
         if getattr(self, "_head_w", None) is None:
             self.refresh_rollout_heads()
+            if not torch.cuda.is_current_stream_capturing():
+                torch.cuda.current_stream(x.device).synchronize()  # other streams read them too
         with torch.no_grad():
             heads = torch.addmm(self._head_b, self._trunk(x, fresh=True), self._head_w.t())
             actions, _, _ = self.sampler.sample(heads, want_entropy=False, actions_out=actions_out, logprob_out=logprob_out,
