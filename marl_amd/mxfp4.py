@@ -8,6 +8,7 @@ gradient of its own; an update of the policy passes them straight through the ro
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -20,10 +21,17 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
+def _no_tangent(t, name):
+    """a forward-mode derivative would be lost without a word"""
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name} has a forward-mode derivative, and this call has none to give")
+
+
 def _rows(x, name):
     """a 2-d float tensor on the GPU whose rows are contiguous (they may lie apart): (tensor, rows, cols, row stride)"""
     if not isinstance(x, torch.Tensor) or x.dtype not in _TYPES or x.dim() != 2 or not x.is_cuda:
         raise ValueError(f"{name} must be a float32, bfloat16 or float16 [rows, cols] tensor on the GPU")
+    _no_tangent(x, name)
     rows, cols = x.shape
     if cols >= 1 << 31:  # a C int
         raise ValueError(f"{name} has 2^31 or more columns")
@@ -115,6 +123,8 @@ def linear(x, weight, bias=None, relu=False, out_dtype=torch.float32):
         raise ValueError("weight has no rows, or more than 2^22")
     if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or not bias.is_contiguous() or bias.device != device):
         raise ValueError(f"bias must be a contiguous float32 tensor of {n} entries on the device of x")
+    if bias is not None:
+        _no_tangent(bias, "bias")
     if out_dtype == "mxfp4":
         y = _empty(torch.Size((rows, n)), device)
         y_data, y_scales, y_type = y.codes, y.scales, _MXFP4

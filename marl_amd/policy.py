@@ -307,7 +307,7 @@ class Agent(nn.Module):
         Calls on other streams read the storage too, so it counts as held once its first codes are there.  A launch that is
         only being captured puts none there: then the weight is the captured call's own, and what needs the storage
         (`fresh`, `keep`) is refused."""
-        weight, held = layer.weight.detach(), self._coarse.get(name)
+        weight, held = layer.weight, self._coarse.get(name)
         if held is None or held.device != weight.device:
             with torch.cuda.device(weight.device):
                 capturing = torch.cuda.is_current_stream_capturing()
