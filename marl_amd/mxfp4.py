@@ -3,7 +3,12 @@
 Blocks of 32 values along a row share a power-of-two scale; a value is one of 0, .5, 1, 1.5, 2, 3, 4, 6 or their
 negatives times it.  `linear` computes a layer with both operands in that form and sums in float32: the reference's
 layers (model.py:13-27) at an eighth of the weight bytes, and on the matrix cores' 4-bit rate.  Nothing here has a
-gradient of its own; an update of the policy passes them straight through the roundings (policy.py).  (The whole numbers of the two-agent observations, -3 to 4, come through unchanged.)
+gradient of its own: `linear` refuses tensors that want one, all calls refuse forward-mode derivatives, and what trains
+through them brings its own backward pass (policy.py).
+
+A value is off by at most a quarter of the largest in its block of 32.  Whole numbers come through unchanged in a block
+whose largest is at most 4; beside larger ones small ones are coarser, and beside the timer of a cooking pot in an
+observation (up to 30) they can vanish: 30 reads as 24, 3 as 4 and 1 as 0.
 """
 from __future__ import annotations
 

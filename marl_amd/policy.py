@@ -288,7 +288,8 @@ class Agent(nn.Module):
         first layer of the centralised critic, whose weight is most of what a rollout step reads.  Updates train this policy:
         their forward pass is the same numbers, and the gradients go straight through the roundings to the float32 weights,
         which the optimizer steps and a checkpoint holds.  (Acting in 4 bits and updating in float32 does not train: the
-        two policies differ by more than the PPO clip.)  Heads stay in float32.  `rollout_step` reads the weights as
+        two policies differ by more than the PPO clip.)  Observations are rounded too: distances and flags of up to 4 are kept
+        but where larger numbers, a cooking pot's timer above all, share their block of 32 (`mxfp4`).  Heads stay in float32.  `rollout_step` reads the weights as
         `refresh_rollout_heads` last quantised them; every other call quantises them anew."""
         if self._coarse is None:  # captured launches read the weights where they are
             self._coarse = {}
