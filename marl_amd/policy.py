@@ -180,7 +180,8 @@ class _LinearReLU(torch.autograd.Function):
     """relu(x @ W^T + b) (or without the ReLU): one GEMM with a fused epilogue, or for the small
     batches where that call is slow a plain product plus in-place bias and ReLU; the backward
     pass forms the weight gradient with `_weight_grad`.  With `coarse`, the weight in 4 bits, the forward pass is
-    `mxfp4.linear`'s, its result in `out_dtype`, and the gradients go straight through its roundings."""
+    `mxfp4.linear`'s, its result in `out_dtype`, and the backward pass is the unrounded layer's: its input and weight as they
+    were before they went to 4 bits, the ReLU's mask that of the 4-bit result."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, relu, coarse=None, out_dtype=None):
@@ -286,8 +287,10 @@ class Agent(nn.Module):
     def use_mxfp4_trunk(self):
         """The trunk is computed in 4-bit floating point (`mxfp4.linear`: weights, observations and the hidden layer), and so is the
         first layer of the centralised critic, whose weight is most of what a rollout step reads.  Updates train this policy:
-        their forward pass is the same numbers, and the gradients go straight through the roundings to the float32 weights,
-        which the optimizer steps and a checkpoint holds.  (Acting in 4 bits and updating in float32 does not train: the
+        their forward pass is the same numbers, their backward pass that of the unrounded layers at the ReLU masks of the
+        4-bit ones: g W and g^T x, with W and x as they were before the rounding.  The optimizer steps those weights, and a
+        checkpoint holds them.  (The straight-through gradient proper reads the rounded operands, g Q(W) and g^T Q(x); it
+        trained no better.)  (Acting in 4 bits and updating in float32 does not train: the
         two policies differ by more than the PPO clip.)  Observations are rounded too: distances and flags of up to 4 are kept
         but where larger numbers, a cooking pot's timer above all, share their block of 32 (`mxfp4`).  Heads stay in float32.  `rollout_step` reads the weights as
         `refresh_rollout_heads` last quantised them; every other call quantises them anew."""

@@ -67,7 +67,7 @@ def build_parser():
                    help="decentralised MAPPO on the GPU: loss and head gradients from one HIP pass instead of autograd's small ops")
     p.add_argument("--trunk-precision", choices=["float32", "mxfp4"], default="float32",
                    help="the policy's trunk in float32, or in 4-bit floating point (marl_amd.mxfp4): acting and updates, whose "
-                        "gradients go straight through the roundings to the float32 weights")
+                        "backward pass is that of the unrounded layers and steps the float32 weights")
     p.add_argument("--activation-bits", type=int, choices=[32, 8], default=32,
                    help="what an update keeps of the trunk's activations for its backward pass: float32, or 8 bits a value "
                         "(marl_amd.act8), a quarter of the memory")

@@ -34,3 +34,23 @@ def test_forward_mode_derivatives_are_refused():
         net.network[0].weight = weight
         with torch.no_grad():  # without one, as ever
             assert torch.equal(mxfp4.linear(x, w, b), want) and torch.equal(net.get_value(x), out)
+
+
+def test_the_backward_pass_is_the_unrounded_layers():
+    """g W and g^T x from the operands before they went to 4 bits, not the g Q(W) and g^T Q(x) of a straight-through estimator"""
+    from marl_amd import mxfp4, policy
+
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, w = torch.randn(300, 202, device="cuda", generator=g, requires_grad=True), torch.randn(70, 202, device="cuda", generator=g, requires_grad=True)
+    b = torch.zeros(70, device="cuda", requires_grad=True)
+    out = policy._LinearReLU.apply(x, w, b, True, mxfp4.quantize(w))
+    grad = torch.randn(300, 70, device="cuda", generator=g)
+    out.backward(grad)
+    with torch.no_grad():
+        xq, wq = mxfp4.quantize(x).dequantize().double(), mxfp4.quantize(w).dequantize().double()
+        assert torch.allclose(out.double(), torch.relu(xq @ wq.t()), rtol=0, atol=1e-4)
+        cut = grad.double() * (out > 0)
+        for got, want, rounded in ((x.grad, cut @ w.double(), cut @ wq), (w.grad, cut.t() @ x.double(), cut.t() @ xq)):
+            assert (got.double() - want).norm() <= 4e-6 * want.norm()  # float32 sums of up to 300 terms
+            assert (got.double() - rounded).norm() > 0.01 * want.norm()  # 4 bits are off by more
+        assert (b.grad.double() - cut.sum(0)).norm() <= 4e-6 * cut.sum(0).norm()
