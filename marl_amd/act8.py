@@ -41,8 +41,10 @@ class Act8:
 
 def compress(x, nonnegative=False):
     """x: float32, bfloat16 or float16 [rows, cols] on the GPU (rows may lie apart).  `nonnegative`: x has no negative
-    values (it comes from a ReLU); any there are count as 0.  One step of a block is at most 1/64 (nonnegative: 1/128) of
-    its largest value, so a value is off by at most half that; a positive one that would round to 0 becomes one step."""
+    values (it comes from a ReLU); any there are count as 0.  A block's largest value is at least 63.75 of its steps
+    (nonnegative: 127.75), unless it lies below 2^-120 (2^-119), where a step is 2^-126, and a value is off by at most half a step.  Two are off by up to a
+    step: a positive value that would round to 0 becomes one step (nonnegative), and what lies above 127 (255) steps of the
+    largest scale is cut to them."""
     x, rows, cols, stride = _rows(x, "x")
     out = Act8.__new__(Act8)
     out.codes = torch.empty(rows, cols, dtype=torch.uint8, device=x.device)

@@ -525,8 +525,8 @@ act_join_kernel(const float* __restrict__ part_w, const float* __restrict__ part
 //     (65000 x 8 x 256: 15.6, with 8 steps 17.9, 2 steps 19.7; 2048 x 8 x 256: 7.6, with 8 steps 17.6)
 //   otherwise tiles of 128 x 256 on one workgroup a compute unit where there is work for them with 4 steps a split (8192 x 512 x
 //     202: 24.5, with small tiles 28.5), else 64 x 64 on two with 4 steps (2048 x 512 x 202: 14.5; 2 steps 18.5, 8 steps 15.8),
-//     and for inputs that one of those covers, with which neither operand is read twice (131072 x 512 x 40: 123 and 132, without a
-//     mask x 64: 81 and 107; with two of them it is slower, x 96: 186 and 134)
+//     and for inputs that one of those covers: the gradient is then read once, and x, the smaller operand, once for every 64 outputs
+//     (131072 x 512 x 40: 123 and 132, without a mask x 64: 81 and 107; with two of them it is slower, x 96: 186 and 134)
 struct ActCut { int bo, bi, splits; int64_t grid; };
 static ActCut act_cut(int64_t rows, int out, int cols) {
     ActCut c;

@@ -300,9 +300,10 @@ class Agent(nn.Module):
 
     def use_activation_checkpoints(self):
         """Updates keep the trunk's activations in 8 bits between the forward and the backward pass (`act8`), a quarter of what
-        autograd keeps: an input of whole numbers up to 127 (the observations) exactly, the hidden layers to half a step of
-        a 1/128 of their block's largest value.  Values, log-probabilities and the loss are unchanged; the gradients of
-        the weights are those of the kept activations."""
+        autograd keeps: an input of whole numbers up to 127 (the observations) exactly, the hidden layers to half a step,
+        or one where a small positive value is kept from becoming 0; a step is at most 1/127.75 of their block's largest
+        value.  Values, log-probabilities and the loss are unchanged; the gradients of the weights are those of the kept
+        activations."""
         self._keep_in_8_bits = True
         return self
 

@@ -37,3 +37,29 @@ def test_small_numbers_beside_a_timer(timer, reads, one, three):
     assert ref.mxfp4(x)[2][0, :4].tolist() == [reads, one, three, -one]
     x[0, 0] = 0
     assert np.array_equal(ref.mxfp4(x)[2], x)
+
+
+@pytest.mark.parametrize("positive", [False, True])
+def test_how_far_8_bits_are_off(positive):
+    rng = np.random.default_rng(1)
+    most = 255 if positive else 127
+    x = np.abs(rng.standard_normal((4000, 64))) * np.exp(3 * rng.standard_normal((4000, 64)))
+    if not positive:
+        x *= rng.choice([-1.0, 1.0], x.shape)
+    x[0] = np.linspace(0, most + 0.5, 64)  # the largest value that takes the next scale
+    x[1] = np.linspace(0, np.nextafter(most + 0.5, 0), 64)
+    x[2], x[3] = x[0] * 2.0 ** -133, x[0] * 2.0 ** 110  # the smallest scale, and near the largest
+    x[4] = 3.4028234663852886e38 * np.linspace(0, 1, 64)
+    _, byte, values = ref.act8(x, positive)
+    step = np.exp2(byte.astype(np.float64) - 127)[:, :, None]
+    before, after = ref.blocks(x), ref.blocks(values)
+    top = np.abs(before).max(axis=2, keepdims=True)
+    ordinary = top >= 2.0 ** (-119 if positive else -120)
+    assert (top >= step * ((most + 0.5) / 2))[ordinary].all() and (step[~ordinary] == 2.0 ** -126).all()
+    assert (step > top * 2 / (most + 1))[ordinary].any()  # 1/64 and 1/128 do not hold
+    error = np.abs(after - before) / step
+    raised = (before > 0) & (before < 0.5 * step) if positive else np.zeros(before.shape, bool)
+    cut = (step == 2.0 ** (120 if positive else 121)) & (np.abs(before) > most * step)
+    assert (error[~raised & ~cut] <= 0.5).all() and (error[raised | cut] <= 1.0).all()
+    assert cut.any() and raised.any() == positive
+    assert not positive or np.array_equal(values > 0, x > 0)
