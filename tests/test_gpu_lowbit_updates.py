@@ -174,3 +174,37 @@ def test_an_update_cuts_no_gradient_that_nothing_reads(monkeypatch):
     want = ((g1 @ d(net.network[2].weight)) * (h0 > 0)) @ d(net.network[0].weight)
     # float32 products of up to 512 terms
     assert (x.grad.double() - want).norm() <= 4e-6 * want.norm()
+
+
+def _update_peak(net, rows):
+    """bytes that an update's forward and backward pass add to what was allocated before, at their peak"""
+    x = _obs(rows)
+    g = torch.randn(rows, 8, device="cuda") / rows
+    for _ in range(2):  # the second time gradients and library workspaces are there
+        net.zero_grad(set_to_none=False)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        base = torch.cuda.memory_allocated()
+        logits, value = net.logits_and_value(x)
+        torch.autograd.backward([logits, value], [g[:, :7], g[:, 7:]])
+        torch.cuda.synchronize()
+        peak = torch.cuda.max_memory_allocated() - base
+        del logits, value
+    return peak
+
+
+def test_the_peak_of_an_update():
+    """forward and backward; bytes a sample, of float32 values unless said"""
+    rows = 262144
+    net = _agent()
+    wide = _update_peak(net, rows)
+    net.use_activation_checkpoints()
+    kept = _update_peak(net, rows)
+    # Float32: in the second layer's backward pass there are both hidden layers (512 + 256), the gradient of its output before and
+    # behind the ReLU (256 each) and that of its input (512).
+    assert wide >= rows * (512 + 256 + 256 + 256 + 512) * 4
+    # 8 bits: a byte and 1/32 for every value of both layers and the observations; at the peak, in the same place, the gradient of
+    # the output before and behind the ReLU and that of the input; the heads' results and their gradients (4 x 8 values); and
+    # the splits' sums, at most 256 tiles of 128 x 256.
+    assert kept <= rows * ((202 + 512 + 256) * 34 / 32 + (256 + 256 + 512) * 4 + 4 * 8 * 4) + 256 * 128 * 257 * 4 + (8 << 20)
+    assert kept <= 0.75 * wide
