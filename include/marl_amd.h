@@ -260,7 +260,7 @@ int marl_ppo_loss(const float *d_logits, int num_samples, int num_actions, int r
                   void *stream);
 size_t marl_ppo_loss_workspace_bytes(int num_samples);
 
-/* element types of the low-bit passes */
+/* Element types of the low-bit passes.  What these passes write must not overlap what they read. */
 enum {
     MARL_F32 = 0,
     MARL_BF16 = 1,

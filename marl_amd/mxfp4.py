@@ -57,7 +57,8 @@ def _bytes_on_gpu(t, name):
 
 class MXFP4:
     """A [rows, cols] tensor in 4 bits: `codes` uint8 [rows, 16 * blocks] (two codes a byte, the lower half first) and
-    `scales` uint8 [rows, blocks] (2^(byte - 127); 255: the block reads as NaN), blocks = ceil(cols / 32)."""
+    `scales` uint8 [rows, blocks] (2^(byte - 127); 255: the block reads as NaN), blocks = ceil(cols / 32).  Codes behind the
+    last column are 0, or 8 (minus 0): a product counts them."""
 
     __slots__ = ("codes", "scales", "shape", "device")
 
