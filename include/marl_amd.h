@@ -353,6 +353,13 @@ int marl_act_param_grad(const void *d_grad, int grad_type, int64_t num_rows, int
                         const uint8_t *d_mask_codes, float *d_grad_weight, float *d_grad_bias,
                         void *d_workspace, void *stream);
 
+/* Column sums of x_type [num_rows][num_cols] (the bias gradient of a layer: agents/MAPPO.py:207): d_sums float32 [num_cols].
+ * Sums in float32 by parts that are added in double; the same call gives the same bits every time, also replayed from a graph
+ * (no memory is cleared).  d_workspace: marl_column_sums_workspace_bytes() bytes, 16-byte aligned. */
+int marl_column_sums(const void *d_x, int x_type, int64_t num_rows, int num_cols, float *d_sums,
+                     void *d_workspace, void *stream);
+size_t marl_column_sums_workspace_bytes(int64_t num_rows, int num_cols);
+
 #ifdef __cplusplus
 }
 #endif

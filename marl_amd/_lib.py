@@ -22,7 +22,7 @@ EXPORTS = (
     "marl_ppo_loss", "marl_ppo_loss_workspace_bytes",
     "marl_mx_quantize", "marl_mx_dequantize", "marl_mx_linear", "marl_mx_linear_workspace_bytes",
     "marl_act_compress", "marl_act_dequantize", "marl_act_weight_grad", "marl_act_weight_grad_workspace_bytes",
-    "marl_act_param_grad",
+    "marl_act_param_grad", "marl_column_sums", "marl_column_sums_workspace_bytes",
 )
 
 _lib = None
@@ -115,6 +115,10 @@ def lib() -> ctypes.CDLL:
     L.marl_act_weight_grad.argtypes = [vp, ci, i64, ci, vp, vp, ci, ci, vp, vp, vp, vp, vp, vp]
     L.marl_act_param_grad.restype = ci
     L.marl_act_param_grad.argtypes = [vp, ci, i64, ci, vp, vp, ci, ci, vp, vp, vp, vp, vp]
+    L.marl_column_sums.restype = ci
+    L.marl_column_sums.argtypes = [vp, ci, i64, ci, vp, vp, vp]
+    L.marl_column_sums_workspace_bytes.restype = ctypes.c_size_t
+    L.marl_column_sums_workspace_bytes.argtypes = [i64, ci]
     L.marl_act_weight_grad_workspace_bytes.restype = ctypes.c_size_t
     L.marl_act_weight_grad_workspace_bytes.argtypes = [i64, ci, ci]
     _lib = L

@@ -86,3 +86,19 @@ def weight_grad(grad, act, mask=None, want_masked=True):
               act.codes.data_ptr(), act.scales.data_ptr(), cols, 1 if act.nonnegative else 0,
               mask_codes, _p(masked), gw.data_ptr(), gb.data_ptr(), _p(work))
     return gw, gb, masked
+
+
+def column_sums(x):
+    """x.sum(0) of a float32, bfloat16 or float16 [rows, cols] tensor on the GPU, in float32.  It clears no memory, so a captured
+    graph of it is right in every replay (torch's sum over many rows records a memory-set node, which is not)."""
+    x, rows, cols, stride = _rows(x, "x")
+    if stride != cols:
+        x = x.contiguous()
+    if rows == 0:
+        return torch.zeros(cols, device=x.device)
+    out = torch.empty(cols, dtype=torch.float32, device=x.device)
+    L = _lib.lib()
+    need = L.marl_column_sums_workspace_bytes(rows, cols)
+    work = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    _lib.call(L.marl_column_sums, "marl_column_sums", x.device, x.data_ptr(), _TYPES[x.dtype], rows, cols, out.data_ptr(), _p(work))
+    return out

@@ -20,6 +20,7 @@ import numpy as np
 import torch
 
 from .. import dist_utils
+from ..act8 import column_sums
 from ..gae import compute_gae as _gae_kernel
 
 
@@ -60,6 +61,11 @@ class MAPPO:
         self._fused_loss = bool(fused_loss) and self.device.type == "cuda" \
             and type(self).compute_value_loss is getattr(type(self), "_value_loss_of_fused_pass", None)
         self._mean_target = None
+        # A captured step must not hold memory-set nodes, which do not do their work in every replay; torch's reductions
+        # record one where they split a sum over blocks.  The policy's sums have launches of their own
+        # (`act8.column_sums`), means of up to 65,536 values take one block, and longer ones of the autograd loss are not captured.
+        if not small and not self._fused_loss:
+            self._graph_update = False
         if self._graph_update:
             for group in optimzer.param_groups:  # the step counter must live on the device to be captured
                 group["capturable"] = True
@@ -138,7 +144,9 @@ class MAPPO:
                 # the target of a sample at the sample's index, so only those entries are written)
                 if self._mean_target is None or self._mean_target.shape != b_value_target.shape:
                     self._mean_target = torch.empty_like(b_value_target)
-                self._mean_target.index_copy_(0, mb, b_value_target[mb].mean().expand(mb.numel()))
+                targets = b_value_target[mb]
+                mean = targets.mean() if targets.numel() <= 65536 or not targets.is_cuda else column_sums(targets.view(-1, 1)) / targets.numel()
+                self._mean_target.index_copy_(0, mb, mean.expand(mb.numel()))
                 b_value_target = self._mean_target
             loss, stats = ppo_loss(logits, newvalue, mb, b_actions_f, b_logprobs, b_advantages, b_value_target,
                                    self.clip_param, self.entropy_coef, self.value_loss_coef)

@@ -518,7 +518,68 @@ act_join_kernel(const float* __restrict__ part_w, const float* __restrict__ part
     else gw[at] = (float)all;
 }
 
+// -------------------------------------------------------------------------------------------------------- column sums
+//
+//   sums[c] = sum_m x[m][c], the bias gradient of a layer whose activations were not kept in 8 bits.  (A library's sum that splits a
+//   column over workgroups clears its counters with a memory-set call, and such a node of a captured graph does not do its work in
+//   every replay; nothing here needs clearing.)
+// A thread has four neighbouring columns of every (256 / groups)-th row of its split, sums in float32, a workgroup's threads are added
+// in order in double, the splits by act_join_kernel.  Bound by memory where rows are many.
+
+template <int TYPE>
+__global__ void __launch_bounds__(256)
+column_sums_kernel(const void* __restrict__ x, int64_t rows, int cols, int groups, int splits, float* __restrict__ part) {
+    __shared__ float sums[256][4];
+    const int tid = threadIdx.x, each = 256 / groups, mine = tid / groups;  // groups of columns: a power of two
+    const int c0 = (blockIdx.x * groups + (tid & (groups - 1))) * 4;
+    float acc[4] = {0, 0, 0, 0};
+    if (c0 + 4 <= cols) {
+#pragma unroll 4
+        for (int64_t m = (int64_t)blockIdx.y * each + mine; m < rows; m += (int64_t)splits * each) {
+            float v[4];
+            const int64_t at = m * cols + c0;
+            if constexpr (TYPE == MARL_F32) {
+                const f32x4 u = *reinterpret_cast<const f32x4_a4*>(static_cast<const float*>(x) + at);
+                v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+            } else {
+                typedef u32x2 u32x2_a2 __attribute__((aligned(2)));
+                const u32x2 u = *reinterpret_cast<const u32x2_a2*>(static_cast<const uint16_t*>(x) + at);
+                use_four<TYPE, false>(u32x4{u.x, u.y, 0, 0}, 0, v);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[k] += v[k];
+        }
+    } else if (c0 < cols) {
+        for (int64_t m = (int64_t)blockIdx.y * each + mine; m < rows; m += (int64_t)splits * each)
+#pragma unroll
+            for (int k = 0; k < 3; ++k)
+                if (c0 + k < cols) acc[k] += load_one<TYPE>(x, m * cols + c0 + k);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) sums[tid][k] = acc[k];
+    __syncthreads();
+    for (int q = tid; q < 4 * groups; q += 256) {  // a column of the tile
+        const int c = blockIdx.x * groups * 4 + q;
+        if (c >= cols) continue;
+        double s = 0.0;
+        for (int r = 0; r < each; ++r) s += (double)sums[r * groups + q / 4][q & 3];
+        part[(int64_t)blockIdx.y * cols + c] = (float)s;
+    }
+}
+
 // ------------------------------------------------------------------------------------------------------------ host
+
+// Tiles of up to 256 columns; a thread has at least eight rows, and there are at most 1024 workgroups (131072 x 512: 512 splits).
+struct SumsCut { int groups, tiles, splits; };
+static SumsCut sums_cut(int64_t rows, int cols) {
+    SumsCut c;
+    c.groups = 1;
+    while (c.groups < 64 && c.groups * 4 < cols) c.groups *= 2;
+    c.tiles = (cols + c.groups * 4 - 1) / (c.groups * 4);
+    const int64_t least = 8 * (256 / c.groups), most = (rows + least - 1) / least, s = c.tiles >= 1024 ? 1 : 1024 / c.tiles;
+    c.splits = (int)(s < most ? s : most);
+    return c;
+}
 
 // How a weight gradient is cut: the tile, and into how many splits of the rows.  Measured in us (float32, with a mask):
 //   out <= 16: tiles of 16 x 256 on two workgroups a compute unit; a split has at least 4 steps, where there are few rows 2
@@ -675,4 +736,31 @@ extern "C" int marl_act_param_grad(const void* d_grad, int grad_type, int64_t nu
                                    float* d_grad_weight, float* d_grad_bias, void* d_workspace, void* stream) {
     return weight_grad(false, d_grad, grad_type, num_rows, num_out, d_codes, d_scales, num_cols, nonnegative, d_mask_codes, nullptr,
                        d_grad_weight, d_grad_bias, d_workspace, stream);
+}
+
+extern "C" size_t marl_column_sums_workspace_bytes(int64_t num_rows, int num_cols) {
+    if (num_rows <= 0 || num_cols <= 0) return 0;
+    const SumsCut c = sums_cut(num_rows, num_cols);
+    return c.splits == 1 ? 0 : (size_t)c.splits * num_cols * sizeof(float);
+}
+
+extern "C" int marl_column_sums(const void* d_x, int x_type, int64_t num_rows, int num_cols, float* d_sums, void* d_workspace, void* stream) {
+    if (num_rows <= 0 || num_cols <= 0) return set_error(MARL_ERR_INVALID, "num_rows and num_cols must be positive");
+    if (x_type != MARL_F32 && x_type != MARL_BF16 && x_type != MARL_F16)
+        return set_error(MARL_ERR_INVALID, "x_type must be MARL_F32, MARL_BF16 or MARL_F16");
+    if (!d_x || !d_sums) return set_error(MARL_ERR_INVALID, "NULL argument to marl_column_sums");
+    if (((uintptr_t)d_x & (lb_type_bytes(x_type) - 1)) != 0 || ((uintptr_t)d_sums & 3u) != 0 || ((uintptr_t)d_workspace & 15u) != 0)
+        return set_error(MARL_ERR_INVALID, "d_workspace must be 16-byte aligned, the others aligned to their elements");
+    if (num_rows >= ((int64_t)1 << 40) || num_cols > (1 << 20)) return set_error(MARL_ERR_INVALID, "at most 2^40 rows and 2^20 columns");
+    const SumsCut c = sums_cut(num_rows, num_cols);
+    if (c.splits > 1 && !d_workspace)
+        return set_error(MARL_ERR_INVALID, "this size needs d_workspace (marl_column_sums_workspace_bytes bytes)");
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    float* part = c.splits == 1 ? d_sums : static_cast<float*>(d_workspace);
+    auto kernel = x_type == MARL_F32 ? column_sums_kernel<MARL_F32> : x_type == MARL_BF16 ? column_sums_kernel<MARL_BF16> : column_sums_kernel<MARL_F16>;
+    hipLaunchKernelGGL(kernel, dim3(c.tiles, c.splits), dim3(256), 0, s, d_x, num_rows, num_cols, c.groups, c.splits, part);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || c.splits == 1) return act_hip(e, "column sums launch");
+    hipLaunchKernelGGL(act_join_kernel<16>, dim3((uint32_t)((num_cols + 63) / 64)), dim3(1024), 0, s, part, part, (int64_t)0, num_cols, c.splits, d_sums, d_sums);
+    return act_hip(hipGetLastError(), "column sums join launch");
 }

@@ -42,6 +42,11 @@ def _weight_grad(gy, x):
     return torch.bmm(gy.view(S, K // S, -1).transpose(1, 2), x.view(S, K // S, -1)).sum(0)
 
 
+def _bias_grad(gy):
+    """gy.sum(0), from launches that replay (`act8.column_sums`): updates of small minibatches are captured"""
+    return act8.column_sums(gy).to(gy.dtype) if gy.is_cuda and gy.dtype in act8._TYPES else gy.sum(0)
+
+
 # Below 512 rows (the reference's batch sizes: 16 envs x 2 agents = 32 rows per rollout step)
 # hipBLASLt's pick for the fused call is erratic on MI355X: rows x 512 -> 256 takes 17.8 us at 32
 # rows, 60 us at 128, 118 us at 256 and 6 us at 512, while a plain rocBLAS product takes 3.7 us at
@@ -197,7 +202,7 @@ class _LinearReLU(torch.autograd.Function):
             gy = torch.ops.aten.threshold_backward(gy, out, 0)
         gy = gy.contiguous().to(weight.dtype)
         gx = gy @ weight if ctx.needs_input_grad[0] else None
-        return gx, _weight_grad(gy, x), gy.sum(0), None, None, None
+        return gx, _weight_grad(gy, x), _bias_grad(gy), None, None, None
 
 
 class _KeptLinear(torch.autograd.Function):
