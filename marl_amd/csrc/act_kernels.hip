@@ -530,7 +530,8 @@ template <int TYPE>
 __global__ void __launch_bounds__(256)
 column_sums_kernel(const void* __restrict__ x, int64_t rows, int cols, int groups, int splits, float* __restrict__ part) {
     __shared__ float sums[256][4];
-    const int tid = threadIdx.x, each = 256 / groups, mine = tid / groups;  // groups of columns: a power of two
+    __shared__ double fours[256];
+    const int tid = threadIdx.x, each = 256 / groups, mine = tid / groups;  // groups of columns: a power of two up to 64
     const int c0 = (blockIdx.x * groups + (tid & (groups - 1))) * 4;
     float acc[4] = {0, 0, 0, 0};
     if (c0 + 4 <= cols) {
@@ -550,6 +551,7 @@ column_sums_kernel(const void* __restrict__ x, int64_t rows, int cols, int group
             for (int k = 0; k < 4; ++k) acc[k] += v[k];
         }
     } else if (c0 < cols) {
+#pragma unroll 4
         for (int64_t m = (int64_t)blockIdx.y * each + mine; m < rows; m += (int64_t)splits * each)
 #pragma unroll
             for (int k = 0; k < 3; ++k)
@@ -558,25 +560,30 @@ column_sums_kernel(const void* __restrict__ x, int64_t rows, int cols, int group
 #pragma unroll
     for (int k = 0; k < 4; ++k) sums[tid][k] = acc[k];
     __syncthreads();
-    for (int q = tid; q < 4 * groups; q += 256) {  // a column of the tile
-        const int c = blockIdx.x * groups * 4 + q;
-        if (c >= cols) continue;
-        double s = 0.0;
-        for (int r = 0; r < each; ++r) s += (double)sums[r * groups + q / 4][q & 3];
-        part[(int64_t)blockIdx.y * cols + c] = (float)s;
-    }
+    const int wide = 4 * groups, q = tid & (wide - 1), c = blockIdx.x * wide + q;  // a column of the tile, four rows of it to a thread
+    double s = 0.0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s += (double)sums[(tid / wide * 4 + k) * groups + q / 4][q & 3];
+    fours[tid] = s;
+    __syncthreads();
+    if (tid >= wide || c >= cols) return;
+    s = 0.0;
+#pragma unroll 8
+    for (int r = 0; r < 256; r += wide) s += fours[r + q];
+    part[(int64_t)blockIdx.y * cols + c] = (float)s;
 }
 
 // ------------------------------------------------------------------------------------------------------------ host
 
-// Tiles of up to 256 columns; a thread has at least eight rows, and there are at most 1024 workgroups (131072 x 512: 512 splits).
+// Tiles of up to 256 columns; a thread has at least eight rows, or up to 32 where that saves the second launch, and there are at most
+// 1024 workgroups (131072 x 512: 512 splits).
 struct SumsCut { int groups, tiles, splits; };
 static SumsCut sums_cut(int64_t rows, int cols) {
     SumsCut c;
     c.groups = 1;
     while (c.groups < 64 && c.groups * 4 < cols) c.groups *= 2;
     c.tiles = (cols + c.groups * 4 - 1) / (c.groups * 4);
-    const int64_t least = 8 * (256 / c.groups), most = (rows + least - 1) / least, s = c.tiles >= 1024 ? 1 : 1024 / c.tiles;
+    const int64_t least = 8 * (256 / c.groups), most = rows <= 4 * least ? 1 : (rows + least - 1) / least, s = c.tiles >= 1024 ? 1 : 1024 / c.tiles;
     c.splits = (int)(s < most ? s : most);
     return c;
 }
