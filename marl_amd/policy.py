@@ -186,37 +186,51 @@ class _LinearReLU(torch.autograd.Function):
     batches where that call is slow a plain product plus in-place bias and ReLU; the backward
     pass forms the weight gradient with `_weight_grad`.  With `coarse`, the weight in 4 bits, the forward pass is
     `mxfp4.linear`'s, its result in `out_dtype`, and the backward pass is the unrounded layer's: its input and weight as they
-    were before they went to 4 bits, the ReLU's mask that of the 4-bit result."""
+    were before they went to 4 bits, the ReLU's mask that of the 4-bit result.  With `straight` it is the 4-bit layer's with
+    the roundings' derivatives taken as one: it reads input and weight as the product did, and keeps the input in 4 bits."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, relu, coarse=None, out_dtype=None):
-        out = _forward(x, weight, bias, relu, coarse, out_dtype)
-        ctx.relu = relu
-        ctx.save_for_backward(x.to(weight.dtype), weight, out if relu else None)
+    def forward(ctx, x, weight, bias, relu, coarse=None, out_dtype=None, straight=False):
+        ctx.relu, ctx.cols, ctx.dtype = relu, x.shape[1] if straight else None, weight.dtype
+        if straight:
+            kept = mxfp4.quantize(x)
+            out = _forward(kept, weight, bias, relu, coarse, out_dtype)
+            back = coarse.dequantize(weight.dtype) if ctx.needs_input_grad[0] else None
+            ctx.save_for_backward(kept.codes, kept.scales, back, out if relu else None)
+        else:
+            out = _forward(x, weight, bias, relu, coarse, out_dtype)
+            ctx.save_for_backward(x.to(weight.dtype), weight, out if relu else None)
         return out
 
     @staticmethod
     def backward(ctx, gy):
-        x, weight, out = ctx.saved_tensors
+        if ctx.cols is None:
+            x, weight, out = ctx.saved_tensors
+        else:
+            codes, scales, weight, out = ctx.saved_tensors
+            x = mxfp4.MXFP4(codes, scales, ctx.cols).dequantize(ctx.dtype)
         if ctx.relu:
             gy = torch.ops.aten.threshold_backward(gy, out, 0)
-        gy = gy.contiguous().to(weight.dtype)
+        gy = gy.contiguous().to(ctx.dtype)
         gx = gy @ weight if ctx.needs_input_grad[0] else None
-        return gx, _weight_grad(gy, x), _bias_grad(gy), None, None, None
+        return gx, _weight_grad(gy, x), _bias_grad(gy), None, None, None, None
 
 
 class _KeptLinear(torch.autograd.Function):
     """`_LinearReLU` that keeps its input, and behind a ReLU its output, in 8 bits for the backward pass instead of in
     float32.  The input comes with its kept form (codes, scales, whether nonnegative); the output's goes on to the next layer, so that
     what lies between two layers is kept once.  The gradient of the weight is formed from the kept input, the ReLU's mask is the
-    kept output's and exact; the forward pass and the gradient of the input are those of `_LinearReLU`."""
+    kept output's and exact; the forward pass and the gradient of the input are those of `_LinearReLU`.  With `straight` the kept
+    input is x in 4 bits (codes and scales of an MXFP4, whose values 8 bits hold exactly)."""
 
     @staticmethod
-    def forward(ctx, x, codes, scales, nonnegative, weight, bias, relu, coarse=None, out_dtype=None):
-        out = _forward(x, weight, bias, relu, coarse, out_dtype)
+    def forward(ctx, x, codes, scales, nonnegative, weight, bias, relu, coarse=None, out_dtype=None, straight=False):
+        ctx.cols = x.shape[1] if straight else None
+        out = _forward(mxfp4.MXFP4(codes, scales, ctx.cols) if straight else x, weight, bias, relu, coarse, out_dtype)
         kept = act8.compress(out, nonnegative=True) if relu else None
-        ctx.nonnegative = nonnegative
-        ctx.save_for_backward(codes, scales, weight, kept.codes if relu else None, kept.scales if relu else None)
+        ctx.nonnegative, ctx.dtype = nonnegative, weight.dtype
+        back = weight if not straight else coarse.dequantize(weight.dtype) if ctx.needs_input_grad[0] else None
+        ctx.save_for_backward(codes, scales, back, kept.codes if relu else None, kept.scales if relu else None)
         if not relu:
             return out
         ctx.set_materialize_grads(False)  # no zeros as large as the codes in the place of their gradients
@@ -228,18 +242,22 @@ class _KeptLinear(torch.autograd.Function):
     def backward(ctx, gy, *_kept):
         codes, scales, weight, out_codes, out_scales = ctx.saved_tensors
         if gy is None:  # what reads the output has no gradient for it
-            return (None,) * 9
+            return (None,) * 10
         mask = None if out_codes is None else act8.Act8(out_codes, out_scales, True)
-        gw, gb, masked = act8.weight_grad(gy, act8.Act8(codes, scales, ctx.nonnegative), mask, want_masked=ctx.needs_input_grad[0])
-        gx = (gy if mask is None else masked).to(weight.dtype) @ weight if ctx.needs_input_grad[0] else None
-        return gx, None, None, None, gw, gb, None, None, None
+        if ctx.cols is None:
+            x = act8.Act8(codes, scales, ctx.nonnegative)
+        else:
+            x = act8.compress(mxfp4.MXFP4(codes, scales, ctx.cols).dequantize(), ctx.nonnegative)
+        gw, gb, masked = act8.weight_grad(gy, x, mask, want_masked=ctx.needs_input_grad[0])
+        gx = (gy if mask is None else masked).to(ctx.dtype) @ weight if ctx.needs_input_grad[0] else None
+        return gx, None, None, None, gw, gb, None, None, None, None
 
 
-def _linear(layer: nn.Linear, x, relu, coarse=None, out_dtype=None):
+def _linear(layer: nn.Linear, x, relu, coarse=None, out_dtype=None, straight=False):
     if x.is_cuda and x.dim() == 2:
         if x.shape[0] < _SMALL_ROWS and coarse is None:
             _announce_blas_switch_quietly(x)
-        return _LinearReLU.apply(x.contiguous(), layer.weight, layer.bias, relu, coarse, out_dtype)
+        return _LinearReLU.apply(x.contiguous(), layer.weight, layer.bias, relu, coarse, out_dtype, straight)
     out = layer(x)
     return torch.relu(out) if relu else out
 
@@ -269,6 +287,7 @@ class Agent(nn.Module):
         self.sampler = None  # set by use_fused_sampling(); plain torch.distributions otherwise
         self._head_w = self._head_b = None  # stacked heads of rollout_step
         self._coarse = None  # 4-bit weights of the trunk, set by use_mxfp4_trunk()
+        self._straight = False  # the 4-bit trunk's backward pass, set by use_mxfp4_trunk()
         self._keep_in_8_bits = False  # set by use_activation_checkpoints()
         self.centralised_critics = (_mlp([d * self.num_agents * self.num_envs, 512, 256, 1], final_activation=False)
                                     if build_centralised else None)
@@ -283,24 +302,31 @@ class Agent(nn.Module):
         rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
         w0, w1 = self._coarse_weight("network.0", l0, fresh), self._coarse_weight("network.2", l1, fresh)
         if torch.is_grad_enabled():  # float32 between the layers also in a 16-bit policy: that is what acting quantises
-            h = _linear(l1, _linear(l0, rows, True, w0, torch.float32), True, w1)
+            h = _linear(l1, _linear(l0, rows, True, w0, torch.float32, self._straight), True, w1, None, self._straight)
         else:  # the same numbers, with what lies between the layers in 4 bits
             h = mxfp4.linear(rows, w0, l0.bias.float(), relu=True, out_dtype="mxfp4")
             h = mxfp4.linear(h, w1, l1.bias.float(), relu=True, out_dtype=l1.weight.dtype)
         return h if x.dim() == 2 else h.view(*x.shape[:-1], -1)
 
-    def use_mxfp4_trunk(self):
+    def use_mxfp4_trunk(self, straight_through=False):
         """The trunk is computed in 4-bit floating point (`mxfp4.linear`: weights, observations and the hidden layer), and so is the
-        first layer of the centralised critic, whose weight is most of what a rollout step reads.  Updates train this policy:
-        their forward pass is the same numbers, their backward pass that of the unrounded layers at the ReLU masks of the
-        4-bit ones: g W and g^T x, with W and x as they were before the rounding.  The optimizer steps those weights, and a
-        checkpoint holds them.  (The straight-through gradient proper reads the rounded operands, g Q(W) and g^T Q(x); it
-        trained no better.)  (Acting in 4 bits and updating in float32 does not train: the
-        two policies differ by more than the PPO clip.)  Observations are rounded too: distances and flags of up to 4 are kept
-        but where larger numbers, a cooking pot's timer above all, share their block of 32 (`mxfp4`).  Heads stay in float32.  `rollout_step` reads the weights as
-        `refresh_rollout_heads` last quantised them; every other call quantises them anew."""
+        first layer of the centralised critic, whose weight is most of what a rollout step reads.  Heads stay in float32.
+
+        Updates train this policy: their forward pass is the same numbers.  Their backward pass is that of the unrounded
+        layers at the ReLU masks of the 4-bit ones, g W and g^T x with W and x as they were before the rounding, or with
+        `straight_through` that of the 4-bit layers with the roundings' derivatives taken as one, g Q(W) and g^T Q(x), which
+        finds hard tasks earlier and returns more there (`train` takes it).  The optimizer steps the unrounded weights, and a
+        checkpoint holds them.  (Acting in 4 bits and updating in float32 does not train: the two policies differ by more
+        than the PPO clip.)  Observations are rounded too: distances and flags of up to 4 are kept but where larger numbers,
+        a cooking pot's timer above all, share their block of 32 (`mxfp4`).
+
+        `rollout_step` reads the weights as `refresh_rollout_heads` last quantised them; every other call quantises them
+        anew, into the same storage: order it behind rollout steps on other streams as a change of the weights would be.
+        For the centralised critic's first layer that reads as much as the float32 product does: where its value is wanted
+        once a change of the weights, as without the fused sampler, 4 bits save nothing there."""
         if self._coarse is None:  # captured launches read the weights where they are
             self._coarse = {}
+        self._straight = bool(straight_through)
         return self
 
     def use_activation_checkpoints(self):
@@ -334,15 +360,19 @@ class Agent(nn.Module):
 
     def _kept_heads(self, x):
         """logits and value with every activation kept in 8 bits: both heads as one layer, so that the hidden layer is read once"""
-        kept = act8.compress(x)
-        codes, scales, nonnegative, h = kept.codes, kept.scales, False, x.contiguous()
+        kept = None if self._coarse is not None and self._straight else act8.compress(x)
+        codes, scales, nonnegative, h = getattr(kept, "codes", None), getattr(kept, "scales", None), False, x.contiguous()
         if x.shape[0] < _SMALL_ROWS:
             _announce_blas_switch_quietly(x)
         for name in ("network.0", "network.2"):
             layer = self.get_submodule(name)
             coarse = None if self._coarse is None else self._coarse_weight(name, layer, False)
             between = torch.float32 if name == "network.0" else None  # with 4-bit weights, as in _trunk
-            h, codes, scales = _KeptLinear.apply(h, codes, scales, nonnegative, layer.weight, layer.bias, True, coarse, between)
+            straight = coarse is not None and self._straight
+            if straight:
+                read = mxfp4.quantize(h)
+                codes, scales = read.codes, read.scales
+            h, codes, scales = _KeptLinear.apply(h, codes, scales, nonnegative, layer.weight, layer.bias, True, coarse, between, straight)
             nonnegative = True
         heads = _KeptLinear.apply(h, codes, scales, True, torch.cat([self.actor.weight, self.critic.weight]),
                                   torch.cat([self.actor.bias, self.critic.bias]), False)
@@ -367,7 +397,8 @@ class Agent(nn.Module):
             return _linear(c[4], _linear(c[2], _linear(c[0], joint_obs, True), True), False)
         rows = joint_obs if joint_obs.dim() == 2 else joint_obs.reshape(-1, joint_obs.shape[-1])
         coarse = self._coarse_weight("centralised_critics.0", c[0], fresh)
-        value = _linear(c[4], _linear(c[2], _linear(c[0], rows, True, coarse), True), False)
+        straight = self._straight and torch.is_grad_enabled()  # without gradients the product quantises its rows itself
+        value = _linear(c[4], _linear(c[2], _linear(c[0], rows, True, coarse, None, straight), True), False)
         return value if joint_obs.dim() == 2 else value.view(*joint_obs.shape[:-1], -1)
 
     def get_value(self, x, joint_obs=None):

@@ -67,7 +67,7 @@ def build_parser():
                    help="decentralised MAPPO on the GPU: loss and head gradients from one HIP pass instead of autograd's small ops")
     p.add_argument("--trunk-precision", choices=["float32", "mxfp4"], default="float32",
                    help="the policy's trunk in float32, or in 4-bit floating point (marl_amd.mxfp4): acting and updates, whose "
-                        "backward pass is that of the unrounded layers and steps the float32 weights")
+                        "gradients go straight through the roundings to the float32 weights")
     p.add_argument("--activation-bits", type=int, choices=[32, 8], default=32,
                    help="what an update keeps of the trunk's activations for its backward pass: float32, or 8 bits a value "
                         "(marl_amd.act8), a quarter of what is kept and two thirds of an update's peak")
@@ -127,7 +127,7 @@ def main(argv=None):
     if args.sampler == "fused":
         net.use_fused_sampling(args.seed, row_index_base=rank * args.num_envs * args.num_agents)
     if args.trunk_precision == "mxfp4":
-        net.use_mxfp4_trunk()
+        net.use_mxfp4_trunk(straight_through=True)
     if args.activation_bits == 8:
         net.use_activation_checkpoints()
     # main.py:294.  fused: the whole Adam step is one multi-tensor launch instead of seventeen

@@ -12,6 +12,10 @@ from marl_amd.env import make_env, make_vector_env  # noqa: E402
 from marl_amd.policy import Agent  # noqa: E402
 
 
+# "straight": the backward pass that reads the rounded operands, as `train` takes it
+TRUNKS = (("float32", 32), ("float32", 8), ("mxfp4", 8), ("mxfp4 straight", 32), ("mxfp4 straight", 8))
+
+
 def us(f, n):
     for _ in range(5):
         f()
@@ -47,8 +51,8 @@ def main():
     for M in (2048, 131072, 1048576):
         x = obs.repeat(-(-M // N), 1)[:M].contiguous()
         g = torch.randn(M, 8, device=dev) / M
-        for trunk, bits in (("float32", 32), ("float32", 8), ("mxfp4", 8)):
-            net._keep_in_8_bits, net._coarse = bits == 8, {} if trunk == "mxfp4" else None
+        for trunk, bits in TRUNKS:
+            net._keep_in_8_bits, net._coarse, net._straight = bits == 8, None if trunk == "float32" else {}, trunk == "mxfp4 straight"
 
             def update():
                 net.zero_grad(set_to_none=True)
@@ -75,8 +79,8 @@ def main():
     for M in (512, 2048, 16384, 65536):  # as updates of up to 65,536 samples run
         x = obs[:M].contiguous()
         g = torch.randn(M, 8, device=dev) / M
-        for trunk, bits in (("float32", 32), ("float32", 8), ("mxfp4", 8)):
-            net._keep_in_8_bits, net._coarse = bits == 8, {} if trunk == "mxfp4" else None
+        for trunk, bits in TRUNKS:
+            net._keep_in_8_bits, net._coarse, net._straight = bits == 8, None if trunk == "float32" else {}, trunk == "mxfp4 straight"
 
             def captured():
                 net.zero_grad(set_to_none=False)

@@ -44,8 +44,8 @@ def _learner(name, minibatch, trunk, bits, fused, graph):
     T = minibatch * 2 // (E * A)
     torch.manual_seed(3)
     net = Agent(Box(-1, 1, (101,)), Discrete(7), A, E, build_centralised=name == "CMAPPO").cuda()
-    if trunk == "mxfp4":
-        net.use_mxfp4_trunk()
+    if trunk != "float32":
+        net.use_mxfp4_trunk(straight_through=trunk == "straight")
     if bits == 8:
         net.use_activation_checkpoints()
     buf = Buffer(101, A, E, max_size=T, device="cuda")
@@ -63,7 +63,7 @@ def _learner(name, minibatch, trunk, bits, fused, graph):
 
 @pytest.mark.parametrize("name", ["MAPPO", "CMAPPO"])
 @pytest.mark.parametrize("fused", [True, False])
-@pytest.mark.parametrize("trunk,bits", [("float32", 32), ("mxfp4", 32), ("float32", 8), ("mxfp4", 8)])
+@pytest.mark.parametrize("trunk,bits", [("float32", 32), ("mxfp4", 32), ("float32", 8), ("mxfp4", 8), ("straight", 32), ("straight", 8)])
 @pytest.mark.parametrize("minibatch", [512, 2048, 65536])
 def test_no_memory_set_nodes(kept_graphs, name, fused, trunk, bits, minibatch):
     learner, _, obs = _learner(name, minibatch, trunk, bits, fused, True)
@@ -103,7 +103,7 @@ def test_no_memory_set_nodes_in_training(tmp_path, monkeypatch, flags):
         assert kinds["kernel"] > 0 and kinds["memset"] == 0, kinds
 
 
-@pytest.mark.parametrize("trunk,bits", [("float32", 32), ("mxfp4", 32), ("mxfp4", 8)])
+@pytest.mark.parametrize("trunk,bits", [("float32", 32), ("mxfp4", 32), ("mxfp4", 8), ("straight", 32), ("straight", 8)])
 def test_replays_between_eager_work_are_the_eager_steps(trunk, bits):
     got = []
     for graph in (False, True):

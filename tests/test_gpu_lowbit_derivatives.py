@@ -1,7 +1,11 @@
-"""Derivatives that the low-bit calls do not have are refused, not dropped."""
+"""Derivatives: those that the low-bit calls do not have are refused, not dropped; the 4-bit trunk's backward passes are what
+they are named."""
+import numpy as np
 import pytest
 import torch
 from torch.autograd import forward_ad
+
+import lowbit_reference as ref
 
 pytestmark = pytest.mark.gpu
 
@@ -54,3 +58,89 @@ def test_the_backward_pass_is_the_unrounded_layers():
             assert (got.double() - want).norm() <= 4e-6 * want.norm()  # float32 sums of up to 300 terms
             assert (got.double() - rounded).norm() > 0.01 * want.norm()  # 4 bits are off by more
         assert (b.grad.double() - cut.sum(0)).norm() <= 4e-6 * cut.sum(0).norm()
+
+
+def _obs(rows, d=202, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(rows, d, device="cuda", generator=g)
+    x = (x.abs() > 0.9).float() * (x * 1.3).round()
+    x[::3, 5] = 30.0  # a pot's timer: its neighbours round
+    return x
+
+
+@pytest.mark.parametrize("rows", [5, 600, 8192])
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_straight_through_backward_pass(rows, bits, dtype):
+    """that of relu(Q(x) Q(W)^T + b) with the roundings' derivatives taken as one, from the formats' definition in 64 bits"""
+    from marl_amd.policy import Agent
+    from marl_amd.spaces import Box, Discrete
+
+    torch.manual_seed(5)
+    net = Agent(Box(-1, 1, (202,)), Discrete(7), 2, 1, build_centralised=False).cuda().to(dtype).use_mxfp4_trunk(straight_through=True)
+    if bits == 8:
+        net.use_activation_checkpoints()
+    x = _obs(rows, seed=rows).to(dtype).requires_grad_()
+    d = lambda t: t.detach().double().cpu().numpy()  # noqa: E731
+    w0, w1 = (ref.mxfp4(d(net.network[k].weight))[2] for k in (0, 2))
+    h, read = d(x), []
+    for w in (w0, w1):  # zero biases
+        read.append(ref.mxfp4(h)[2])
+        h = np.maximum(read[-1] @ w.T, 0.0).astype(np.float32).astype(np.float64)
+        read.append(h)
+    out = h if dtype == torch.float32 else d(torch.from_numpy(h).to(dtype))
+    kept = ref.act8(out, True)[2] if bits == 8 else out
+    g = torch.randn(rows, 8, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).to(dtype)
+    gh, wh = d(g), np.concatenate([d(net.actor.weight), d(net.critic.weight)])
+    g1 = (gh @ wh) * (read[3] > 0)
+    g0 = (g1 @ w1) * (read[1] > 0)
+    want = {"heads.weight": gh.T @ kept, "network.2.weight": g1.T @ read[2], "network.2.bias": g1.sum(0),
+            "network.0.weight": g0.T @ read[0], "network.0.bias": g0.sum(0), "x": g0 @ w0}
+    logits, value = net.logits_and_value(x)
+    with torch.no_grad():
+        assert torch.equal(net._trunk(x), (net._trunk(x.detach()) if bits == 8 else torch.enable_grad()(net._trunk)(x)))
+    torch.autograd.backward([logits, value], [g[:, :7], g[:, 7:]])
+    got = {k: d(p.grad) for k, p in net.named_parameters()}
+    got["heads.weight"], got["x"] = np.concatenate([got.pop("actor.weight"), got.pop("critic.weight")]), d(x.grad)
+    # float32: sums through at most two products of up to 256 terms.  bfloat16: the gradient is rounded behind each layer (the two
+    # heads' before they are added), in the first layer's input gradient once more, and the result: at most five half steps.
+    close = 4e-6 if dtype == torch.float32 else 5 * 2.0 ** -8
+    for name, w in want.items():
+        assert np.linalg.norm(got[name] - w) <= close * np.linalg.norm(w) + 1e-12, name
+    if dtype == torch.float32 and rows > 5:  # the unrounded layers' are other numbers
+        other = ((gh @ wh) * (read[3] > 0)).T @ read[1]
+        assert np.linalg.norm(got["network.2.weight"] - other) > 0.01 * np.linalg.norm(other)
+
+
+def test_the_straight_through_backward_pass_of_the_centralised_critic():
+    from marl_amd.policy import Agent
+    from marl_amd.spaces import Box, Discrete
+
+    torch.manual_seed(5)
+    net = Agent(Box(-1, 1, (40,)), Discrete(7), 2, 8).cuda().use_mxfp4_trunk(straight_through=True)
+    x = _obs(16, 40)
+    joint = x.view(1, -1).clone().requires_grad_()
+    c = net.centralised_critics
+    value = net.get_value(x, joint_obs=joint)
+    with torch.no_grad():
+        assert torch.equal(net.get_value(x, joint_obs=joint), value)
+    value.sum().backward()
+    d = lambda t: t.detach().double().cpu().numpy()  # noqa: E731
+    xq, wq = ref.mxfp4(d(joint))[2], ref.mxfp4(d(c[0].weight))[2]
+    h0 = np.maximum(xq @ wq.T + d(c[0].bias), 0.0)
+    h1 = np.maximum(h0 @ d(c[2].weight).T + d(c[2].bias), 0.0)
+    g0 = ((d(c[4].weight) * (h1 > 0)) @ d(c[2].weight)) * (h0 > 0)
+    for got, want in ((c[0].weight.grad, g0.T @ xq), (joint.grad, g0 @ wq)):
+        assert np.linalg.norm(d(got) - want) <= 4e-6 * np.linalg.norm(want)  # float32 sums of up to 512 terms
+
+
+def test_the_command_trains_straight_through(monkeypatch, tmp_path):
+    from marl_amd import train
+    from marl_amd.policy import Agent
+
+    asked = []
+    use = Agent.use_mxfp4_trunk
+    monkeypatch.setattr(Agent, "use_mxfp4_trunk", lambda self, *a, **kw: (asked.append((a, kw)), use(self, *a, **kw))[1])
+    train.main(["--num-agents", "2", "--num-envs", "16", "--layout", "overcooked_cramped_room_v0", "--num-steps", "32", "--total-steps", "2048",
+                "--ppo-epoch", "1", "--max-steps", "50", "--data-path", str(tmp_path), "--seed", "3", "--trunk-precision", "mxfp4"])
+    assert asked == [((), {"straight_through": True})]
