@@ -4,7 +4,7 @@ SEEDS=1 STEPS=5000000 bash results/run_reference_recipes.sh 2>&1 | tail -4
 python - <<'PY'
 import glob
 import numpy as np
-for d in ("r02_makefile_cramped", "r02_readme_cramped", "r02_makefile_forced"):
+for d in ("float32_makefile_cramped", "float32_readme_cramped", "float32_makefile_forced"):
     for f in sorted(glob.glob("gpurun_out/results/%s/*return*" % d))[:1]:
         x = np.loadtxt(f, skiprows=1)
         print(d, len(x), "episodes, mean return of the last 10: %.2f" % x[-10:].mean())
