@@ -2,7 +2,7 @@
 
 Autograd keeps every layer's float32 input until its backward pass: at 8.4 million samples a minibatch (131,072 envs)
 the trunk's inputs and outputs (202 + 512 + 256 values a sample) are 33 GB.  Here they are kept as one byte a value and
-one scale byte per 32, a quarter of that (an update's peak, with its gradients in flight, falls by a third), and the
+one scale byte per 32, a quarter of that (an update's peak, with its gradients in flight, falls by three tenths), and the
 backward pass reads them as they are: a code times a power of two is exactly a bfloat16, so the weight gradient takes it
 straight into the bf16 matrix cores while the gradient itself goes in with all its bits.  What the ReLU of a layer let through is read off its kept output's codes, exactly.
 """

@@ -70,7 +70,7 @@ def build_parser():
                         "gradients go straight through the roundings to the float32 weights")
     p.add_argument("--activation-bits", type=int, choices=[32, 8], default=32,
                    help="what an update keeps of the trunk's activations for its backward pass: float32, or 8 bits a value "
-                        "(marl_amd.act8), a quarter of what is kept and two thirds of an update's peak")
+                        "(marl_amd.act8), a quarter of what is kept and seven tenths of an update's peak")
     p.add_argument("--env-shards", type=int, default=1,
                    help="run the envs of a rank as this many shards on HIP streams of their own; with the decentralised "
                         "critic and the fused sampler every shard then runs act -> step on its stream and one shard's "

@@ -35,6 +35,8 @@ FORMS = [
     ("grad_1048576x8x256", 1048576, 256, 8, "float32", "plain"),
     ("grad_131072x1024x1024", 131072, 1024, 1024, "float32", "plain"),
     ("grad_131072x2048x2048", 131072, 2048, 2048, "float32", "plain"),
+    ("sums_2048x512", 2048, 512, 0, "float32", "plain"),
+    ("sums_131072x512", 131072, 512, 0, "float32", "plain"),
 ]
 
 
@@ -46,7 +48,9 @@ def form(name, rows, cols, out, kind, what):
     for k in range(3):
         g = torch.Generator(device="cuda").manual_seed(k)
         rand = lambda *shape: torch.randn(*shape, device="cuda", generator=g)  # noqa: E731
-        if name.startswith("grad"):
+        if name.startswith("sums"):
+            calls.append(lambda x=rand(rows, cols): act8.column_sums(x))
+        elif name.startswith("grad"):
             act, grad = act8.compress(torch.relu(rand(rows, cols)), nonnegative=True), rand(rows, out).to(getattr(torch, kind))
             mask = None if what == "plain" else act8.compress(torch.relu(rand(rows, out)), nonnegative=True)
             calls.append(lambda a=act, g=grad, m=mask: act8.weight_grad(g, a, m, want_masked=what == "kept"))
@@ -93,7 +97,7 @@ def summary(path, names):
         name = r["Kernel_Name"]
         if "spin_kernel" in name and r["Dispatch_Id"] not in marks:  # a counter file has a line for each counter
             marks.append(r["Dispatch_Id"])
-        if len(marks) % 2 == 0 or not ("mx_" in name or "act_" in name):
+        if len(marks) % 2 == 0 or not any(k in name for k in ("mx_", "act_", "column_sums")):
             continue
         case, name = names[len(marks) // 2], name.split("(")[0].replace("void ", "")
         if "Counter_Name" in r:

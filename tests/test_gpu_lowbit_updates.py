@@ -208,3 +208,10 @@ def test_the_peak_of_an_update():
     # the splits' sums, at most 256 tiles of 128 x 256.
     assert kept <= rows * ((202 + 512 + 256) * 34 / 32 + (256 + 256 + 512) * 4 + 4 * 8 * 4) + 256 * 128 * 257 * 4 + (8 << 20)
     assert kept <= 0.75 * wide
+    # Straight through the 4-bit trunk: 17 bytes for 32 values of the observations and of the first hidden layer more (the observations
+    # in 8 bits are not kept then).  With float32 activations the second layer's input, as large as its gradient, is there while the
+    # weight's gradient is formed, beside the 128 slabs that that adds up; otherwise the slabs are gone before the peak.
+    trunk = _agent().use_mxfp4_trunk(straight_through=True)
+    assert _update_peak(trunk, rows) <= wide + rows * (202 + 512) * 18 / 32 + 128 * 256 * 512 * 4 + (32 << 20)
+    trunk.use_activation_checkpoints()
+    assert _update_peak(trunk, rows) <= kept + rows * (202 + 512) * 18 / 32 + (32 << 20)
