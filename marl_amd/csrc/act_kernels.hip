@@ -186,13 +186,15 @@ __device__ __forceinline__ uint32_t load_four_bytes(const uint8_t* p, uint32_t a
 // A column of the tile lies in LDS at (column % 4) * (columns / 4) + column / 4, so that the lanes of a wave, which take
 // four neighbouring columns each, write to neighbouring places, and a lane's results are four neighbouring inputs.
 //
-// 131072 rows x 256 outputs x 512 inputs, float32 gradient with a mask: 116 us and 6 us for the joining kernel (bfloat16, one
-// product, 75 and 6).  237 MB come from HBM once and 168 MB go there, 78 us at a copy's rate; three bf16 products take 85 us at
+// 131072 rows x 256 outputs x 512 inputs, float32 gradient with a mask that is written: 117 us and 6 us for the joining kernel (float16, two
+// products, 108; bfloat16, one, 89, without a mask 69).  The float32 form has 256 registers and 12 bytes of scratch a thread; without
+// the written gradient it has none, and takes 119 us instead of 137 at 131072 x 512 x 202.  237 MB come from HBM once and 168 MB go there, 78 us at a copy's rate; three bf16 products take 85 us at
 // the rate of a large library product, 41 us at the matrix units' own.  Those are busy 37 % of the time and the vector units as
 // long; g and x reach the compute units twice, 470 MB at 4.1 TB/s, which is what loads alone in this order reach (4.5).
 // Measured and no faster, 118 to 137 us: 1024 threads; waves that only load and convert before waves that only multiply, over
 // three buffers; loads three and four steps ahead; a quarter fewer vector instructions; fewer output features to the waves that
 // convert g.  Two workgroups a compute unit double the partial sums (34 MB): 10 us more.
+// Not tried: 128 x 512, which would read g and its mask once and x twice (306 MB instead of 470).
 template <int TYPE, int BO, int BI, int WO, int WI, int MASK, bool NARROW>
 struct WeightGrad {
     static constexpr int PARTS = grad_parts<TYPE>(), BYTES = TYPE == MARL_F32 ? 4 : 2;
@@ -524,7 +526,8 @@ act_join_kernel(const float* __restrict__ part_w, const float* __restrict__ part
 //   column over workgroups clears its counters with a memory-set call, and such a node of a captured graph does not do its work in
 //   every replay; nothing here needs clearing.)
 // A thread has four neighbouring columns of every (256 / groups)-th row of its split, sums in float32, a workgroup's threads are added
-// in order in double, the splits by act_join_kernel.  Bound by memory where rows are many.
+// in order in double, the splits by act_join_kernel.  Bound by memory where rows are many: 131072 x 512 float32 values in 50 us, 5.4 TB/s
+// (the library's sum 89); 2048 x 512 in 5.6 us, two launches (11).
 
 template <int TYPE>
 __global__ void __launch_bounds__(256)
@@ -595,6 +598,9 @@ static SumsCut sums_cut(int64_t rows, int cols) {
 //     202: 24.5, with small tiles 28.5), else 64 x 64 on two with 4 steps (2048 x 512 x 202: 14.5; 2 steps 18.5, 8 steps 15.8),
 //     and for inputs that one of those covers: the gradient is then read once, and x, the smaller operand, once for every 64 outputs
 //     (131072 x 512 x 40: 123 and 132, without a mask x 64: 81 and 107; with two of them it is slower, x 96: 186 and 134)
+// Two sizes are slow, though right: 17 to 64 outputs of more than 64 inputs multiply outputs that are not there (131072 x 20 x 512: 52
+// us, 15 of bytes), and weights of so many tiles that there are fewer than eight splits leave XCDs without work, since a split's tiles
+// stay on one (131072 x 2048 x 2048, two splits: 10.6 ms; 1024 x 1024, eight: 0.8).
 struct ActCut { int bo, bi, splits; int64_t grid; };
 static ActCut act_cut(int64_t rows, int out, int cols) {
     ActCut c;

@@ -222,7 +222,7 @@ __device__ __forceinline__ void raw_use(const MxRaw<TYPE>& raw, float (&v)[8]) {
 }
 
 // Workgroups on a compute unit.  Two where a wave has two tiles of features, and for MXFP4 results of float rows, which are small and
-// leave the quantising, if the registers suffice (131072 x 202 -> 512 in float32: 48 against 41 us; not with 16 blocks a row, 59
+// leave the quantising, if the registers suffice (131072 x 202 -> 512 in float32: 48 against 42 us; not with 16 blocks a row, 59
 // and 65 us, nor with the 64 rows that two waves side by side have, 24 and 28).  Elsewhere two read the weight twice and are slower
 // (131072 x 512 -> 256 from MXFP4 to MXFP4 27 and 35 us).
 constexpr int mx_workgroups(int ks, int in, int out, int wn, int nt) {
@@ -460,7 +460,7 @@ mx_few_rows_kernel(MxLinear P) {
 
 // More rows of any length: 64 features and 64 rows to a workgroup, whose four waves take every fourth stretch of 512 values
 // each and add their sums through LDS; with few workgroups the row is split over them too (grid z).  Fragments come straight
-// from the caches, four waves reading the same lines: 4096 x 4096 -> 4096 in 155 us, 0.9 PFLOP/s.
+// from the caches, four waves reading the same lines: 4096 x 4096 -> 4096 in 165 us, 0.83 PFLOP/s.
 constexpr int MX_RM = 4;  // groups of 16 rows
 template <int OUT>
 __global__ void __launch_bounds__(256, 2)
