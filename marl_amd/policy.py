@@ -43,8 +43,11 @@ def _weight_grad(gy, x):
 
 
 def _bias_grad(gy):
-    """gy.sum(0), from launches that replay (`act8.column_sums`): updates of small minibatches are captured"""
-    return act8.column_sums(gy).to(gy.dtype) if gy.is_cuda and gy.dtype in act8._TYPES else gy.sum(0)
+    """gy.sum(0), from launches that replay (`act8.column_sums`): updates of small minibatches are captured.  Where the
+    backward pass itself is differentiated it is torch's sum, which has a derivative."""
+    if not gy.is_cuda or gy.dtype not in act8._TYPES or torch.is_grad_enabled():
+        return gy.sum(0)
+    return act8.column_sums(gy).to(gy.dtype)
 
 
 # Below 512 rows (the reference's batch sizes: 16 envs x 2 agents = 32 rows per rollout step)
@@ -186,36 +189,50 @@ class _LinearReLU(torch.autograd.Function):
     batches where that call is slow a plain product plus in-place bias and ReLU; the backward
     pass forms the weight gradient with `_weight_grad`.  With `coarse`, the weight in 4 bits, the forward pass is
     `mxfp4.linear`'s, its result in `out_dtype`, and the backward pass is the unrounded layer's: its input and weight as they
-    were before they went to 4 bits, the ReLU's mask that of the 4-bit result.  With `straight` it is the 4-bit layer's with
-    the roundings' derivatives taken as one: it reads input and weight as the product did, and keeps the input in 4 bits."""
+    were before they went to 4 bits, the ReLU's mask that of the 4-bit result."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, relu, coarse=None, out_dtype=None, straight=False):
-        ctx.relu, ctx.cols, ctx.dtype = relu, x.shape[1] if straight else None, weight.dtype
-        if straight:
-            kept = mxfp4.quantize(x)
-            out = _forward(kept, weight, bias, relu, coarse, out_dtype)
-            back = coarse.dequantize(weight.dtype) if ctx.needs_input_grad[0] else None
-            ctx.save_for_backward(kept.codes, kept.scales, back, out if relu else None)
-        else:
-            out = _forward(x, weight, bias, relu, coarse, out_dtype)
-            ctx.save_for_backward(x.to(weight.dtype), weight, out if relu else None)
+    def forward(ctx, x, weight, bias, relu, coarse=None, out_dtype=None):
+        out = _forward(x, weight, bias, relu, coarse, out_dtype)
+        ctx.relu = relu
+        ctx.save_for_backward(x.to(weight.dtype), weight, out if relu else None)
         return out
 
     @staticmethod
     def backward(ctx, gy):
-        if ctx.cols is None:
-            x, weight, out = ctx.saved_tensors
-        else:
-            codes, scales, weight, out = ctx.saved_tensors
-            x = mxfp4.MXFP4(codes, scales, ctx.cols).dequantize(ctx.dtype)
+        x, weight, out = ctx.saved_tensors
+        if ctx.relu:
+            gy = torch.ops.aten.threshold_backward(gy, out, 0)
+        gy = gy.contiguous().to(weight.dtype)
+        gw, gb = _weight_grad(gy, x), _bias_grad(gy)
+        gx = gy @ weight if ctx.needs_input_grad[0] else None
+        return gx, gw, gb, None, None, None
+
+
+class _StraightLinear(torch.autograd.Function):
+    """`_LinearReLU` with a weight in 4 bits whose backward pass is the 4-bit layer's, with the roundings' derivatives taken as
+    one: it reads input and weight as the product did, and keeps the input in 4 bits."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, relu, coarse, out_dtype=None):
+        kept = mxfp4.quantize(x)
+        out = _forward(kept, weight, bias, relu, coarse, out_dtype)
+        ctx.relu, ctx.cols, ctx.dtype = relu, x.shape[1], weight.dtype
+        back = coarse.dequantize(weight.dtype) if ctx.needs_input_grad[0] else None
+        ctx.save_for_backward(kept.codes, kept.scales, back, out if relu else None)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        codes, scales, back, out = ctx.saved_tensors
         if ctx.relu:
             gy = torch.ops.aten.threshold_backward(gy, out, 0)
         gy = gy.contiguous().to(ctx.dtype)
-        gw, gb = _weight_grad(gy, x), _bias_grad(gy)
-        del x  # the values of kept codes are gone before there is a gradient of their size
-        gx = gy @ weight if ctx.needs_input_grad[0] else None
-        return gx, gw, gb, None, None, None, None
+        # the input's values are gone before there is a gradient of their size
+        gw = _weight_grad(gy, mxfp4.MXFP4(codes, scales, ctx.cols).dequantize(ctx.dtype))
+        gb, gx = _bias_grad(gy), gy @ back if ctx.needs_input_grad[0] else None
+        return gx, gw, gb, None, None, None
 
 
 class _KeptLinear(torch.autograd.Function):
@@ -260,7 +277,7 @@ def _linear(layer: nn.Linear, x, relu, coarse=None, out_dtype=None, straight=Fal
     if x.is_cuda and x.dim() == 2:
         if x.shape[0] < _SMALL_ROWS and coarse is None:
             _announce_blas_switch_quietly(x)
-        return _LinearReLU.apply(x.contiguous(), layer.weight, layer.bias, relu, coarse, out_dtype, straight)
+        return (_StraightLinear if straight else _LinearReLU).apply(x.contiguous(), layer.weight, layer.bias, relu, coarse, out_dtype)
     out = layer(x)
     return torch.relu(out) if relu else out
 

@@ -144,3 +144,35 @@ def test_the_command_trains_straight_through(monkeypatch, tmp_path):
     train.main(["--num-agents", "2", "--num-envs", "16", "--layout", "overcooked_cramped_room_v0", "--num-steps", "32", "--total-steps", "2048",
                 "--ppo-epoch", "1", "--max-steps", "50", "--data-path", str(tmp_path), "--seed", "3", "--trunk-precision", "mxfp4"])
     assert asked == [((), {"straight_through": True})]
+
+
+def _first(layer, tensors):
+    """leaves and the squared gradients, which can be differentiated again"""
+    x, w, b, v = (t.clone().requires_grad_() for t in tensors)
+    out = (layer(x, w, b) * v).sum(1).square().sum()
+    return (x, w, v), sum(f.square().sum() for f in torch.autograd.grad(out, (w, b), create_graph=True))
+
+
+def _leaves():
+    g = torch.Generator(device="cuda").manual_seed(1)
+    return [torch.randn(*shape, device="cuda", generator=g) for shape in ((700, 40), (30, 40), (30,), (1, 30))]
+
+
+def test_second_derivatives_of_a_float32_layer():
+    from marl_amd import policy
+
+    pairs = []
+    for layer, tensors in ((lambda x, w, b: policy._LinearReLU.apply(x, w, b, True), _leaves()),
+                           (lambda x, w, b: torch.relu(x @ w.t() + b), [t.double() for t in _leaves()])):
+        leaves, squares = _first(layer, tensors)
+        pairs.append(torch.autograd.grad(squares, leaves))
+    for a, b in zip(*pairs):
+        assert (a.double() - b).norm() <= 1e-5 * b.norm()  # float32, six products and sums of up to 700 terms in a row
+
+
+def test_a_straight_through_pass_has_no_second_derivatives():
+    from marl_amd import mxfp4, policy
+
+    _, squares = _first(lambda x, w, b: policy._StraightLinear.apply(x, w, b, True, mxfp4.quantize(w)), _leaves())
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        squares.backward()
