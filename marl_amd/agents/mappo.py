@@ -145,7 +145,10 @@ class MAPPO:
                 if self._mean_target is None or self._mean_target.shape != b_value_target.shape:
                     self._mean_target = torch.empty_like(b_value_target)
                 targets = b_value_target[mb]
-                mean = targets.mean() if targets.numel() <= 65536 or not targets.is_cuda else column_sums(targets.view(-1, 1)) / targets.numel()
+                if self._graph_update and targets.numel() > 65536:
+                    mean = column_sums(targets.view(-1, 1)) / targets.numel()
+                else:
+                    mean = targets.mean()
                 self._mean_target.index_copy_(0, mb, mean.expand(mb.numel()))
                 b_value_target = self._mean_target
             loss, stats = ppo_loss(logits, newvalue, mb, b_actions_f, b_logprobs, b_advantages, b_value_target,

@@ -60,7 +60,8 @@ def build_parser():
     p.add_argument("--sampler", choices=["fused", "torch"], default="fused",
                    help="rollout action sampling: one HIP launch with a counter RNG, or torch.distributions")
     p.add_argument("--graph-update", choices=["auto", "on", "off"], default="auto",
-                   help="replay the PPO minibatch step from a hipGraph (auto: single rank and minibatches of at most 65,536 samples)")
+                   help="replay the PPO minibatch step from a hipGraph (auto: single rank and minibatches of at most 65,536 samples; "
+                        "with the autograd loss no larger ones are captured)")
     p.add_argument("--adam", choices=["fused", "foreach"], default="fused",
                    help="Adam step as one multi-tensor launch (GPU only) or PyTorch's default per-operation launches")
     p.add_argument("--fused-loss", choices=["on", "off"], default="on",
